@@ -65,6 +65,36 @@ class TinyModelConfig(C.Structure):
                [("eps", _f32)]
 
 
+class XentParams(C.Structure):
+    _fields_ = [(n, _u32) for n in ("T", "V", "D", "ldx", "ldw", "lddx", "lddw")] + \
+               [("w_vocab_major", _i32), ("grads_bf16", _i32), ("scale", _f32)]
+
+
+ROPE_MAX_PAIRS = 128
+ROPE_SCALING = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("rotary_dim", _u32), ("scaling", _i32)] + \
+               [(n, C.c_double) for n in ("base", "factor", "context", "low", "high")] + [("amplitude", _f32)]
+
+
+class RopeTable(C.Structure):
+    _fields_ = [("pairs", _u32), ("amplitude", _f32), ("turns", _u64 * ROPE_MAX_PAIRS)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [(n, _u32) for n in ("tokens", "heads_q", "heads_k", "head_dim", "ldq", "ldk", "ldq_out",
+                                    "ldk_out", "seq")] + \
+               [(n, _i32) for n in ("pos0", "interleaved", "inverse", "head_major_in", "head_major_out")]
+
+
+class JunctionParams(C.Structure):
+    _fields_ = [(n, _u32) for n in ("rows", "cols", "ldh", "ldb", "ldy", "ldgate", "gate_rows")] + \
+               [("norm_after", _i32)] + \
+               [(n, _f32) for n in ("scale_h", "scale_b", "eps_post", "eps_pre")]
+
+
 class Arena(C.Structure):
     _fields_ = [("buffer", _vp), ("capacity", _sz), ("offset", _sz)]
 
@@ -105,6 +135,20 @@ _SIGS = {
     "bwpp_cuda_reduce_sum_f32": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, C.c_int]),
     "bwpp_cuda_broadcast_f32": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, C.c_int]),
     "bwpp_cuda_cast_f32_bf16": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32]),
+    "bwpp_cuda_xent_workspace_size": (_sz, [C.POINTER(XentParams), _i32]),
+    "bwpp_cuda_xent_fwd_bf16": (_i32, [_vp] * 6 + [C.POINTER(XentParams)]),
+    "bwpp_cuda_xent_bwd_bf16": (_i32, [_vp] * 8 + [C.POINTER(XentParams)]),
+    "bwpp_cuda_rope_table": (_i32, [C.POINTER(RopeTable), C.POINTER(RopeConfig)]),
+    "bwpp_cuda_rope_bf16": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), C.POINTER(RopeParams)]),
+    "bwpp_cuda_rope_f16": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), C.POINTER(RopeParams)]),
+    "bwpp_cuda_rope_f32": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), C.POINTER(RopeParams)]),
+    "bwpp_cuda_junction_fwd_f32": (_i32, [_vp] * 8 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_junction_fwd_bf16": (_i32, [_vp] * 8 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_junction_fwd_f16": (_i32, [_vp] * 8 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_junction_bwd_workspace_size": (_sz, [_vp, _u32, _u32, _u32]),
+    "bwpp_cuda_junction_bwd_f32": (_i32, [_vp] * 13 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_junction_bwd_bf16": (_i32, [_vp] * 13 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_junction_bwd_f16": (_i32, [_vp] * 13 + [C.POINTER(JunctionParams)]),
     "bwpp_cuda_comm_unique_id": (_i32, [_vp]),
     "bwpp_cuda_comm_create": (_i32, [C.POINTER(_vp), _vp, _i32, _i32, _i32]),
     "bwpp_cuda_comm_allreduce_sum_f32": (_i32, [_vp, _vp, _sz, _vp]),
@@ -345,6 +389,92 @@ class Ctx:
     def cast_f32_bf16(self, src, dst, rows, cols, ld_src):
         self.check(self.lib.bwpp_cuda_cast_f32_bf16(self.handle, _ptr(src), _ptr(dst), rows, cols, ld_src),
                    "cast_f32_bf16")
+
+    # training-step operators around a decoder block
+    def xent_fwd(self, x, w, target, loss, lse, T, V, D, ldx, ldw, w_vocab_major=0, scale=1.0):
+        p = XentParams(T, V, D, ldx, ldw, 0, 0, int(w_vocab_major), 0, float(scale))
+        self.check(self.lib.bwpp_cuda_xent_fwd_bf16(self.handle, _ptr(x), _ptr(w), _ptr(target), _ptr(loss),
+                                                    _ptr(lse), C.byref(p)), "xent_fwd")
+
+    def xent_bwd(self, x, w, target, lse, dloss, dx, dw, T, V, D, ldx, ldw, lddx, lddw, w_vocab_major=0,
+                 scale=1.0, grads_bf16=0):
+        p = XentParams(T, V, D, ldx, ldw, lddx, lddw, int(w_vocab_major), int(grads_bf16), float(scale))
+        self.check(self.lib.bwpp_cuda_xent_bwd_bf16(self.handle, _ptr(x), _ptr(w), _ptr(target), _ptr(lse),
+                                                    _ptr(dloss), _ptr(dx), _ptr(dw), C.byref(p)), "xent_bwd")
+
+    def _rope(self, fn, q, k, q_out, k_out, table, tokens, heads_q, heads_k, head_dim, ldq, ldk, ldq_out,
+              ldk_out, positions=None, seq=0, pos0=0, interleaved=0, inverse=0, head_major_in=0,
+              head_major_out=0):
+        p = RopeParams(tokens, heads_q, heads_k, head_dim, ldq, ldk, ldq_out, ldk_out, seq, pos0,
+                       int(interleaved), int(inverse), int(head_major_in), int(head_major_out))
+        self.check(fn(self.handle, _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(positions),
+                      C.byref(table), C.byref(p)), "rope")
+
+    def rope_bf16(self, *args, **kw):
+        self._rope(self.lib.bwpp_cuda_rope_bf16, *args, **kw)
+
+    def rope_f16(self, *args, **kw):
+        self._rope(self.lib.bwpp_cuda_rope_f16, *args, **kw)
+
+    def rope_f32(self, *args, **kw):
+        self._rope(self.lib.bwpp_cuda_rope_f32, *args, **kw)
+
+    def _junction_params(self, rows, cols, gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre,
+                         ldh, ldb, ldy, ldgate):
+        return JunctionParams(rows, cols, ldh or cols, ldb or cols, ldy or cols, ldgate or cols, gate_rows,
+                              int(norm_after), scale_h, scale_b, eps_post, eps_pre)
+
+    def _junction_fwd(self, fn, h, b, gain_post, gate, gain_pre, h_out, y, rows, cols, gate_rows=0,
+                      norm_after=1, scale_h=1.0, scale_b=1.0, eps_post=1e-5, eps_pre=1e-5, ldh=0, ldb=0,
+                      ldy=0, ldgate=0):
+        p = self._junction_params(rows, cols, gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre,
+                                  ldh, ldb, ldy, ldgate)
+        self.check(fn(self.handle, _ptr(h), _ptr(b), _ptr(gain_post), _ptr(gate), _ptr(gain_pre),
+                      _ptr(h_out), _ptr(y), C.byref(p)), "junction_fwd")
+
+    def _junction_bwd(self, fn, h_out, b, gain_post, gate, gain_pre, dh_out, dy, dh, db, dgain_post, dgate,
+                      dgain_pre, rows, cols, gate_rows=0, norm_after=1, scale_h=1.0, scale_b=1.0,
+                      eps_post=1e-5, eps_pre=1e-5, ldh=0, ldb=0, ldy=0, ldgate=0):
+        p = self._junction_params(rows, cols, gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre,
+                                  ldh, ldb, ldy, ldgate)
+        self.check(fn(self.handle, _ptr(h_out), _ptr(b), _ptr(gain_post), _ptr(gate), _ptr(gain_pre),
+                      _ptr(dh_out), _ptr(dy), _ptr(dh), _ptr(db), _ptr(dgain_post), _ptr(dgate),
+                      _ptr(dgain_pre), C.byref(p)), "junction_bwd")
+
+    def junction_fwd_f32(self, *args, **kw):
+        self._junction_fwd(self.lib.bwpp_cuda_junction_fwd_f32, *args, **kw)
+
+    def junction_fwd_bf16(self, *args, **kw):
+        self._junction_fwd(self.lib.bwpp_cuda_junction_fwd_bf16, *args, **kw)
+
+    def junction_fwd_f16(self, *args, **kw):
+        self._junction_fwd(self.lib.bwpp_cuda_junction_fwd_f16, *args, **kw)
+
+    def junction_bwd_f32(self, *args, **kw):
+        self._junction_bwd(self.lib.bwpp_cuda_junction_bwd_f32, *args, **kw)
+
+    def junction_bwd_bf16(self, *args, **kw):
+        self._junction_bwd(self.lib.bwpp_cuda_junction_bwd_bf16, *args, **kw)
+
+    def junction_bwd_f16(self, *args, **kw):
+        self._junction_bwd(self.lib.bwpp_cuda_junction_bwd_f16, *args, **kw)
+
+
+def xent_workspace_size(T, V, D, ldx, ldw, w_vocab_major=0, backward=0, grads_bf16=0) -> int:
+    """Scratch bytes of Ctx.xent_fwd (backward=0) or Ctx.xent_bwd (backward=1)."""
+    p = XentParams(T, V, D, ldx, ldw, 0, 0, int(w_vocab_major), int(grads_bf16), 1.0)
+    return load().bwpp_cuda_xent_workspace_size(C.byref(p), int(backward))
+
+
+def rope_table(rotary_dim, base=10000.0, scaling="none", factor=1.0, context=0.0, low=1.0, high=32.0,
+               amplitude=1.0) -> RopeTable:
+    """The rotary frequencies of one model configuration, for Ctx.rope_*."""
+    cfg = RopeConfig(rotary_dim, ROPE_SCALING[scaling], base, factor, context, low, high, amplitude)
+    table = RopeTable()
+    rc = load().bwpp_cuda_rope_table(C.byref(table), C.byref(cfg))
+    if rc != OK:
+        raise BwppError(rc, f"rope_table: {status_string(rc)}")
+    return table
 
 
 class Plan:

@@ -60,6 +60,18 @@ int bwpp_ctx_enter(BwppCudaCtx *ctx);
 // grown: a too-small one is an error).  NULL on failure (error recorded).
 void *bwpp_ctx_workspace(BwppCudaCtx *ctx, size_t bytes);
 
+// Whether ctx's stream is being captured into a graph (true as well where the
+// stream cannot be asked, as the legacy stream while another stream captures).
+bool bwpp_ctx_capturing(BwppCudaCtx *ctx);
+
+// `bytes` of ctx scratch at a 256-byte boundary, BWPP_OP_SCRATCH_PAD of them
+// for the alignment (callers' size queries add it).  A captured graph keeps
+// the address, and ctx-owned scratch may move when a later call grows it, so
+// a call under capture needs a caller's workspace: without one it is refused
+// (BWPP_CUDA_ERR_UNSUPPORTED, nothing allocated).
+#define BWPP_OP_SCRATCH_PAD 256
+int bwpp_op_scratch(BwppCudaCtx *ctx, size_t bytes, const char *what, uint8_t **out);
+
 // Launch-error check after a kernel launch.
 #define BWPP_LAUNCH_CHECK(ctx, name)                                        \
   do {                                                                     \

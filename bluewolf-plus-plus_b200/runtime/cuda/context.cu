@@ -75,6 +75,28 @@ void *bwpp_ctx_workspace(BwppCudaCtx *ctx, size_t bytes) {
   return ctx->workspace;
 }
 
+bool bwpp_ctx_capturing(BwppCudaCtx *ctx) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return true;
+  }
+  return st != cudaStreamCaptureStatusNone;
+}
+
+int bwpp_op_scratch(BwppCudaCtx *ctx, size_t bytes, const char *what, uint8_t **out) {
+  *out = NULL;
+  if (!ctx->user_workspace && bwpp_ctx_capturing(ctx))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED,
+                          "%s: a captured call needs a caller's workspace of %zu bytes "
+                          "(bwpp_cuda_ctx_set_workspace)",
+                          what, bytes + BWPP_OP_SCRATCH_PAD);
+  void *p = bwpp_ctx_workspace(ctx, bytes + BWPP_OP_SCRATCH_PAD);
+  if (!p) return BWPP_CUDA_ERR_NOMEM;
+  *out = (uint8_t *)(((uintptr_t)p + 255) & ~(uintptr_t)255);
+  return BWPP_CUDA_OK;
+}
+
 static bwpp_encode_tiled_fn g_encode = NULL;
 
 bwpp_encode_tiled_fn bwpp_get_encode_tiled(void) {

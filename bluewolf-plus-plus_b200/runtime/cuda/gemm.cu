@@ -862,8 +862,11 @@ inline bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) 
 // slot takes two of them; a launch uses at most cap slots) and, per slot, an
 // (arrived, written) pair of 64-bit class counters for each of the 2 CTAs x
 // 8 epilogue warps.  Allocated on first use; never when the caller owns the
-// workspace (then GEMMs use the half-tile tail).
+// workspace (then GEMMs use the half-tile tail), nor for a captured launch:
+// the counters are told apart by a tag that is an argument of the launch, and
+// a graph's second replay would come with the tag of its first.
 bool gemm_scratch(BwppCudaCtx *ctx) {
+  if (bwpp_ctx_capturing(ctx)) return false;
   if (ctx->gemm_partials) return true;
   if (ctx->user_workspace || ctx->gemm_scratch_failed) return false;
   const size_t slots = 2 * (size_t)ctx->num_sms;

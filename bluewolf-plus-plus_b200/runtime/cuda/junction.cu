@@ -1,0 +1,724 @@
+// The junction between two blocks of a decoder, forward and gradient: the
+// norm after a block, its gate and the scaled residual sum, and the norm
+// before the next block, in one pass over the rows.
+//
+//   u  = b / rms(b) * gain_post  (norm_after; else u = b)
+//   h' = scale_h h + scale_b gate u
+//   y  = h' / rms(h') * gain_pre            rms(x) = sqrt(mean(x^2) + eps)
+//
+// Gradient, with g = gain_pre dy, hat = h' / rms(h'), bhat = b / rms(b):
+//   dH = dh' + (g - hat mean(g hat)) / rms(h')
+//   dh = scale_h dH,  e = scale_b dH,  dgate = sum e u,  du = gate e
+//   db = (gain_post du - bhat mean(gain_post du bhat)) / rms(b)
+//   dgain_post = sum du bhat,  dgain_pre = sum dy hat
+// The statistics are recomputed from the rows, which are read anyway.
+//
+// h, h', gains and gates are fp32; b, y, db, dy are fp32, bf16 or f16.  All
+// arithmetic is fp32; y and db are rounded once.  HBM-bound: a row is held in
+// registers, read once and written once.
+//
+// Column sums (deterministic): a CTA walks a chunk of consecutive rows that
+// share one gate row and keeps sum e bhat (or sum e b) and sum dy hat of its
+// columns in registers, then writes one partial row per chunk.  A second
+// kernel adds the partial rows in a fixed order: dgain_post weights each
+// with its chunk's gate row, dgate adds those of its group.
+#include "bwpp_cuda_internal.cuh"
+#include "elem.cuh"
+#include "rowwise.cuh"
+
+namespace {
+
+using bwpp_elem::aligned_to;
+using bwpp_elem::Elem;
+using bwpp_elem::Raw;
+using bwpp_row::block_sum;
+
+constexpr int F32 = BWPP_CUDA_DTYPE_F32;
+
+struct JunctionArgs {
+  BwppCudaJunctionParams p;  // gate_rows > 0
+  const float *h;            // forward: h; backward: h'
+  const void *b;
+  const float *gain_post, *gate, *gain_pre;
+  float *h_out;              // forward: h'
+  void *y;                   // forward
+  const float *dh_out;       // backward from here on
+  const void *dy;
+  float *dh;
+  void *db;
+  float *dgate;              // written by the row kernel when gate_rows == 1
+  float *part_post, *part_pre;  // [chunks][cols] or NULL
+  uint32_t chunk_rows, chunks_per_group, group_rows;
+};
+
+// Sums NV values over the TPR threads of a row.
+template <int TPR, int NV>
+__device__ __forceinline__ void row_sum(float (&v)[NV], float *red) {
+  if constexpr (TPR == 32) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+  } else {
+    block_sum<NV>(v, red);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_gain(const float *g, uint32_t c, float (&o)[VEC]) {
+  if (!g) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = 1.0f;
+  } else if constexpr (VEC >= 4) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 t = __ldg(reinterpret_cast<const float4 *>(g + c) + i);
+      o[4 * i] = t.x; o[4 * i + 1] = t.y; o[4 * i + 2] = t.z; o[4 * i + 3] = t.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = __ldg(g + c + e);
+  }
+}
+
+constexpr int block_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
+
+// ---- forward -----------------------------------------------------------------
+
+// TPR threads hold a row, thread t the vectors t, t + TPR, ... (NV of them).
+template <int DT, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(block_threads(TPR))
+    junction_fwd_kernel(const __grid_constant__ JunctionArgs a) {
+  using T = typename Elem<DT>::type;
+  __shared__ float red[32];
+  const BwppCudaJunctionParams &p = a.p;
+  const uint32_t r = blockIdx.x * (block_threads(TPR) / TPR) + threadIdx.x / TPR;
+  if (r >= p.rows) return;  // a whole warp (TPR 32), or none
+  const uint32_t t = threadIdx.x % TPR;
+  const float *h = a.h + (size_t)r * p.ldh;
+  const T *b = static_cast<const T *>(a.b) + (size_t)r * p.ldb;
+  const float *gate = a.gate ? a.gate + (size_t)(r / p.gate_rows) * p.ldgate : nullptr;
+  Raw<F32, VEC> hv[NV];
+  Raw<DT, VEC> bv[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = (t + i * TPR) * VEC;
+    if (c < p.cols) {
+      hv[i].load(h + c);
+      bv[i].load(b + c);
+    } else {
+      hv[i].zero();
+      bv[i].zero();
+    }
+  }
+  float rb = 1.0f;
+  if (p.norm_after) {
+    float ss[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) ss[0] += bv[i].get(e) * bv[i].get(e);
+    row_sum<TPR, 1>(ss, red);
+    rb = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps_post);
+  }
+  float ss[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = (t + i * TPR) * VEC;
+    if (c >= p.cols) continue;
+    float gp[VEC], gt[VEC], v[VEC];
+    load_gain<VEC>(p.norm_after ? a.gain_post : nullptr, c, gp);
+    load_gain<VEC>(gate, c, gt);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float u = bv[i].get(e) * rb * gp[e];
+      v[e] = p.scale_h * hv[i].get(e) + p.scale_b * (gt[e] * u);
+      ss[0] += v[e] * v[e];
+    }
+    hv[i].set(v);
+    hv[i].store(a.h_out + (size_t)r * p.ldh + c);
+  }
+  if (!a.y) return;
+  row_sum<TPR, 1>(ss, red);
+  const float rh = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps_pre);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = (t + i * TPR) * VEC;
+    if (c >= p.cols) continue;
+    float gq[VEC], v[VEC];
+    load_gain<VEC>(a.gain_pre, c, gq);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = hv[i].get(e) * rh * gq[e];
+    Raw<DT, VEC> o;
+    o.set(v);
+    o.store(static_cast<T *>(a.y) + (size_t)r * p.ldy + c);
+  }
+}
+
+constexpr int kLoopThreads = 1024;
+
+// Rows of any width, read again for each step (a thread keeps to its own
+// columns, so it sees its own stores).
+template <int DT>
+__global__ void __launch_bounds__(kLoopThreads)
+    junction_fwd_looped_kernel(const __grid_constant__ JunctionArgs a) {
+  using T = typename Elem<DT>::type;
+  __shared__ float red[32];
+  const BwppCudaJunctionParams &p = a.p;
+  const uint32_t r = blockIdx.x;
+  const float *h = a.h + (size_t)r * p.ldh;
+  const T *b = static_cast<const T *>(a.b) + (size_t)r * p.ldb;
+  const float *gate = a.gate ? a.gate + (size_t)(r / p.gate_rows) * p.ldgate : nullptr;
+  float *ho = a.h_out + (size_t)r * p.ldh;
+  Raw<DT, 1> x;
+  float rb = 1.0f;
+  if (p.norm_after) {
+    float ss[1] = {0.0f};
+    for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+      x.load(b + c);
+      ss[0] += x.get(0) * x.get(0);
+    }
+    block_sum<1>(ss, red);
+    rb = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps_post);
+  }
+  float ss[1] = {0.0f};
+  for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+    x.load(b + c);
+    float u = x.get(0) * rb;
+    if (p.norm_after && a.gain_post) u *= a.gain_post[c];
+    if (gate) u *= gate[c];
+    const float v = p.scale_h * h[c] + p.scale_b * u;
+    ho[c] = v;
+    ss[0] += v * v;
+  }
+  if (!a.y) return;
+  block_sum<1>(ss, red);
+  const float rh = 1.0f / sqrtf(ss[0] / (float)p.cols + p.eps_pre);
+  for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+    const float v[1] = {ho[c] * rh * (a.gain_pre ? a.gain_pre[c] : 1.0f)};
+    x.set(v);
+    x.store(static_cast<T *>(a.y) + (size_t)r * p.ldy + c);
+  }
+}
+
+// ---- backward ----------------------------------------------------------------
+
+// The rows [first, last) of chunk k.
+__device__ __forceinline__ void chunk_range(const JunctionArgs &a, uint32_t k, uint32_t &first,
+                                            uint32_t &last) {
+  const uint32_t g = k / a.chunks_per_group;
+  const uint64_t begin = (uint64_t)g * a.group_rows;
+  const uint64_t end = min(begin + a.group_rows, (uint64_t)a.p.rows);
+  const uint64_t f = begin + (uint64_t)(k - g * a.chunks_per_group) * a.chunk_rows;
+  first = (uint32_t)min(f, end);
+  last = (uint32_t)min(f + a.chunk_rows, end);
+}
+
+template <int DT, int VEC, int NV, int TPR>
+__global__ void __launch_bounds__(block_threads(TPR))
+    junction_bwd_kernel(const __grid_constant__ JunctionArgs a) {
+  using T = typename Elem<DT>::type;
+  constexpr int RPB = block_threads(TPR) / TPR;  // rows that a block works on together
+  __shared__ float red[3 * 32];
+  const BwppCudaJunctionParams &p = a.p;
+  const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  uint32_t first, last;
+  chunk_range(a, blockIdx.x, first, last);
+  const float inv_c = 1.0f / (float)p.cols;
+  float acc_post[NV][VEC], acc_pre[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc_post[i][e] = acc_pre[i][e] = 0.0f;
+
+  for (uint32_t r = first + sub; r < last; r += RPB) {
+    Raw<F32, VEC> hv[NV], dv[NV];
+    Raw<DT, VEC> bv[NV], yv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * VEC;
+      hv[i].zero();
+      dv[i].zero();
+      bv[i].zero();
+      yv[i].zero();
+      if (c < p.cols) {
+        if (a.dy) {
+          hv[i].load(a.h + (size_t)r * p.ldh + c);
+          yv[i].load(static_cast<const T *>(a.dy) + (size_t)r * p.ldy + c);
+        }
+        if (a.dh_out) dv[i].load(a.dh_out + (size_t)r * p.ldh + c);
+        if (a.b) bv[i].load(static_cast<const T *>(a.b) + (size_t)r * p.ldb + c);
+      }
+    }
+    float s[3] = {0.0f, 0.0f, 0.0f};  // sum h'^2, sum gain_pre dy h', sum b^2
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * VEC;
+      if (c >= p.cols) continue;
+      float gq[VEC];
+      load_gain<VEC>(a.gain_pre, c, gq);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float hh = hv[i].get(e), bb = bv[i].get(e);
+        s[0] += hh * hh;
+        s[1] += gq[e] * yv[i].get(e) * hh;
+        s[2] += bb * bb;
+      }
+    }
+    row_sum<TPR, 3>(s, red);
+    const float rh = a.dy ? 1.0f / sqrtf(s[0] * inv_c + p.eps_pre) : 0.0f;
+    const float m2 = rh * s[1] * inv_c;  // mean(g hat)
+    const float rb = p.norm_after ? 1.0f / sqrtf(s[2] * inv_c + p.eps_post) : 1.0f;
+    const float *gate = a.gate ? a.gate + (size_t)(r / p.gate_rows) * p.ldgate : nullptr;
+    float *dgate = a.dgate ? a.dgate + (size_t)r * p.ldgate : nullptr;
+    float m[1] = {0.0f};  // sum gain_post du bhat
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * VEC;
+      if (c >= p.cols) continue;
+      float gq[VEC], gp[VEC], gt[VEC], w[VEC], dg[VEC];
+      load_gain<VEC>(a.gain_pre, c, gq);
+      load_gain<VEC>(p.norm_after ? a.gain_post : nullptr, c, gp);
+      load_gain<VEC>(gate, c, gt);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float hat = hv[i].get(e) * rh, dy = yv[i].get(e);
+        const float dH = dv[i].get(e) + rh * (gq[e] * dy - hat * m2);
+        const float bh = bv[i].get(e) * rb, ee = p.scale_b * dH;
+        const float du = ee * gt[e];
+        acc_pre[i][e] += dy * hat;
+        acc_post[i][e] += (p.gate_rows == 1 ? du : ee) * bh;
+        m[0] += gp[e] * du * bh;
+        dg[e] = ee * bh * gp[e];
+        w[e] = p.scale_h * dH;
+        // kept for the second pass: gain_post du in place of dh'
+        gp[e] *= du;
+      }
+      if (dgate) {
+        Raw<F32, VEC> o;
+        o.set(dg);
+        o.store(dgate + c);
+      }
+      if (a.dh) {
+        Raw<F32, VEC> o;
+        o.set(w);
+        o.store(a.dh + (size_t)r * p.ldh + c);
+      }
+      dv[i].set(gp);
+    }
+    if (!a.db) continue;
+    if (p.norm_after) row_sum<TPR, 1>(m, red);
+    const float m1 = p.norm_after ? m[0] * inv_c : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * VEC;
+      if (c >= p.cols) continue;
+      float w[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = rb * (dv[i].get(e) - bv[i].get(e) * rb * m1);
+      Raw<DT, VEC> o;
+      o.set(w);
+      o.store(static_cast<T *>(a.db) + (size_t)r * p.ldb + c);
+    }
+  }
+
+  // the chunk's partial rows; with several rows at a time, their warps' sums
+  // are added in warp order
+  auto write = [&](float (&acc)[NV][VEC], float *part) {
+    if (!part) return;  // the same for the whole block
+    part += (size_t)blockIdx.x * p.cols;
+    if constexpr (RPB == 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const uint32_t c = (t + i * TPR) * VEC;
+        if (c >= p.cols) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) part[c + e] = acc[i][e];
+      }
+    } else {
+      __shared__ float sums[RPB][NV * TPR * VEC];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sums[sub][(t + i * TPR) * VEC + e] = acc[i][e];
+      __syncthreads();
+      for (uint32_t c = threadIdx.x; c < p.cols; c += block_threads(TPR)) {
+        float v = sums[0][c];
+#pragma unroll
+        for (int w = 1; w < RPB; ++w) v += sums[w][c];
+        part[c] = v;
+      }
+    }
+  };
+  write(acc_post, a.part_post);
+  write(acc_pre, a.part_pre);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kLoopThreads)
+    junction_bwd_looped_kernel(const __grid_constant__ JunctionArgs a) {
+  using T = typename Elem<DT>::type;
+  __shared__ float red[3 * 32];
+  const BwppCudaJunctionParams &p = a.p;
+  uint32_t first, last;
+  chunk_range(a, blockIdx.x, first, last);
+  const float inv_c = 1.0f / (float)p.cols;
+  float *pp = a.part_post ? a.part_post + (size_t)blockIdx.x * p.cols : nullptr;
+  float *pq = a.part_pre ? a.part_pre + (size_t)blockIdx.x * p.cols : nullptr;
+  for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+    if (pp) pp[c] = 0.0f;
+    if (pq) pq[c] = 0.0f;
+  }
+  for (uint32_t r = first; r < last; ++r) {
+    const float *h = a.h + (size_t)r * p.ldh;
+    const float *dho = a.dh_out ? a.dh_out + (size_t)r * p.ldh : nullptr;
+    const T *b = a.b ? static_cast<const T *>(a.b) + (size_t)r * p.ldb : nullptr;
+    const T *dyr = a.dy ? static_cast<const T *>(a.dy) + (size_t)r * p.ldy : nullptr;
+    const float *gate = a.gate ? a.gate + (size_t)(r / p.gate_rows) * p.ldgate : nullptr;
+    Raw<DT, 1> x;
+    float s[3] = {0.0f, 0.0f, 0.0f};
+    for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+      if (dyr) {
+        x.load(dyr + c);
+        s[0] += h[c] * h[c];
+        s[1] += (a.gain_pre ? a.gain_pre[c] : 1.0f) * x.get(0) * h[c];
+      }
+      if (b) {
+        x.load(b + c);
+        s[2] += x.get(0) * x.get(0);
+      }
+    }
+    block_sum<3>(s, red);
+    const float rh = dyr ? 1.0f / sqrtf(s[0] * inv_c + p.eps_pre) : 0.0f;
+    const float m2 = rh * s[1] * inv_c;
+    const float rb = p.norm_after ? 1.0f / sqrtf(s[2] * inv_c + p.eps_post) : 1.0f;
+    auto dH_of = [&](uint32_t c, float &dyhat) {
+      float v = dho ? dho[c] : 0.0f;
+      dyhat = 0.0f;
+      if (dyr) {
+        Raw<DT, 1> z;
+        z.load(dyr + c);
+        const float hat = h[c] * rh;
+        v += rh * ((a.gain_pre ? a.gain_pre[c] : 1.0f) * z.get(0) - hat * m2);
+        dyhat = z.get(0) * hat;
+      }
+      return v;
+    };
+    const bool gained = p.norm_after && a.gain_post;
+    float m[1] = {0.0f};
+    if (p.norm_after && b) {
+      for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+        float unused;
+        const float du = p.scale_b * dH_of(c, unused) * (gate ? gate[c] : 1.0f);
+        x.load(b + c);
+        m[0] += (gained ? a.gain_post[c] : 1.0f) * du * (x.get(0) * rb);
+      }
+      block_sum<1>(m, red);
+    }
+    const float m1 = m[0] * inv_c;
+    for (uint32_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
+      float dyhat;
+      const float dH = dH_of(c, dyhat), ee = p.scale_b * dH;
+      const float du = ee * (gate ? gate[c] : 1.0f), gp = gained ? a.gain_post[c] : 1.0f;
+      if (pq) pq[c] += dyhat;
+      if (b) {
+        x.load(b + c);
+        const float bh = x.get(0) * rb;
+        if (pp) pp[c] += (p.gate_rows == 1 ? du : ee) * bh;
+        if (a.dgate) a.dgate[(size_t)r * p.ldgate + c] = ee * bh * gp;
+        const float w[1] = {rb * (gp * du - bh * m1)};
+        x.set(w);
+      } else {
+        const float w[1] = {du};
+        x.set(w);
+      }
+      if (a.db) x.store(static_cast<T *>(a.db) + (size_t)r * p.ldb + c);
+      if (a.dh) a.dh[(size_t)r * p.ldh + c] = p.scale_h * dH;
+    }
+  }
+}
+
+// Sums of the chunks' partial rows.  blockIdx.x: 0 dgain_post, 1 dgain_pre,
+// 2 + g dgate of group g; blockIdx.y: 32 columns, one per lane.  Warp w adds
+// rows w, w + 32, ... in order, then a thread per column adds the 32 warps'
+// sums in warp order.
+struct JunctionSums {
+  const float *part_post, *part_pre;
+  const float *gain_post, *gate;
+  float *dgain_post, *dgain_pre, *dgate;
+  uint32_t chunks, chunks_per_group, cols, ldgate;
+  int weighted;  // dgain_post: weight the partial rows with their gate rows
+};
+
+constexpr int kSumWarps = 32;
+__global__ void __launch_bounds__(32 * kSumWarps) junction_sums_kernel(const JunctionSums a) {
+  const uint32_t job = blockIdx.x;
+  float *out = job == 0 ? a.dgain_post : job == 1 ? a.dgain_pre : a.dgate;
+  if (!out) return;
+  __shared__ float sums[kSumWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t c = blockIdx.y * 32 + lane;
+  const float *part = job == 1 ? a.part_pre : a.part_post;
+  const uint32_t begin = job < 2 ? 0 : (job - 2) * a.chunks_per_group;
+  const uint32_t end = job < 2 ? a.chunks : begin + a.chunks_per_group;
+  float acc = 0.0f;
+  if (c < a.cols) {
+    if (job == 0 && a.weighted) {
+      for (uint32_t k = begin + warp; k < end; k += kSumWarps)
+        acc += part[(size_t)k * a.cols + c] * a.gate[(size_t)(k / a.chunks_per_group) * a.ldgate + c];
+    } else {
+#pragma unroll 4
+      for (uint32_t k = begin + warp; k < end; k += kSumWarps) acc += part[(size_t)k * a.cols + c];
+    }
+  }
+  sums[warp][lane] = acc;
+  __syncthreads();
+  if (warp == 0 && c < a.cols) {
+    float v = sums[0][lane];
+    for (int w = 1; w < kSumWarps; ++w) v += sums[w][lane];
+    if (job >= 2) {
+      if (a.gain_post) v *= a.gain_post[c];
+      out[(size_t)(job - 2) * a.ldgate + c] = v;
+    } else {
+      out[c] = v;
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------
+
+struct Chunks {
+  uint32_t group_rows, groups, chunk_rows, per_group, chunks;
+};
+
+// A chunk holds consecutive rows of one group (rows that share a gate row and
+// whose dgate is summed), about `per_sm` chunks per SM.
+bool make_chunks(BwppCudaCtx *ctx, uint32_t rows, uint32_t gate_rows, Chunks &k) {
+  constexpr uint32_t per_sm = 4;
+  k.group_rows = gate_rows <= 1 || gate_rows > rows ? rows : gate_rows;
+  k.groups = (uint32_t)(((uint64_t)rows + k.group_rows - 1) / k.group_rows);
+  const uint32_t want = (uint32_t)ctx->num_sms * per_sm;
+  k.chunk_rows = (uint32_t)(((uint64_t)rows + want - 1) / want);
+  k.per_group = (uint32_t)(((uint64_t)k.group_rows + k.chunk_rows - 1) / k.chunk_rows);
+  const uint64_t n = (uint64_t)k.groups * k.per_group;
+  k.chunks = (uint32_t)n;
+  return n < (1u << 31) - 2;
+}
+
+int check_args(BwppCudaCtx *ctx, const BwppCudaJunctionParams *p, bool has_b, bool has_gate,
+               bool has_y) {
+  if (!p) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: NULL params");
+  if (p->ldh < p->cols || (has_b && p->ldb < p->cols) || (has_gate && p->ldgate < p->cols) ||
+      (has_y && p->ldy < p->cols))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: leading dim smaller than row");
+  if (p->rows > 0x7fffffffu)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: more than 2^31 - 1 rows");
+  return BWPP_CUDA_OK;
+}
+
+// Whether all of a's tensors take eight-element transfers.
+template <int DT>
+bool vectors(const JunctionArgs &a) {
+  const BwppCudaJunctionParams &p = a.p;
+  if (p.cols % 8 || p.ldh % 8 || p.ldb % 8 || p.ldy % 8 || (a.gate && p.ldgate % 8)) return false;
+  for (const void *q : {(const void *)a.h, a.b, (const void *)a.gain_post, (const void *)a.gate,
+                        (const void *)a.gain_pre, (const void *)a.h_out, (const void *)a.y,
+                        (const void *)a.dh_out, a.dy, (const void *)a.dh, (const void *)a.db,
+                        (const void *)a.dgate})
+    if (!aligned_to(q, 16)) return false;
+  return true;
+}
+
+template <int DT>
+void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
+  const uint32_t cols = a.p.cols;
+  cudaStream_t s = ctx->stream;
+#define BWPP_FWD(VEC, NV, TPR)                                                             \
+  junction_fwd_kernel<DT, VEC, NV, TPR>                                                    \
+      <<<(a.p.rows + block_threads(TPR) / TPR - 1) / (block_threads(TPR) / TPR),           \
+         block_threads(TPR), 0, s>>>(a)
+  if (vectors<DT>(a)) {
+    if (cols <= 256) BWPP_FWD(8, 1, 32);
+    else if (cols <= 512) BWPP_FWD(8, 2, 32);
+    else if (cols <= 1024) BWPP_FWD(8, 1, 128);
+    else if (cols <= 2048) BWPP_FWD(8, 1, 256);
+    else if (cols <= 4096) BWPP_FWD(8, 2, 256);
+    else if (cols <= 8192) BWPP_FWD(8, 2, 512);
+    else if (cols <= 16384) BWPP_FWD(8, 2, 1024);
+    else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
+  } else {
+    if (cols <= 128) BWPP_FWD(1, 4, 32);
+    else if (cols <= 1024) BWPP_FWD(1, 8, 128);
+    else if (cols <= 4096) BWPP_FWD(1, 8, 512);
+    else if (cols <= 16384) BWPP_FWD(1, 16, 1024);
+    else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
+  }
+#undef BWPP_FWD
+}
+
+template <int DT>
+void launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks) {
+  const uint32_t cols = a.p.cols;
+  cudaStream_t s = ctx->stream;
+#define BWPP_BWD(VEC, NV, TPR) \
+  junction_bwd_kernel<DT, VEC, NV, TPR><<<chunks, block_threads(TPR), 0, s>>>(a)
+  if (vectors<DT>(a)) {
+    if (cols <= 256) BWPP_BWD(8, 1, 32);
+    else if (cols <= 1024) BWPP_BWD(8, 1, 128);
+    else if (cols <= 2048) BWPP_BWD(8, 1, 256);
+    else if (cols <= 4096) BWPP_BWD(8, 1, 512);
+    else if (cols <= 8192) BWPP_BWD(8, 1, 1024);
+    else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
+  } else {
+    if (cols <= 128) BWPP_BWD(1, 4, 32);
+    else if (cols <= 1024) BWPP_BWD(1, 8, 128);
+    else if (cols <= 4096) BWPP_BWD(1, 8, 512);
+    else if (cols <= 8192) BWPP_BWD(1, 8, 1024);
+    else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
+  }
+#undef BWPP_BWD
+}
+
+template <int DT>
+int junction_fwd(BwppCudaCtx *ctx, const float *h, const void *b, const float *gain_post,
+                 const float *gate, const float *gain_pre, float *h_out, void *y,
+                 const BwppCudaJunctionParams *p) {
+  int rc = bwpp_ctx_enter(ctx);
+  if (!rc) rc = check_args(ctx, p, true, gate != nullptr, y != nullptr);
+  if (rc) return rc;
+  if (p->rows == 0 || p->cols == 0) return BWPP_CUDA_OK;
+  if (!h || !b || !h_out) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: NULL buffer");
+  JunctionArgs a{};
+  a.p = *p;
+  if (a.p.gate_rows == 0) a.p.gate_rows = a.p.rows;
+  if (!y) a.p.ldy = 0;
+  a.h = h;
+  a.b = b;
+  a.gain_post = gain_post;
+  a.gate = gate;
+  a.gain_pre = gain_pre;
+  a.h_out = h_out;
+  a.y = y;
+  launch_fwd<DT>(ctx, a);
+  BWPP_LAUNCH_CHECK(ctx, "junction fwd");
+  return BWPP_CUDA_OK;
+}
+
+template <int DT>
+int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const float *gain_post,
+                 const float *gate, const float *gain_pre, const float *dh_out, const void *dy,
+                 float *dh, void *db, float *dgain_post, float *dgate, float *dgain_pre,
+                 const BwppCudaJunctionParams *p) {
+  int rc = bwpp_ctx_enter(ctx);
+  if (!rc) rc = check_args(ctx, p, b || db, gate || dgate, dy != nullptr);
+  if (rc) return rc;
+  if (dgate && !gate)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction bwd: dgate without a gate");
+  if (dgain_post && !p->norm_after)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction bwd: dgain_post without norm_after");
+  if (p->cols == 0) return BWPP_CUDA_OK;
+  cudaStream_t s = ctx->stream;
+  if (p->rows == 0) {
+    if (dgain_post)
+      rc = bwpp_check_cuda(ctx, cudaMemsetAsync(dgain_post, 0, sizeof(float) * p->cols, s), "memset");
+    if (!rc && dgain_pre)
+      rc = bwpp_check_cuda(ctx, cudaMemsetAsync(dgain_pre, 0, sizeof(float) * p->cols, s), "memset");
+    return rc;
+  }
+  // b is read where the norm's, the gate's or the gain's gradient needs it
+  const bool need_b = (db && p->norm_after) || dgain_post || dgate;
+  if ((dy && !h_out) || (need_b && !b))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction bwd: NULL buffer");
+  if (db && db == b)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction bwd: db may not be b");
+  JunctionArgs a{};
+  a.p = *p;
+  if (a.p.gate_rows == 0) a.p.gate_rows = a.p.rows;
+  if (!dy) a.p.ldy = 0;
+  if (!b && !db) a.p.ldb = 0;
+  a.h = h_out;
+  a.b = need_b ? b : nullptr;
+  a.gain_post = gain_post;
+  a.gate = gate;
+  a.gain_pre = gain_pre;
+  a.dh_out = dh_out;
+  a.dy = dy;
+  a.dh = dh;
+  a.db = db;
+  const bool per_row = a.p.gate_rows == 1;
+  a.dgate = per_row ? dgate : nullptr;
+  Chunks k;
+  if (!make_chunks(ctx, a.p.rows, a.p.gate_rows, k))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: too many gate rows");
+  a.chunk_rows = k.chunk_rows;
+  a.chunks_per_group = k.per_group;
+  a.group_rows = k.group_rows;
+  const bool sum_post = dgain_post || (dgate && !per_row);
+  const bool sums = sum_post || dgain_pre;
+  if (sums) {
+    uint8_t *scratch;
+    const size_t part = (size_t)k.chunks * a.p.cols;
+    rc = bwpp_op_scratch(ctx, 2 * part * sizeof(float), "junction bwd", &scratch);
+    if (rc) return rc;
+    if (sum_post) a.part_post = reinterpret_cast<float *>(scratch);
+    if (dgain_pre) a.part_pre = reinterpret_cast<float *>(scratch) + part;
+  }
+  launch_bwd<DT>(ctx, a, k.chunks);
+  BWPP_LAUNCH_CHECK(ctx, "junction bwd");
+  if (sums) {
+    JunctionSums q{};
+    q.part_post = a.part_post;
+    q.part_pre = a.part_pre;
+    q.gain_post = a.p.norm_after ? gain_post : nullptr;
+    q.gate = gate;
+    q.dgain_post = dgain_post;
+    q.dgain_pre = dgain_pre;
+    q.dgate = per_row ? nullptr : dgate;
+    q.chunks = k.chunks;
+    q.chunks_per_group = k.per_group;
+    q.cols = a.p.cols;
+    q.ldgate = a.p.ldgate;
+    q.weighted = gate && !per_row;
+    const dim3 grid(2 + (q.dgate ? k.groups : 0), (a.p.cols + 31) / 32);
+    if (grid.y > 65535)
+      return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: row too wide");
+    junction_sums_kernel<<<grid, 32 * kSumWarps, 0, s>>>(q);
+    BWPP_LAUNCH_CHECK(ctx, "junction sums");
+  }
+  return BWPP_CUDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t bwpp_cuda_junction_bwd_workspace_size(BwppCudaCtx *ctx, uint32_t rows, uint32_t cols,
+                                             uint32_t gate_rows) {
+  if (!ctx || rows == 0 || cols == 0) return 0;
+  Chunks k;
+  if (!make_chunks(ctx, rows, gate_rows ? gate_rows : rows, k)) return 0;
+  return 2 * (size_t)k.chunks * cols * sizeof(float) + BWPP_OP_SCRATCH_PAD;
+}
+
+#define BWPP_JUNCTION(SUFFIX, DT, T)                                                             \
+  int bwpp_cuda_junction_fwd_##SUFFIX(BwppCudaCtx *ctx, const float *h, const T *b,              \
+                                      const float *gain_post, const float *gate,                 \
+                                      const float *gain_pre, float *h_out, T *y,                 \
+                                      const BwppCudaJunctionParams *params) {                    \
+    return junction_fwd<DT>(ctx, h, b, gain_post, gate, gain_pre, h_out, y, params);             \
+  }                                                                                              \
+  int bwpp_cuda_junction_bwd_##SUFFIX(                                                           \
+      BwppCudaCtx *ctx, const float *h_out, const T *b, const float *gain_post,                  \
+      const float *gate, const float *gain_pre, const float *dh_out, const T *dy, float *dh,     \
+      T *db, float *dgain_post, float *dgate, float *dgain_pre,                                  \
+      const BwppCudaJunctionParams *params) {                                                    \
+    return junction_bwd<DT>(ctx, h_out, b, gain_post, gate, gain_pre, dh_out, dy, dh, db,        \
+                            dgain_post, dgate, dgain_pre, params);                               \
+  }
+BWPP_JUNCTION(f32, BWPP_CUDA_DTYPE_F32, float)
+BWPP_JUNCTION(bf16, BWPP_CUDA_DTYPE_BF16, uint16_t)
+BWPP_JUNCTION(f16, BWPP_CUDA_DTYPE_F16, uint16_t)
+#undef BWPP_JUNCTION
+
+}  // extern "C"

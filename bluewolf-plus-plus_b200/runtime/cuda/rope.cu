@@ -1,0 +1,267 @@
+// Rotary positions on q and k, forward and gradient, f16 / bf16 / fp32.
+//
+// Pair i of a head turns by position * f_i:
+//   (y0, y1) = a (x0 cos - x1 sin, x1 cos + x0 sin)
+// over pairs (i, i + R/2) or, interleaved, (2i, 2i + 1) of the first R
+// columns of each head; the columns behind R are copied (left alone in place).
+// The map is a rotation times the amplitude a, so its gradient is the same
+// kernel turning back.
+//
+// Angles.  The table holds each frequency as a 64-bit fraction of a turn, and
+// position * fraction mod 2^64 is the angle's fraction of a turn: the whole
+// turns, which carry no information, drop out exactly for any 32-bit position
+// (an fp32 product is 0.03 rad off at position 10^6).  The top 32 bits go to
+// sincospif, whose argument is then within [-1, 1).
+#include <math.h>
+
+#include "bwpp_cuda_internal.cuh"
+#include "elem.cuh"
+
+namespace {
+
+using bwpp_elem::aligned_to;
+using bwpp_elem::Elem;
+using bwpp_elem::Raw;
+
+constexpr int kThreads = 256;
+
+struct RopeArgs {
+  BwppCudaRopeTable table;
+  const void *q, *k;
+  void *qo, *ko;
+  const int32_t *positions;
+  BwppCudaRopeParams p;
+  uint32_t seq;     // p.seq, or tokens where it is 0
+  uint32_t token0;  // first token of this launch
+  uint32_t units;   // threads with work: tokens * slots * lanes
+  uint32_t turn_slots, slots, lanes;
+};
+
+// A thread owns one slot (VEC pairs, or VEC columns behind R) of one token in
+// heads lane, lane + lanes, ...
+template <int DT, int VEC, bool IL>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+  using T = typename Elem<DT>::type;
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  if (id >= a.units) return;
+  const uint32_t per = a.slots * a.lanes;
+  const uint32_t t = a.token0 + id / per, rem = id % per;
+  const uint32_t lane = rem / a.slots, slot = rem % a.slots;
+  const uint32_t b = t / a.seq, s = t - b * a.seq;
+  const uint32_t heads = a.p.heads_q + a.p.heads_k;
+  const bool turns = slot < a.turn_slots;
+  const bool two = turns && !(IL && VEC > 1);  // the slot's pairs lie in two vectors
+  const uint32_t half = a.table.pairs;
+  uint32_t c0, c1;
+  if (!turns) {
+    c0 = c1 = 2 * half + (slot - a.turn_slots) * VEC;
+  } else if (IL) {
+    c0 = VEC > 1 ? slot * VEC : 2 * slot;
+    c1 = c0 + 1;
+  } else {
+    c0 = slot * VEC;
+    c1 = c0 + half;
+  }
+  constexpr int PAIRS = IL && VEC > 1 ? VEC / 2 : VEC;
+  float cs[PAIRS], sn[PAIRS];
+  if (turns) {
+    const int64_t pos =
+        a.positions ? (int64_t)a.positions[t] : (int64_t)a.p.pos0 + (int64_t)s;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const uint64_t turn = (uint64_t)pos * a.table.turns[slot * PAIRS + i];
+      sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &sn[i], &cs[i]);
+      cs[i] *= a.table.amplitude;
+      sn[i] *= a.p.inverse ? -a.table.amplitude : a.table.amplitude;
+    }
+  }
+  for (uint32_t h = lane; h < heads; h += a.lanes) {
+    const bool isq = h < a.p.heads_q;
+    const uint32_t hh = isq ? h : h - a.p.heads_q, nh = isq ? a.p.heads_q : a.p.heads_k;
+    const size_t ldi = isq ? a.p.ldq : a.p.ldk, ldo = isq ? a.p.ldq_out : a.p.ldk_out;
+    const size_t at = a.p.head_major_in ? (((size_t)b * nh + hh) * a.seq + s) * ldi
+                                        : t * ldi + (size_t)hh * a.p.head_dim;
+    const size_t to = a.p.head_major_out ? (((size_t)b * nh + hh) * a.seq + s) * ldo
+                                         : t * ldo + (size_t)hh * a.p.head_dim;
+    const T *src = static_cast<const T *>(isq ? a.q : a.k) + at;
+    T *dst = static_cast<T *>(isq ? a.qo : a.ko) + to;
+    Raw<DT, VEC> x, y;
+    x.load(src + c0);
+    if (two) y.load(src + c1);
+    if (turns) {
+      float v[VEC], w[VEC];
+      if constexpr (IL && VEC > 1) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          const float x0 = x.get(2 * i), x1 = x.get(2 * i + 1);
+          v[2 * i] = x0 * cs[i] - x1 * sn[i];
+          v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+        }
+        x.set(v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float x0 = x.get(i), x1 = y.get(i);
+          v[i] = x0 * cs[i] - x1 * sn[i];
+          w[i] = x1 * cs[i] + x0 * sn[i];
+        }
+        x.set(v);
+        y.set(w);
+      }
+    }
+    x.store(dst + c0);
+    if (two) y.store(dst + c1);
+  }
+}
+
+template <int DT, int VEC>
+int rope_launch(BwppCudaCtx *ctx, RopeArgs &a) {
+  const BwppCudaRopeParams &p = a.p;
+  const uint32_t R = 2 * a.table.pairs;
+  const bool pairs_in_one = p.interleaved && VEC > 1;
+  a.turn_slots = (pairs_in_one ? R : R / 2) / VEC;
+  const bool in_place = a.qo == a.q && a.ko == a.k;
+  a.slots = a.turn_slots + (in_place ? 0 : (p.head_dim - R) / VEC);
+  a.lanes = p.heads_q + p.heads_k;
+  const uint64_t per = (uint64_t)a.slots * a.lanes;
+  const uint64_t most = (1u << 30) / per;  // tokens of a launch: unit ids stay in 31 bits
+  if (most == 0)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "rope: heads * head_dim too large");
+  for (uint64_t t0 = 0; t0 < p.tokens; t0 += most) {
+    const uint64_t n = p.tokens - t0 < most ? p.tokens - t0 : most;
+    a.token0 = (uint32_t)t0;
+    a.units = (uint32_t)(n * per);
+    const uint32_t grid = (a.units + kThreads - 1) / kThreads;
+    if (p.interleaved) rope_kernel<DT, VEC, true><<<grid, kThreads, 0, ctx->stream>>>(a);
+    else rope_kernel<DT, VEC, false><<<grid, kThreads, 0, ctx->stream>>>(a);
+    BWPP_LAUNCH_CHECK(ctx, "rope");
+  }
+  return BWPP_CUDA_OK;
+}
+
+template <int DT>
+int rope(BwppCudaCtx *ctx, const void *q, const void *k, void *qo, void *ko,
+         const int32_t *positions, const BwppCudaRopeTable *table, const BwppCudaRopeParams *pp) {
+  int rc = bwpp_ctx_enter(ctx);
+  if (rc) return rc;
+  if (!table || !pp) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: NULL table or params");
+  const BwppCudaRopeParams &p = *pp;
+  const uint32_t R = 2 * table->pairs;
+  if (table->pairs == 0 || table->pairs > BWPP_CUDA_ROPE_MAX_PAIRS || R > p.head_dim)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: table of %u pairs for head_dim %u",
+                          table->pairs, p.head_dim);
+  if (p.tokens == 0 || (p.heads_q == 0 && p.heads_k == 0)) return BWPP_CUDA_OK;
+  if ((p.heads_q && (!q || !qo)) || (p.heads_k && (!k || !ko)))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: NULL buffer");
+  const uint64_t rq = (uint64_t)p.heads_q * p.head_dim, rk = (uint64_t)p.heads_k * p.head_dim;
+  if ((p.heads_q && (p.ldq < (p.head_major_in ? p.head_dim : rq) ||
+                     p.ldq_out < (p.head_major_out ? p.head_dim : rq))) ||
+      (p.heads_k && (p.ldk < (p.head_major_in ? p.head_dim : rk) ||
+                     p.ldk_out < (p.head_major_out ? p.head_dim : rk))))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: leading dim smaller than row");
+  const uint32_t seq = p.seq ? p.seq : p.tokens;
+  if ((p.head_major_in || p.head_major_out) && p.tokens % seq)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: tokens is not a multiple of seq");
+  const bool same = (p.head_major_in != 0) == (p.head_major_out != 0);
+  if ((p.heads_q && q == qo && !(same && p.ldq == p.ldq_out)) ||
+      (p.heads_k && k == ko && !(same && p.ldk == p.ldk_out)))
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: in place needs one layout and pitch");
+  RopeArgs a{};
+  a.table = *table;
+  a.q = q;
+  a.k = p.heads_k ? k : q;
+  a.qo = qo;
+  a.ko = p.heads_k ? ko : qo;
+  if (!p.heads_q) {
+    a.q = k;
+    a.qo = ko;
+  }
+  a.positions = positions;
+  a.p = p;
+  a.seq = seq;
+  // the widest transfer that every address and the pairs' halves allow
+  constexpr int ES = (int)sizeof(typename Elem<DT>::type);
+  auto fits = [&](uint32_t v) {
+    if (p.head_dim % v || (p.interleaved ? R : R / 2) % v || R % v) return false;
+    if (p.heads_q && (p.ldq % v || p.ldq_out % v || !aligned_to(q, v * ES) || !aligned_to(qo, v * ES)))
+      return false;
+    if (p.heads_k && (p.ldk % v || p.ldk_out % v || !aligned_to(k, v * ES) || !aligned_to(ko, v * ES)))
+      return false;
+    return true;
+  };
+  if constexpr (ES == 2) {
+    if (fits(8)) return rope_launch<DT, 8>(ctx, a);
+  }
+  if (fits(4)) return rope_launch<DT, 4>(ctx, a);
+  if (fits(2)) return rope_launch<DT, 2>(ctx, a);
+  return rope_launch<DT, 1>(ctx, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bwpp_cuda_rope_table(BwppCudaRopeTable *out, const BwppCudaRopeConfig *cfg) {
+  if (!out || !cfg) return BWPP_CUDA_ERR_ARG;
+  const uint32_t R = cfg->rotary_dim;
+  if (R == 0 || (R & 1) || R / 2 > BWPP_CUDA_ROPE_MAX_PAIRS) return BWPP_CUDA_ERR_ARG;
+  if (!(cfg->base > 0) || !isfinite(cfg->base) || !(cfg->amplitude > 0) || !isfinite(cfg->amplitude))
+    return BWPP_CUDA_ERR_ARG;
+  const bool scaled = cfg->scaling != BWPP_CUDA_ROPE_NONE;
+  if (scaled && (!(cfg->factor > 0) || !isfinite(cfg->factor))) return BWPP_CUDA_ERR_ARG;
+  double base = cfg->base;
+  switch (cfg->scaling) {
+    case BWPP_CUDA_ROPE_NONE:
+    case BWPP_CUDA_ROPE_LINEAR: break;
+    case BWPP_CUDA_ROPE_BASE:
+      if (R == 2) return BWPP_CUDA_ERR_ARG;  // one pair does not depend on the base
+      base *= pow(cfg->factor, (double)R / (R - 2));
+      break;
+    case BWPP_CUDA_ROPE_PARTS:
+      if (!(cfg->context > 0) || !isfinite(cfg->context) || !(cfg->high > cfg->low) ||
+          !isfinite(cfg->high) || !isfinite(cfg->low))
+        return BWPP_CUDA_ERR_ARG;
+      break;
+    default: return BWPP_CUDA_ERR_ARG;
+  }
+  const double two_pi = 6.283185307179586476925286766559;
+  BwppCudaRopeTable t = {};
+  t.pairs = R / 2;
+  t.amplitude = cfg->amplitude;
+  for (uint32_t i = 0; i < R / 2; ++i) {
+    double f = pow(base, -2.0 * i / R);  // radians per position
+    if (cfg->scaling == BWPP_CUDA_ROPE_LINEAR) f /= cfg->factor;
+    if (cfg->scaling == BWPP_CUDA_ROPE_PARTS) {
+      double keep = (cfg->context * f / two_pi - cfg->low) / (cfg->high - cfg->low);
+      keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+      f = f * keep + f / cfg->factor * (1 - keep);
+    }
+    const double turn = f / two_pi;
+    if (!isfinite(turn)) return BWPP_CUDA_ERR_ARG;
+    // whole turns per position drop out; ldexp is exact, llrint would not fit
+    const double frac = turn - floor(turn);
+    t.turns[i] = (uint64_t)ldexp(frac, 64);
+  }
+  *out = t;
+  return BWPP_CUDA_OK;
+}
+
+int bwpp_cuda_rope_bf16(BwppCudaCtx *ctx, const uint16_t *q, const uint16_t *k, uint16_t *q_out,
+                        uint16_t *k_out, const int32_t *positions, const BwppCudaRopeTable *table,
+                        const BwppCudaRopeParams *params) {
+  return rope<BWPP_CUDA_DTYPE_BF16>(ctx, q, k, q_out, k_out, positions, table, params);
+}
+
+int bwpp_cuda_rope_f16(BwppCudaCtx *ctx, const uint16_t *q, const uint16_t *k, uint16_t *q_out,
+                       uint16_t *k_out, const int32_t *positions, const BwppCudaRopeTable *table,
+                       const BwppCudaRopeParams *params) {
+  return rope<BWPP_CUDA_DTYPE_F16>(ctx, q, k, q_out, k_out, positions, table, params);
+}
+
+int bwpp_cuda_rope_f32(BwppCudaCtx *ctx, const float *q, const float *k, float *q_out, float *k_out,
+                       const int32_t *positions, const BwppCudaRopeTable *table,
+                       const BwppCudaRopeParams *params) {
+  return rope<BWPP_CUDA_DTYPE_F32>(ctx, q, k, q_out, k_out, positions, table, params);
+}
+
+}  // extern "C"

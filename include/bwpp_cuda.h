@@ -332,6 +332,163 @@ int bwpp_cuda_broadcast_f32(BwppCudaCtx *ctx, const float *src, float *dst,
 int bwpp_cuda_cast_f32_bf16(BwppCudaCtx *ctx, const float *src, uint16_t *dst,
                             uint32_t rows, uint32_t cols, uint32_t ld_src);
 
+/* ---- training-step operators around a decoder block ---------------------- */
+/* No counterparts in the reference.  All are stream-async on the ctx's stream.
+ * Scratch comes from the ctx (bwpp_cuda_ctx_set_workspace or ctx-owned).  A
+ * captured graph keeps the scratch's address, so a call that needs scratch
+ * and is made while the ctx's stream is capturing needs a caller's workspace
+ * (BWPP_CUDA_ERR_UNSUPPORTED without one); graphs that share a workspace must
+ * not run at the same time. */
+
+/* Softmax cross entropy over a vocabulary of V, from hidden states x [T, ldx]
+ * and the vocabulary weight, without keeping the T x V logits:
+ *   logit[t, v] = scale * sum_d x[t, d] W[v, d]
+ *   lse[t]  = log sum_v exp(logit[t, v])      (natural logarithm)
+ *   loss[t] = lse[t] - logit[t, target[t]]
+ * W[v, d] = w_vocab_major ? w[v*ldw + d] : w[d*ldw + v].  x and w are bf16
+ * bits, products accumulate in fp32 on the tensor cores; loss and lse are
+ * fp32.  Any sizes and pitches; row pitches that are no multiple of 8, or
+ * addresses that are not 16-byte aligned, cost packed copies in scratch.
+ * A negative target ignores its row (loss 0, zero gradient, whatever its x
+ * holds).  A target >= V is an error that the next bwpp_cuda_sync reports
+ * (BWPP_CUDA_ERR_ARG); its loss is NaN and its gradient zero. */
+typedef struct {
+  uint32_t T, V, D;
+  uint32_t ldx, ldw;
+  uint32_t lddx, lddw;  /* backward: pitches of dx and dw (dw laid out like w) */
+  int w_vocab_major;
+  int grads_bf16;       /* backward: dx and dw are bf16, else fp32 */
+  float scale;
+} BwppCudaXentParams;
+
+/* Scratch bytes of a call whose buffers are 16-byte aligned. */
+size_t bwpp_cuda_xent_workspace_size(const BwppCudaXentParams *params, int backward);
+/* loss (with target) or lse may be NULL. */
+int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,
+                            const int32_t *target, float *loss, float *lse,
+                            const BwppCudaXentParams *params);
+/* dx = scale * dlogit W, dw = scale * dlogit^T x, overwritten, with dlogit[t, v]
+ * = dloss[t] (exp(logit - lse[t]) - [v == target[t]]); lse as the forward wrote
+ * it; dloss [T] or NULL (ones); dx or dw may be NULL.  dlogit is rounded to
+ * bf16 for the tensor cores, so fp32 gradients carry that rounding too. */
+int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,
+                            const int32_t *target, const float *lse, const float *dloss, void *dx,
+                            void *dw, const BwppCudaXentParams *params);
+
+/* Rotary positions.  Pair i of each head turns by position * f_i:
+ *   (y0, y1) = amplitude * (x0 cos - x1 sin, x1 cos + x0 sin)
+ * with f_i = base^(-2i / rotary_dim) radians, scaled for longer contexts:
+ *   LINEAR  f_i / factor
+ *   BASE    base * factor^(rotary_dim / (rotary_dim - 2)) instead of base
+ *   PARTS   pairs that turn at least `high` times over `context` positions keep
+ *           f_i, below `low` times they take f_i / factor, in between a blend
+ *           linear in the number of turns
+ * A table is made once per model configuration and passed by value into each
+ * launch: no device memory. */
+#define BWPP_CUDA_ROPE_MAX_PAIRS 128
+typedef enum {
+  BWPP_CUDA_ROPE_NONE = 0,
+  BWPP_CUDA_ROPE_LINEAR = 1,
+  BWPP_CUDA_ROPE_BASE = 2,
+  BWPP_CUDA_ROPE_PARTS = 3
+} BwppCudaRopeScaling;
+
+typedef struct {
+  uint32_t rotary_dim;  /* even, 2..256 */
+  int scaling;          /* BwppCudaRopeScaling */
+  double base, factor;
+  double context, low, high;  /* PARTS */
+  float amplitude;
+} BwppCudaRopeConfig;
+
+typedef struct {
+  uint32_t pairs;       /* rotary_dim / 2 */
+  float amplitude;
+  uint64_t turns[BWPP_CUDA_ROPE_MAX_PAIRS]; /* f_i / 2 pi mod 1, in 2^-64 turns */
+} BwppCudaRopeTable;
+
+/* Host only.  BWPP_CUDA_ERR_ARG for a configuration without meaning. */
+int bwpp_cuda_rope_table(BwppCudaRopeTable *table, const BwppCudaRopeConfig *config);
+
+/* q and k (heads_k 0: q alone; heads_q 0: k alone) of `tokens` rows.  Token
+ * major: head h of row r at r*ld + h*head_dim (a slice of a fused qkv product
+ * will do).  Head major: [tokens / seq, heads, seq, ld], the layout of
+ * bwpp_cuda_attention_bf16 with ld == head_dim.  Row r is at positions[r], or
+ * with positions NULL at pos0 + r % seq (seq 0: tokens). */
+typedef struct {
+  uint32_t tokens, heads_q, heads_k, head_dim;
+  uint32_t ldq, ldk, ldq_out, ldk_out;
+  uint32_t seq;
+  int32_t pos0;
+  int interleaved;      /* pairs (2i, 2i+1); else (i, i + rotary_dim/2) */
+  int inverse;          /* turns back: the gradient of the forward call */
+  int head_major_in, head_major_out;
+} BwppCudaRopeParams;
+
+/* Columns of a head behind rotary_dim are copied.  q_out may be q and k_out
+ * may be k (same layout and pitch); otherwise outputs overlap no input.
+ * Arithmetic in fp32, one rounding; angles exact for all 32-bit positions. */
+int bwpp_cuda_rope_bf16(BwppCudaCtx *ctx, const uint16_t *q, const uint16_t *k, uint16_t *q_out,
+                        uint16_t *k_out, const int32_t *positions, const BwppCudaRopeTable *table,
+                        const BwppCudaRopeParams *params);
+int bwpp_cuda_rope_f16(BwppCudaCtx *ctx, const uint16_t *q, const uint16_t *k, uint16_t *q_out,
+                       uint16_t *k_out, const int32_t *positions, const BwppCudaRopeTable *table,
+                       const BwppCudaRopeParams *params);
+int bwpp_cuda_rope_f32(BwppCudaCtx *ctx, const float *q, const float *k, float *q_out, float *k_out,
+                       const int32_t *positions, const BwppCudaRopeTable *table,
+                       const BwppCudaRopeParams *params);
+
+/* The junction between two decoder blocks: the norm after a block, its gate,
+ * the scaled residual sum and the norm before the next block, in one pass.
+ *   u  = norm_after ? b / sqrt(mean(b^2) + eps_post) * gain_post : b
+ *   h' = scale_h * h + scale_b * gate * u
+ *   y  = h' / sqrt(mean(h'^2) + eps_pre) * gain_pre
+ * The stream h, the gains [cols] and the gate are fp32; b and y have the
+ * call's type.  Gains and gate may be NULL (1), y NULL (not computed).  Row r
+ * takes gate row r / gate_rows: 1 a gate per token, the sequence length one
+ * per sequence, rows (or 0) one for all.  h_out may be h. */
+typedef struct {
+  uint32_t rows, cols;
+  uint32_t ldh, ldb, ldy, ldgate;  /* pitches of h/h_out/dh_out/dh, b/db, y/dy, gate/dgate */
+  uint32_t gate_rows;
+  int norm_after;
+  float scale_h, scale_b;
+  float eps_post, eps_pre;
+} BwppCudaJunctionParams;
+
+int bwpp_cuda_junction_fwd_f32(BwppCudaCtx *ctx, const float *h, const float *b,
+                               const float *gain_post, const float *gate, const float *gain_pre,
+                               float *h_out, float *y, const BwppCudaJunctionParams *params);
+int bwpp_cuda_junction_fwd_bf16(BwppCudaCtx *ctx, const float *h, const uint16_t *b,
+                                const float *gain_post, const float *gate, const float *gain_pre,
+                                float *h_out, uint16_t *y, const BwppCudaJunctionParams *params);
+int bwpp_cuda_junction_fwd_f16(BwppCudaCtx *ctx, const float *h, const uint16_t *b,
+                               const float *gain_post, const float *gate, const float *gain_pre,
+                               float *h_out, uint16_t *y, const BwppCudaJunctionParams *params);
+
+/* Scratch bytes of the backward. */
+size_t bwpp_cuda_junction_bwd_workspace_size(BwppCudaCtx *ctx, uint32_t rows, uint32_t cols,
+                                             uint32_t gate_rows);
+/* From the forward's h_out and b, the gradient dh_out of h_out (NULL: zero) and
+ * dy of y (NULL: zero): dh, db, dgain_post, dgate (laid out like the gate) and
+ * dgain_pre, each overwritten, or skipped where NULL.  dh may be dh_out; db may
+ * not be b.  Column sums run in a fixed order: results repeat bit for bit. */
+int bwpp_cuda_junction_bwd_f32(BwppCudaCtx *ctx, const float *h_out, const float *b,
+                               const float *gain_post, const float *gate, const float *gain_pre,
+                               const float *dh_out, const float *dy, float *dh, float *db,
+                               float *dgain_post, float *dgate, float *dgain_pre,
+                               const BwppCudaJunctionParams *params);
+int bwpp_cuda_junction_bwd_bf16(BwppCudaCtx *ctx, const float *h_out, const uint16_t *b,
+                                const float *gain_post, const float *gate, const float *gain_pre,
+                                const float *dh_out, const uint16_t *dy, float *dh, uint16_t *db,
+                                float *dgain_post, float *dgate, float *dgain_pre,
+                                const BwppCudaJunctionParams *params);
+int bwpp_cuda_junction_bwd_f16(BwppCudaCtx *ctx, const float *h_out, const uint16_t *b,
+                               const float *gain_post, const float *gate, const float *gain_pre,
+                               const float *dh_out, const uint16_t *dy, float *dh, uint16_t *db,
+                               float *dgain_post, float *dgate, float *dgain_pre,
+                               const BwppCudaJunctionParams *params);
+
 /* ---- data-parallel communicator (NCCL) ----------------------------------- */
 /* The gradient allreduce of the tiny_model training step (no reference
  * counterpart: the reference has no multi-device code).  NCCL is loaded at

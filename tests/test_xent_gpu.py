@@ -1,0 +1,320 @@
+"""Softmax cross entropy over a vocabulary on the GPU, forward and gradient,
+against the formula in 64 bits.
+
+Tolerances, per element.  A logit is a sum of D bf16 products in fp32 on the
+tensor cores, 16 at a time: D / 16 + 1 additions, each off by at most 2^-22 of
+sum |x w| (the adder keeps at least 22 bits), DL = (D / 16 + 1) 2^-22 sum |x w|.
+lse and loss are off by DL, and by 2^-20 (|value| + |target's logit| + 1) for
+the exponentials, their sum and the logarithm.  dlogit = g (p - hit) is off by
+g p (2 DL + 2^-20) and rounded to bf16, half a step 2^-8; the products with it
+add (K / 16 + 1) 2^-22 of the sum of magnitudes, once more for each piece's
+sum in fp32; a bf16 gradient adds half a step of its own.
+"""
+import pytest
+import torch
+
+import bwpp
+
+pytestmark = pytest.mark.gpu
+HALF = 2.0**-8  # half a step of bf16
+
+
+def make(T, V, D, vocab_major, seed, ignored=0.2, sharp=2.0, pad=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randn(V, D, device="cuda", generator=g) * (sharp / D**0.5)).bfloat16()
+    target = torch.randint(0, V, (T,), device="cuda", generator=g)
+    lift = 4.0 * torch.rand(T, 1, device="cuda", generator=g)
+    x = (torch.randn(T, D, device="cuda", generator=g) + lift * w[target].float()).bfloat16()
+    keep = torch.rand(T, device="cuda", generator=g) >= ignored
+    target = torch.where(keep, target, -1 - target).int()
+    dloss = torch.rand(T, device="cuda", generator=g) + 0.5
+    xs = torch.full((T, D + pad), float("nan"), device="cuda").bfloat16()
+    xs[:, :D] = x
+    ws = torch.full((V, D + pad) if vocab_major else (D, V + pad), float("nan"), device="cuda").bfloat16()
+    ws[:, :D if vocab_major else V] = w if vocab_major else w.t()
+    return x, w, target, dloss, xs, ws
+
+
+def formula(x, w, target, scale):
+    """logits, lse, loss, DL per row, all in 64 bits."""
+    x, w = x.double(), w.double()
+    logits = scale * (x @ w.t())
+    lse = torch.logsumexp(logits, 1)
+    hit = logits.gather(1, target.long().clamp(min=0)[:, None])[:, 0]
+    loss = torch.where(target >= 0, lse - hit, torch.zeros_like(lse))
+    dl = (x.shape[1] // 16 + 2) * 2.0**-22 * abs(scale) * (x.abs() @ w.abs().t()).amax(1)
+    return logits, lse, loss, hit, dl
+
+
+def within(got, want, tol):
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), (float((err - tol).max()), float(err.max()))
+
+
+def check(ctx, T, V, D, vocab_major, scale=1.0, bf16=1, pad=0, seed=0, ones=False, sharp=2.0, ignored=0.2):
+    x, w, target, dloss, xs, ws = make(T, V, D, vocab_major, seed + T + V, ignored, sharp, pad)
+    ldw = ws.shape[1]
+    scale = float(torch.tensor(scale))
+    loss, lse = (torch.full((T,), float("nan"), device="cuda") for _ in range(2))
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D + pad, ldw, w_vocab_major=vocab_major, scale=scale)
+    ctx.sync()
+    logits, wlse, wloss, hit, dl = formula(x, w, target, scale)
+    tol = 2 * dl + 2.0**-20 * (wlse.abs() + hit.abs() + 1)
+    within(lse, wlse, tol)
+    within(loss, wloss, tol)
+    assert not bool(loss[target < 0].any())
+
+    t = torch.bfloat16 if bf16 else torch.float32
+    dx = torch.full((T, D + pad), 7.0, device="cuda", dtype=t)
+    dw = torch.full(tuple(ws.shape), 7.0, device="cuda", dtype=t)
+    ctx.xent_bwd(xs, ws, target, lse, None if ones else dloss, dx, dw, T, V, D, D + pad, ldw, D + pad, ldw,
+                 w_vocab_major=vocab_major, scale=scale, grads_bf16=bf16)
+    ctx.sync()
+    g = torch.where(target >= 0, torch.ones_like(wlse) if ones else dloss.double(), torch.zeros_like(wlse))
+    p = (logits - wlse[:, None]).exp()
+    d = p.clone()
+    d[torch.arange(T, device="cuda"), target.long().clamp(min=0)] -= 1.0
+    d, off = d * g[:, None] * scale, p * (g * abs(scale) * (4 * dl + 2.0**-20 * (wlse.abs() + 2)))[:, None]
+    each = off + HALF * d.abs()
+    xd, wd = x.double(), w.double()
+    out = HALF if bf16 else 2.0**-24
+    pieces = 66  # 2^-22 of a sum of magnitudes for each piece, at most 64 here
+    add = lambda K: (K // 16 + pieces) * 2.0**-22  # noqa: E731
+    within(dx[:, :D], d @ wd, (each + add(V) * d.abs()) @ wd.abs() * (1 + HALF) + out * (d @ wd).abs() + 1e-30)
+    want = d.t() @ xd
+    tol = (each + add(T) * d.abs()).t() @ xd.abs() * (1 + HALF) + out * want.abs() + 1e-30
+    got = dw[:, :D] if vocab_major else dw[:, :V].t()
+    within(got, want, tol)
+    if pad:
+        assert bool((dx[:, D:] == 7.0).all()) and bool((dw[:, D if vocab_major else V:] == 7.0).all())
+
+
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (1, 2, 8), (1, 1000, 64), (3, 257, 16), (5, 255, 33), (64, 256, 64),
+                                   (127, 1000, 72), (128, 512, 128), (129, 513, 65), (200, 3001, 100),
+                                   (257, 770, 256), (300, 5000, 520), (1, 32000, 256), (777, 1009, 101)])
+def test_sizes(ctx, T, V, D, vocab_major):
+    check(ctx, T, V, D, vocab_major, ignored=0.0 if T == 1 else 0.2)
+
+
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("kw", [dict(scale=0.125), dict(scale=-3.0), dict(bf16=0), dict(pad=8), dict(pad=3),
+                                dict(pad=3, bf16=0), dict(ones=True), dict(sharp=30.0), dict(ignored=1.0)])
+def test_options(ctx, vocab_major, kw):
+    check(ctx, 150, 1111, 136, vocab_major, **kw)
+    check(ctx, 40, 300, 31, vocab_major, **kw)
+
+
+@pytest.mark.parametrize("vocab_major", [0, 1])
+def test_several_pieces(ctx, vocab_major):
+    """Enough rows that the vocabulary goes by in several pieces, the last short."""
+    check(ctx, 9000, 9003 if vocab_major else 9000, 64, vocab_major, bf16=vocab_major)
+
+
+def test_ignored_rows_may_hold_anything(ctx):
+    T, V, D = 70, 520, 96
+    x, w, target, dloss, xs, ws = make(T, V, D, 1, 5)
+    target[::3] = -100
+    good = xs.clone()
+    xs[::3] = float("nan")
+    xs[3, 5] = float("inf")
+    outs = []
+    for src in (good, xs):
+        loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        ctx.xent_fwd(src, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1)
+        ctx.xent_bwd(src, ws, target, lse, dloss, dx, dw, T, V, D, D, D, D, D, w_vocab_major=1, grads_bf16=1)
+        ctx.sync()
+        outs.append((loss, dx, dw))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert not bool(outs[1][1][::3].any())
+
+
+def test_target_outside_the_vocabulary_is_reported(ctx):
+    T, V, D = 20, 100, 32
+    x, w, target, dloss, xs, ws = make(T, V, D, 1, 6, ignored=0.0)
+    want_dw, dw = torch.empty_like(w), torch.empty_like(w)
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    dx = torch.empty_like(x)
+    target[4] = -1
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1)
+    ctx.xent_bwd(xs, ws, target, lse, dloss, dx, want_dw, T, V, D, D, D, D, D, w_vocab_major=1, grads_bf16=1)
+    ctx.sync()
+    for bad in (V, 2**31 - 1):
+        target[4] = bad
+        ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1)
+        with pytest.raises(bwpp.BwppError) as e:
+            ctx.sync()
+        assert e.value.status == bwpp.ERR_ARG
+        assert bool(torch.isnan(loss[4])) and int(torch.isnan(loss).sum()) == 1
+        ctx.xent_bwd(xs, ws, target, lse, dloss, dx, dw, T, V, D, D, D, D, D, w_vocab_major=1, grads_bf16=1)
+        with pytest.raises(bwpp.BwppError) as e:
+            ctx.sync()
+        assert e.value.status == bwpp.ERR_ARG
+        assert torch.equal(dw, want_dw) and not bool(dx[4].any())
+    ctx.sync()
+
+
+def test_large_logits_and_infinities(ctx):
+    """Logits of +-3000 neither overflow nor lose the sum; -inf logits drop out;
+    a NaN row stays alone."""
+    T, V, D = 9, 600, 8
+    x, w, target, _, xs, ws = make(T, V, D, 1, 7, ignored=0.0)
+    xs[0] *= 2000
+    xs[1] *= -2000
+    xs[2, 3] = float("nan")
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1)
+    ctx.sync()
+    _, wlse, wloss, hit, dl = formula(xs, w, target, 1.0)
+    rows = [0, 1, 3, 4, 5, 6, 7, 8]
+    tol = 2 * dl + 2.0**-20 * (wlse.abs() + hit.abs() + 1)
+    within(lse[rows], wlse[rows], tol[rows])
+    within(loss[rows], wloss[rows], tol[rows])
+    assert bool(torch.isnan(loss[2]))
+    ws[5] = float("-inf")  # with positive x: a logit of -inf
+    xs[:] = xs.abs().nan_to_num(1.0)
+    target[:] = 7
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1)
+    ctx.sync()
+    keep = [v for v in range(V) if v != 5]
+    _, wlse, _, _, dl = formula(xs, w[keep], torch.zeros_like(target), 1.0)
+    within(lse, wlse, 2 * dl + 2.0**-20 * (wlse.abs() + 1))
+
+
+def test_one_output_at_a_time(ctx):
+    T, V, D = 130, 700, 64
+    x, w, target, dloss, xs, ws = make(T, V, D, 0, 9)
+    loss, lse, l1, l2 = (torch.empty(T, device="cuda") for _ in range(4))
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, V)
+    ctx.xent_fwd(xs, ws, target, l1, None, T, V, D, D, V)
+    ctx.xent_fwd(xs, ws, None, None, l2, T, V, D, D, V)
+    dx, dw, d1, d2 = torch.empty_like(x), torch.empty_like(ws), torch.empty_like(x), torch.empty_like(ws)
+    a = (T, V, D, D, V, D, V)
+    ctx.xent_bwd(xs, ws, target, lse, dloss, dx, dw, *a, grads_bf16=1)
+    ctx.xent_bwd(xs, ws, target, lse, dloss, d1, None, *a, grads_bf16=1)
+    ctx.xent_bwd(xs, ws, target, lse, dloss, None, d2, *a, grads_bf16=1)
+    ctx.sync()
+    assert torch.equal(loss, l1) and torch.equal(lse, l2) and torch.equal(dx, d1) and torch.equal(dw, d2)
+
+
+def test_gradient_by_differences(ctx):
+    """d sum(dloss loss) along random directions, by central differences of the
+    64-bit formula; the kernel's gradient carries bf16's half step twice."""
+    T, V, D = 24, 400, 64
+    x, w, target, dloss, xs, ws = make(T, V, D, 1, 11)
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    dx, dw = torch.empty(T, D, device="cuda"), torch.empty(V, D, device="cuda")
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1, scale=0.5)
+    ctx.xent_bwd(xs, ws, target, lse, dloss, dx, dw, T, V, D, D, D, D, D, w_vocab_major=1, scale=0.5)
+    ctx.sync()
+
+    def f(x, w):
+        return float((formula(x, w, target, 0.5)[2] * dloss.double()).sum())
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    for arg, grad in ((0, dx), (1, dw)):
+        at = [x.double(), w.double()]
+        d = torch.randn(at[arg].shape, device="cuda", generator=gen, dtype=torch.float64)
+        up, dn = list(at), list(at)
+        up[arg], dn[arg] = at[arg] + 1e-4 * d, at[arg] - 1e-4 * d
+        num = (f(*up) - f(*dn)) / 2e-4
+        terms = grad.double() * d
+        # each element is within half a step of bf16 of the sum of its terms'
+        # magnitudes, at most sqrt(V) or sqrt(T) times its own size; the
+        # directions are random, so elements' errors add as a root
+        tol = 4 * HALF * float(terms.square().sum().sqrt()) * max(V, T) ** 0.5 + 1e-5
+        assert abs(num - float(terms.sum())) <= tol, (arg, num, float(terms.sum()), tol)
+
+
+def test_no_rows_and_refusals(ctx):
+    z = torch.zeros(16, 16, device="cuda").bfloat16()
+    t = torch.zeros(16, device="cuda").int()
+    f = torch.zeros(16, device="cuda")
+    dw = torch.full((16, 16), 3.0, device="cuda").bfloat16()
+    ctx.xent_fwd(z, z, t, f, f, 0, 16, 16, 16, 16)
+    ctx.xent_bwd(z, z, t, f, None, z, dw, 0, 16, 8, 8, 16, 8, 16, grads_bf16=1)
+    ctx.sync()
+    assert not bool(dw[:8].any()) and bool((dw[8:] == 3.0).all())
+
+    def refused(fn, *a, **kw):
+        with pytest.raises(bwpp.BwppError) as e:
+            fn(*a, **kw)
+        assert e.value.status == bwpp.ERR_ARG
+
+    fw, bw = ctx.xent_fwd, ctx.xent_bwd
+    refused(fw, z, z, t, f, f, 16, 0, 16, 16, 16)
+    refused(fw, z, z, t, f, f, 16, 16, 0, 16, 16)
+    refused(fw, z, z, t, f, f, 16, 16, 16, 15, 16)
+    refused(fw, z, z, t, f, f, 16, 16, 16, 16, 15)
+    refused(fw, z, z, t, f, f, 16, 16, 16, 16, 16, scale=float("nan"))
+    refused(fw, None, z, t, f, f, 16, 16, 16, 16, 16)
+    refused(fw, z, None, t, f, f, 16, 16, 16, 16, 16)
+    refused(fw, z, z, None, f, f, 16, 16, 16, 16, 16)
+    refused(fw, z, z, t, None, None, 16, 16, 16, 16, 16)
+    refused(bw, z, z, t, f, None, z, dw, 16, 16, 16, 16, 16, 15, 16)
+    refused(bw, z, z, t, f, None, z, dw, 16, 16, 16, 16, 16, 16, 15)
+    refused(bw, z, z, None, f, None, z, dw, 16, 16, 16, 16, 16, 16, 16)
+    refused(bw, z, z, t, None, None, z, dw, 16, 16, 16, 16, 16, 16, 16)
+    ctx.xent_bwd(z, z, t, f, None, None, None, 16, 16, 16, 16, 16, 16, 16)
+    ctx.sync()
+
+
+def test_rows_past_32_bits(ctx):
+    ld = 2**31
+    T, V, D = 3, 300, 64
+    x, w, target, dloss, _, ws = make(T, V, D, 1, 13, ignored=0.0)
+    far = torch.empty(2 * ld + D, dtype=torch.bfloat16, device="cuda")
+    torch.as_strided(far, (T, D), (ld, 1)).copy_(x)
+    got, want = [], []
+    for src, pitch, out in ((x, D, want), (far, ld, got)):
+        loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        ctx.xent_fwd(src, ws, target, loss, lse, T, V, D, pitch, D, w_vocab_major=1)
+        ctx.xent_bwd(src, ws, target, lse, dloss, dx, dw, T, V, D, pitch, D, D, D, w_vocab_major=1, grads_bf16=1)
+        ctx.sync()
+        out += [loss, lse, dx, dw]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_and_replayed(ctx):
+    """Forward and gradient in one graph with a caller's workspace, replayed on
+    new inputs; without a workspace the capture is refused."""
+    T, V, D = 400, 2100, 128
+    stream = torch.cuda.Stream()
+    c = bwpp.Ctx(0, stream.cuda_stream)
+    x, w, target, dloss, xs, ws = make(T, V, D, 0, 15)
+    need = max(bwpp.xent_workspace_size(T, V, D, D, ws.shape[1], 0, b, 1) for b in (0, 1))
+    room = torch.empty(need, dtype=torch.uint8, device="cuda")
+    bufs = [[torch.empty(T, device="cuda"), torch.empty(T, device="cuda"), torch.empty_like(x), torch.empty_like(ws)]
+            for _ in range(2)]
+
+    def run(k, o):
+        k.xent_fwd(xs, ws, target, o[0], o[1], T, V, D, D, V)
+        k.xent_bwd(xs, ws, target, o[1], dloss, o[2], o[3], T, V, D, D, V, D, V, grads_bf16=1)
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(bwpp.BwppError) as e:
+            run(c, bufs[0])
+        assert e.value.status == bwpp.ERR_UNSUPPORTED
+        c.set_workspace(room, need)
+        run(c, bufs[0])
+    k = bwpp.Ctx(0)
+    other = torch.empty(need, dtype=torch.uint8, device="cuda")
+    k.set_workspace(other, need)
+    for seed in (1, 2, 3):
+        xs.copy_(make(T, V, D, 0, seed)[4])
+        graph.replay()
+        torch.cuda.synchronize()
+        run(k, bufs[1])
+        k.sync()
+        assert all(torch.equal(a, b) for a, b in zip(*bufs))
+    c.set_workspace(room, 256)
+    with pytest.raises(bwpp.BwppError) as e:
+        run(c, bufs[0])
+    assert e.value.status == bwpp.ERR_NOMEM
+    del graph
+    c.close()
+    k.close()
