@@ -6,11 +6,11 @@
 //   dlogit[t, v] = dloss[t] (exp(logit - lse) - [v == target])
 //   dx = scale dlogit W;   dW = scale dlogit^T x
 //
-// The vocabulary goes by in pieces of C columns.  Forward: a piece's logits
-// are one tensor-core product, folded into each row's running maximum, sum of
-// exponentials and target logit.  Backward: a piece's logits are computed
-// again (they were not kept), turned into bf16 dlogit, and two more products
-// add the piece's share to dx and write its part of dW.
+// The products run on the tensor cores (xent_tc.cu): the forward's logits are
+// folded into a (maximum, sum) pair per row and 128 columns in the product's
+// epilogue.  The backward computes them again, a piece of the vocabulary at a
+// time, and writes bf16 dlogit; two GEMMs add the piece's share to dx (in
+// fp32) and write its part of dW.
 //
 // A negative target ignores its row: loss 0, no share in any gradient (its x
 // may hold anything, so the backward reads a copy of x with such rows zeroed:
@@ -23,7 +23,7 @@
 
 #include "bwpp_cuda_internal.cuh"
 #include "elem.cuh"
-#include "rowwise.cuh"
+#include "xent.cuh"
 
 int bwpp_gemm_launch_dt(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint32_t lda,
                         const uint16_t *b, int b_mn, uint32_t ldb, void *c,
@@ -35,107 +35,88 @@ int bwpp_gemm_launch_dt(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint32_t 
 namespace {
 
 using bwpp_elem::aligned_to;
-using bwpp_row::block_sum;
 
 constexpr int kThreads = 256;
 
-// dst[r, c] = src[r, c] of 16-bit elements; rows whose target is ignored
-// become zero (target != NULL).
+// dst[r, c] = src[r, c] of 16-bit elements, eight a thread, into rows of 16
+// bytes (the last eight filled up with zeros).  With targets, rows that are
+// ignored become zero, and a target outside the vocabulary is reported.
 __global__ void __launch_bounds__(kThreads)
     pack_rows_kernel(const uint16_t *__restrict__ src, uint16_t *__restrict__ dst, uint32_t rows,
-                     uint32_t cols, size_t ld_src, size_t ld_dst, const int32_t *target,
-                     uint32_t V) {
-  for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const bool live = !target || (uint32_t)target[r] < V;
-    for (uint32_t c = threadIdx.x; c < cols; c += kThreads)
-      dst[r * ld_dst + c] = live ? src[r * ld_src + c] : (uint16_t)0;
+                     uint32_t cols, size_t ld_src, size_t ld_dst, int wide, const int32_t *target,
+                     uint32_t V, int *status) {
+  const uint32_t chunks = (cols + 7) / 8, i = blockIdx.x * kThreads + threadIdx.x;
+  if (i >= rows * chunks) return;
+  const uint32_t r = i / chunks, c = (i - r * chunks) * 8;
+  bool live = true;
+  if (target) {
+    const int32_t y = target[r];
+    live = (uint32_t)y < V;
+    if (y >= 0 && !live && c == 0) bwpp_report(status, BWPP_CUDA_ERR_ARG);
   }
-}
-
-// Results from scratch into rows of any pitch.
-__global__ void __launch_bounds__(kThreads)
-    unpack_rows_kernel(const void *__restrict__ src, void *__restrict__ dst, uint32_t rows,
-                       uint32_t cols, size_t ld_src, size_t ld_dst, int bf16) {
-  for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (uint32_t c = threadIdx.x; c < cols; c += kThreads) {
-      if (bf16)
-        static_cast<uint16_t *>(dst)[r * ld_dst + c] =
-            static_cast<const uint16_t *>(src)[r * ld_src + c];
-      else
-        static_cast<float *>(dst)[r * ld_dst + c] = static_cast<const float *>(src)[r * ld_src + c];
-    }
-}
-
-// Folds the logits of vocabulary columns [v0, v0 + n) into the rows' state:
-// [T] maximum, [T] sum of exponentials over it, [T] the target's logit.
-__global__ void __launch_bounds__(kThreads)
-    fold_kernel(const float *__restrict__ logits, uint32_t ld, uint32_t n, uint32_t v0, float scale,
-                const int32_t *__restrict__ target, float *__restrict__ state, uint32_t T) {
-  __shared__ float red[32];
-  const uint32_t t = blockIdx.x;
-  const float *row = logits + (size_t)t * ld;
-  float m = -INFINITY;
-  for (uint32_t c = threadIdx.x; c < n; c += kThreads) m = fmaxf(m, scale * row[c]);
+  uint4 t = make_uint4(0u, 0u, 0u, 0u);
+  if (live) {
+    const uint16_t *p = src + r * ld_src + c;
+    if (wide && c + 8 <= cols) {
+      t = __ldg(reinterpret_cast<const uint4 *>(p));
+    } else {
+      uint32_t w[8];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
-  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, red[w]);
-  const float before = v0 ? state[t] : -INFINITY;
-  const float top = fmaxf(m, before);
-  // rows of infinities: exp(-inf - -inf) is 0 here
-  const float base = isinf(top) && top < 0 ? 0.0f : top;
-  float s[1] = {0.0f};
-  for (uint32_t c = threadIdx.x; c < n; c += kThreads) s[0] += expf(scale * row[c] - base);
-  block_sum<1>(s, red);
-  if (threadIdx.x == 0) {
-    state[t] = top;
-    state[T + t] = s[0] + (v0 ? state[T + t] * expf(before - base) : 0.0f);
-    if (target) {
-      const uint32_t at = (uint32_t)target[t] - v0;
-      if ((uint32_t)target[t] >= v0 && at < n) state[2 * (size_t)T + t] = scale * row[at];
+      for (int e = 0; e < 8; ++e) w[e] = c + e < cols ? __ldg(p + e) : 0u;
+      t = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
   }
+  *reinterpret_cast<uint4 *>(dst + r * ld_dst + c) = t;
 }
 
+// Results from 16-byte rows of scratch into rows of any pitch, ES bytes an
+// element, 16 bytes a thread.
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    finish_kernel(const float *__restrict__ state, const int32_t *__restrict__ target,
-                  float *__restrict__ loss, float *__restrict__ lse, uint32_t T, uint32_t V,
-                  int *status) {
-  const uint32_t t = blockIdx.x * kThreads + threadIdx.x;
-  if (t >= T) return;
-  const float l = state[t] + logf(state[T + t]);
-  if (lse) lse[t] = l;
-  if (loss) {
-    const int32_t y = target[t];
-    float v = 0.0f;
-    if (y >= 0) {
-      v = l - state[2 * (size_t)T + t];
-      if ((uint32_t)y >= V) {
-        v = NAN;
-        bwpp_report(status, BWPP_CUDA_ERR_ARG);
-      }
-    }
-    loss[t] = v;
-  }
+    unpack_rows_kernel(const T *__restrict__ src, T *__restrict__ dst, uint32_t rows, uint32_t cols,
+                       size_t ld_src, size_t ld_dst) {
+  constexpr uint32_t N = 16 / sizeof(T);
+  const uint32_t chunks = (cols + N - 1) / N, i = blockIdx.x * kThreads + threadIdx.x;
+  if (i >= rows * chunks) return;
+  const uint32_t r = i / chunks, c = (i - r * chunks) * N;
+  union {
+    uint4 q;
+    T e[N];
+  } t;
+  t.q = *reinterpret_cast<const uint4 *>(src + r * ld_src + c);
+#pragma unroll
+  for (uint32_t e = 0; e < N; ++e)
+    if (c + e < cols) dst[r * ld_dst + c + e] = t.e[e];
 }
 
-// bf16 scale * dlogit of vocabulary columns [v0, v0 + n).
-__global__ void __launch_bounds__(kThreads)
-    dlogit_kernel(const float *__restrict__ logits, uint32_t ld, uint32_t n, uint32_t v0,
-                  float scale, const int32_t *__restrict__ target, const float *__restrict__ lse,
-                  const float *__restrict__ dloss, uint16_t *__restrict__ out, uint32_t ldo,
-                  uint32_t V, int *status) {
-  const uint32_t t = blockIdx.x;
-  const int32_t y = target[t];
-  const bool live = (uint32_t)y < V;
-  if (y >= 0 && !live && threadIdx.x == 0) bwpp_report(status, BWPP_CUDA_ERR_ARG);
-  const float l = lse[t], g = scale * (dloss ? dloss[t] : 1.0f);
-  for (uint32_t c = threadIdx.x; c < n; c += kThreads) {
-    const float p = expf(scale * logits[(size_t)t * ld + c] - l);
-    const float d = live ? g * (v0 + c == (uint32_t)y ? p - 1.0f : p) : 0.0f;
-    out[(size_t)t * ldo + c] = (uint16_t)(pack2_16<false>(d, 0.0f) & 0xFFFFu);
+int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t rows, uint32_t cols,
+              uint32_t ld_src, uint32_t ld_dst, const int32_t *target, uint32_t V) {
+  const uint32_t chunks = (cols + 7) / 8;
+  const int wide = ld_src % 8 == 0 && aligned_to(src, 16);
+  const uint32_t most = (1u << 30) / chunks;  // rows of a launch: indices stay in 31 bits
+  for (uint32_t r0 = 0; r0 < rows; r0 += most) {
+    const uint32_t n = rows - r0 < most ? rows - r0 : most;
+    pack_rows_kernel<<<(n * chunks + kThreads - 1) / kThreads, kThreads, 0, ctx->stream>>>(
+        src + (size_t)r0 * ld_src, dst + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst, wide,
+        target ? target + r0 : nullptr, V, ctx->status_word);
+    BWPP_LAUNCH_CHECK(ctx, "xent pack");
   }
+  return BWPP_CUDA_OK;
+}
+
+template <typename T>
+int unpack_rows(BwppCudaCtx *ctx, const void *src, void *dst, uint32_t rows, uint32_t cols,
+                uint32_t ld_src, uint32_t ld_dst) {
+  const uint32_t chunks = (cols + 16 / sizeof(T) - 1) / (16 / sizeof(T));
+  const uint32_t most = (1u << 30) / chunks;
+  for (uint32_t r0 = 0; r0 < rows; r0 += most) {
+    const uint32_t n = rows - r0 < most ? rows - r0 : most;
+    unpack_rows_kernel<T><<<(n * chunks + kThreads - 1) / kThreads, kThreads, 0, ctx->stream>>>(
+        static_cast<const T *>(src) + (size_t)r0 * ld_src, static_cast<T *>(dst) + (size_t)r0 * ld_dst,
+        n, cols, ld_src, ld_dst);
+    BWPP_LAUNCH_CHECK(ctx, "xent unpack");
+  }
+  return BWPP_CUDA_OK;
 }
 
 inline uint32_t up8(uint32_t n) { return (n + 7) & ~7u; }
@@ -145,22 +126,25 @@ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct Layout {
   uint32_t piece;             // vocabulary columns of a piece
   uint32_t dp;                // D rounded up
-  size_t state, x, w, logits, dlogit, dx, dx16, dw, total;
+  size_t part, hit, x, w, dlogit, dx, dx16, dw, total;
 };
 
-// Vocabulary columns of a piece: about 2^26 logits at a time.
-uint32_t piece_of(uint32_t T, uint32_t V) {
-  uint64_t c = ((1ull << 26) / (T ? T : 1)) & ~255ull;
+uint32_t clamp_piece(uint64_t c, uint32_t V) {
+  c &= ~255ull;
   if (c < 1024) c = 1024;
   const uint64_t all = ((uint64_t)V + 255) & ~255ull;
   return (uint32_t)(c < all ? c : all);
 }
 
+// Vocabulary columns of a piece.  Backward: about 2^26 dlogit at a time.
+// Forward: the whole vocabulary, or about 2^25 weights at a time where they
+// are packed.
 Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool backward, bool stage_dx,
                  bool stage_dw) {
   Layout l{};
-  l.piece = piece_of(p.T, p.V);
   l.dp = up8(p.D);
+  l.piece = backward ? clamp_piece((1ull << 26) / p.T, p.V)
+                     : clamp_piece(pack_w ? (1ull << 25) / l.dp : (uint64_t)p.V + 255, p.V);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -168,11 +152,12 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
     return here;
   };
   const size_t es = p.grads_bf16 ? 2 : 4;
-  l.logits = take((size_t)p.T * l.piece * 4);
-  if (!backward) l.state = take((size_t)p.T * 12);
   if (pack_x || backward) l.x = take((size_t)p.T * l.dp * 2);
   if (pack_w) l.w = take((size_t)l.piece * l.dp * 2);
-  if (backward) {
+  if (!backward) {
+    l.part = take((((size_t)p.V + 127) / 128) * p.T * sizeof(float2));
+    l.hit = take((size_t)p.T * 4);
+  } else {
     l.dlogit = take((size_t)p.T * l.piece * 2);
     if (stage_dx) {
       l.dx = take((size_t)p.T * l.dp * 4);
@@ -186,17 +171,13 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
 
 int check(BwppCudaCtx *ctx, const BwppCudaXentParams *p) {
   if (!p) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: NULL params");
-  if (p->V == 0 || p->D == 0 || p->V > 0x7fffffffu || p->T > 0x7fffffffu)
-    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: V and D must be positive, V and T < 2^31");
+  if (p->V == 0 || p->D == 0 || p->V > 0x7ffffe00u || p->T > 0x7ffffe00u)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG,
+                          "xent: V and D must be positive, V and T at most 2^31 - 512");
   if (p->ldx < p->D || p->ldw < (p->w_vocab_major ? p->D : p->V))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: leading dim smaller than row");
   if (!isfinite(p->scale)) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: scale is not finite");
   return BWPP_CUDA_OK;
-}
-
-inline unsigned row_blocks(BwppCudaCtx *ctx, uint32_t rows) {
-  const uint32_t most = (uint32_t)ctx->num_sms * 8;
-  return rows < most ? rows : most;
 }
 
 // The piece [v0, v0 + n) of W as a GEMM operand.
@@ -211,11 +192,8 @@ int piece_w(BwppCudaCtx *ctx, const BwppCudaXentParams &p, const uint16_t *w, bo
   out = Piece{src, p.ldw};
   if (!pack) return BWPP_CUDA_OK;
   const uint32_t rows = p.w_vocab_major ? n : p.D, cols = p.w_vocab_major ? p.D : n;
-  pack_rows_kernel<<<row_blocks(ctx, rows), kThreads, 0, ctx->stream>>>(src, scratch, rows, cols,
-                                                                       p.ldw, ld_packed, nullptr, 0);
-  BWPP_LAUNCH_CHECK(ctx, "xent pack");
   out = Piece{scratch, ld_packed};
-  return BWPP_CUDA_OK;
+  return pack_rows(ctx, src, scratch, rows, cols, p.ldw, ld_packed, nullptr, 0);
 }
 
 bool needs_pack(const void *base, uint32_t ld) { return ld % 8 != 0 || !aligned_to(base, 16); }
@@ -244,33 +222,26 @@ int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   uint8_t *scratch;
   rc = bwpp_op_scratch(ctx, l.total, "xent fwd", &scratch);
   if (rc) return rc;
-  cudaStream_t s = ctx->stream;
   uint32_t ldx = p.ldx;
   if (pack_x) {
     uint16_t *xp = reinterpret_cast<uint16_t *>(scratch + l.x);
-    pack_rows_kernel<<<row_blocks(ctx, p.T), kThreads, 0, s>>>(x, xp, p.T, p.D, p.ldx, l.dp, nullptr, 0);
-    BWPP_LAUNCH_CHECK(ctx, "xent pack");
+    rc = pack_rows(ctx, x, xp, p.T, p.D, p.ldx, l.dp, nullptr, 0);
+    if (rc) return rc;
     x = xp;
     ldx = l.dp;
   }
-  float *logits = reinterpret_cast<float *>(scratch + l.logits);
-  float *state = reinterpret_cast<float *>(scratch + l.state);
+  float2 *part = reinterpret_cast<float2 *>(scratch + l.part);
+  float *hit = reinterpret_cast<float *>(scratch + l.hit);
   for (uint32_t v0 = 0; v0 < p.V; v0 += l.piece) {
     const uint32_t n = p.V - v0 < l.piece ? p.V - v0 : l.piece;
     Piece w1;
     rc = piece_w(ctx, p, w, pack_w, reinterpret_cast<uint16_t *>(scratch + l.w), v0, n,
                  p.w_vocab_major ? l.dp : l.piece, w1);
-    if (!rc)
-      rc = bwpp_gemm_launch_dt(ctx, x, 0, ldx, w1.w, p.w_vocab_major ? 0 : 1, w1.ld, logits, l.piece,
-                               p.T, n, p.D, nullptr, 0, nullptr, 0, 0, 0, 0, 0, 0);
+    const XentOperands o{x, w1.w, p.T, n, p.D, ldx, w1.ld, v0, p.V, p.w_vocab_major != 0, p.scale};
+    if (!rc) rc = bwpp_xent_stats_launch(ctx, o, loss ? target : nullptr, part + (size_t)(v0 / 128) * p.T, hit);
     if (rc) return rc;
-    fold_kernel<<<p.T, kThreads, 0, s>>>(logits, l.piece, n, v0, p.scale, target, state, p.T);
-    BWPP_LAUNCH_CHECK(ctx, "xent fold");
   }
-  finish_kernel<<<(p.T + kThreads - 1) / kThreads, kThreads, 0, s>>>(state, target, loss, lse, p.T,
-                                                                     p.V, ctx->status_word);
-  BWPP_LAUNCH_CHECK(ctx, "xent finish");
-  return BWPP_CUDA_OK;
+  return bwpp_xent_combine_launch(ctx, part, (p.V + 127) / 128, hit, target, loss, lse, p.T, p.V);
 }
 
 int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,
@@ -283,20 +254,19 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   const uint32_t es = p.grads_bf16 ? 2 : 4;
   if ((dx && p.lddx < p.D) || (dw && p.lddw < (p.w_vocab_major ? p.D : p.V)))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent bwd: leading dim smaller than row");
-  cudaStream_t s = ctx->stream;
   if (p.T == 0) {  // no rows: dW is zero
     if (!dw) return BWPP_CUDA_OK;
     return bwpp_check_cuda(
         ctx,
         cudaMemset2DAsync(dw, (size_t)p.lddw * es, 0, (size_t)(p.w_vocab_major ? p.D : p.V) * es,
-                          p.w_vocab_major ? p.V : p.D, s),
+                          p.w_vocab_major ? p.V : p.D, ctx->stream),
         "xent memset");
   }
   if (!dx && !dw) return BWPP_CUDA_OK;
   if (!x || !w || !target || !lse)
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent bwd: NULL buffer");
   const bool pack_w = needs_pack(w, p.ldw);
-  const uint32_t piece = piece_of(p.T, p.V);
+  const uint32_t piece = layout_of(p, true, pack_w, true, true, true).piece;
   const bool one = piece >= p.V;
   auto tma_out = [&](const void *q, uint32_t ld) { return (size_t)ld * es % 16 == 0 && aligned_to(q, 16); };
   // dx is summed over the pieces in fp32: in place where the caller's rows
@@ -308,9 +278,8 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   rc = bwpp_op_scratch(ctx, l.total, "xent bwd", &scratch);
   if (rc) return rc;
   uint16_t *xp = reinterpret_cast<uint16_t *>(scratch + l.x);
-  pack_rows_kernel<<<row_blocks(ctx, p.T), kThreads, 0, s>>>(x, xp, p.T, p.D, p.ldx, l.dp, target, p.V);
-  BWPP_LAUNCH_CHECK(ctx, "xent pack");
-  float *logits = reinterpret_cast<float *>(scratch + l.logits);
+  rc = pack_rows(ctx, x, xp, p.T, p.D, p.ldx, l.dp, target, p.V);
+  if (rc) return rc;
   uint16_t *dlogit = reinterpret_cast<uint16_t *>(scratch + l.dlogit);
   float *dx32 = reinterpret_cast<float *>(scratch + l.dx);
   for (uint32_t v0 = 0; v0 < p.V; v0 += piece) {
@@ -319,13 +288,9 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     Piece w1;
     rc = piece_w(ctx, p, w, pack_w, reinterpret_cast<uint16_t *>(scratch + l.w), v0, n,
                  p.w_vocab_major ? l.dp : piece, w1);
-    if (!rc)
-      rc = bwpp_gemm_launch_dt(ctx, xp, 0, l.dp, w1.w, p.w_vocab_major ? 0 : 1, w1.ld, logits, piece,
-                               p.T, n, p.D, nullptr, 0, nullptr, 0, 0, 0, 0, 0, 0);
+    const XentOperands o{xp, w1.w, p.T, n, p.D, l.dp, w1.ld, v0, p.V, p.w_vocab_major != 0, p.scale};
+    if (!rc) rc = bwpp_xent_dlogit_launch(ctx, o, target, lse, dloss, dlogit, piece);
     if (rc) return rc;
-    dlogit_kernel<<<p.T, kThreads, 0, s>>>(logits, piece, n, v0, p.scale, target, lse, dloss, dlogit,
-                                           piece, p.V, ctx->status_word);
-    BWPP_LAUNCH_CHECK(ctx, "xent dlogit");
     if (dx) {
       // dx (+)= dlogit W: the last piece leaves the sum in the caller's rows
       // where TMA can store them
@@ -339,9 +304,9 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
                                bf16_out ? 1 : 0, 0, 0, 0, 0);
       if (rc) return rc;
       if (!to_user && last) {
-        unpack_rows_kernel<<<row_blocks(ctx, p.T), kThreads, 0, s>>>(out, dx, p.T, p.D, l.dp, p.lddx,
-                                                                    p.grads_bf16);
-        BWPP_LAUNCH_CHECK(ctx, "xent unpack");
+        rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, out, dx, p.T, p.D, l.dp, p.lddx)
+                          : unpack_rows<float>(ctx, out, dx, p.T, p.D, l.dp, p.lddx);
+        if (rc) return rc;
       }
     }
     if (dw) {
@@ -359,9 +324,9 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
       if (rc) return rc;
       if (stage_dw) {
         const uint32_t rows = p.w_vocab_major ? n : p.D, cols = p.w_vocab_major ? p.D : n;
-        unpack_rows_kernel<<<row_blocks(ctx, rows), kThreads, 0, s>>>(out, user, rows, cols, ldo,
-                                                                      p.lddw, p.grads_bf16);
-        BWPP_LAUNCH_CHECK(ctx, "xent unpack");
+        rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, out, user, rows, cols, ldo, p.lddw)
+                          : unpack_rows<float>(ctx, out, user, rows, cols, ldo, p.lddw);
+        if (rc) return rc;
       }
     }
   }

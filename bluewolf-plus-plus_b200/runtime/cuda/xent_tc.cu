@@ -1,0 +1,517 @@
+// The logits of the vocabulary cross entropy on the tensor cores, used up in
+// the epilogue: they never reach memory.
+//
+// logit[t, v] = scale sum_d x[t, d] W[v, d], in tiles of 256 rows x 256
+// vocabulary columns (a CTA pair, cta_group::2) or 128 x 256 (one CTA, at most
+// 128 rows).  Persistent, warp-specialised like the GEMM (gemm.cu): warp 0
+// feeds a ring of operand stages by TMA, one thread of warp 1 issues
+// tcgen05.mma, warps 2..9 drain the accumulator; two TMEM accumulators, so the
+// epilogue of a tile runs beside the next tile's main loop.
+//
+// FWD.  An epilogue thread owns a row of the tile and 128 of its columns: the
+// running maximum and sum of 2^(logit log2 e - maximum) stay in registers over
+// its four 32-column chunks and leave as one (maximum, sum) pair per row and
+// 128 columns, 8 bytes for every 512 of logits.  xent_combine_kernel folds a
+// row's pairs.  The thread that meets the row's target writes its logit.
+// Backward.  The epilogue turns the logits into bf16 scale g (p - hit) and
+// stores the tile by TMA: 2 bytes a logit, read by the two gradient products.
+//
+// Exponentials are ex2.approx (2 ulp): one per logit, 128 x 256 of them for a
+// tile are 2048 cycles of an SM's MUFU, against 128 cycles of MMA for every 16
+// of D: below D = 256 the exponentials set the pace, above it the products.
+//
+// Every wait is bounded as in the GEMM.
+#include "bwpp_cuda_internal.cuh"
+#include "xent.cuh"
+
+namespace {
+
+constexpr int BM = 128, BN = 256, BK = 64;
+constexpr int A_STAGE = BM * BK * 2;
+constexpr int B_BOX = 64 * BK * 2;  // 64 vocabulary columns x 64 of D
+constexpr int EPI_WARPS = 8;
+constexpr int EPI_BUF = 32 * 128;   // 32 rows x 64 bf16
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr uint32_t TMEM_COLS = 2 * BN;
+constexpr uint32_t GROUP_M = 8;     // row blocks that share W panels in L2
+
+template <bool PAIR>
+struct Cfg {
+  static constexpr int STAGES = PAIR ? 6 : 4;
+  static constexpr int B_STAGE = (PAIR ? 128 : 256) * BK * 2;
+  static constexpr int OFF_B = STAGES * A_STAGE;
+  static constexpr int OFF_C = OFF_B + STAGES * B_STAGE;
+  static constexpr int OFF_BAR = OFF_C + EPI_WARPS * EPI_BUF;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;  // slack: 1024-byte alignment
+  static constexpr uint32_t TILE_M = PAIR ? 2 * BM : BM;
+  static_assert(SMEM <= 232448, "exceeds the 227 KB opt-in limit");
+  static_assert((2 * STAGES + 5) * 8 + 8 <= 256, "barrier block");
+};
+
+struct XentTile {
+  uint32_t T, V, D;     // V: columns of this launch
+  uint32_t v0;          // vocabulary index of column 0
+  float c;              // scale * log2(e)
+  const int32_t *target;
+  // FWD
+  float2 *part;         // [ceil(V / 128)][T]
+  float *hit;           // [T] logit of the target
+  // backward
+  const float *lse, *dloss;
+  float scale;
+  uint32_t vocab;       // targets below it are live
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tile_at(uint32_t i, uint32_t tiles_m, uint32_t tiles_n,
+                                        uint32_t &mb, uint32_t &nb) {
+  const uint32_t per_group = GROUP_M * tiles_n, g = i / per_group, first = g * GROUP_M;
+  const uint32_t gm = min(GROUP_M, tiles_m - first), r = i - g * per_group;
+  mb = first + r % gm;
+  nb = r / gm;
+}
+
+template <bool B_MN, bool PAIR, bool FWD>
+__global__ void __launch_bounds__(THREADS, 1)
+    xent_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmOut, const XentTile a, int *status) {
+  using C = Cfg<PAIR>;
+  constexpr int STAGES = C::STAGES;
+  constexpr uint32_t IDESC = make_idesc_bf16_f32(C::TILE_M, BN, 0u, B_MN ? 1u : 0u);
+  constexpr int B_BOXES = C::B_STAGE / B_BOX;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t *smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
+  uint64_t *empty = full + STAGES;
+  uint64_t *tfull = empty + STAGES;
+  uint64_t *tempty = tfull + 2;
+  uint64_t *drain = tempty + 2;
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const uint32_t worker = PAIR ? cluster_id_x() : blockIdx.x;
+  const uint32_t workers = PAIR ? cluster_count_x() : gridDim.x;
+  const uint32_t tiles_m = (a.T + C::TILE_M - 1) / C::TILE_M, tiles_n = (a.V + BN - 1) / BN;
+  const uint32_t tiles = tiles_m * tiles_n, num_kb = (a.D + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmW);
+    if (!FWD) prefetch_tmap(&tmOut);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_holder, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_holder, TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      for (uint32_t i = worker; i < tiles && !*abort_flag; i += workers) {
+        uint32_t mb, nb;
+        tile_at(i, tiles_m, tiles_n, mb, nb);
+        const int32_t row0 = (int32_t)(mb * C::TILE_M + rank * BM);
+        const int32_t col0 = (int32_t)(nb * BN + rank * (BN / 2));  // rank is 0 for one CTA
+        for (uint32_t kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, status)) {
+            *abort_flag = 1;
+            break;
+          }
+          // both CTAs' bytes count on rank 0's barrier
+          if (rank == 0)
+            mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * (A_STAGE + C::B_STAGE));
+          uint32_t fbar = 0;
+          if constexpr (PAIR) fbar = cluster_addr(&full[stage], 0);
+          auto load = [&](void *dst, const CUtensorMap *map, int32_t x, int32_t y) {
+            if constexpr (PAIR) tma_load_2d_pair(dst, map, fbar, x, y);
+            else tma_load_2d(dst, map, &full[stage], x, y);
+          };
+          const int32_t k0 = (int32_t)(kb * BK);
+          uint8_t *sb = smem + C::OFF_B + stage * C::B_STAGE;
+          load(smem + stage * A_STAGE, &tmX, k0, row0);
+#pragma unroll
+          for (int j = 0; j < B_BOXES; ++j) {
+            if (B_MN) load(sb + j * B_BOX, &tmW, col0 + j * 64, k0);
+            else load(sb + j * B_BOX, &tmW, k0, col0 + j * 64);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      auto commit = [&](uint64_t *bar) {
+        if constexpr (PAIR) {
+          tc_commit_pair(smem_u32(bar));
+          tc_commit_pair(cluster_addr(bar, 1));
+        } else {
+          tc_commit(bar);
+        }
+      };
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      for (uint32_t i = worker; i < tiles && !*abort_flag; i += workers) {
+        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        bool ok = true;
+        for (uint32_t kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, status)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + stage * A_STAGE);
+          const uint32_t b0 = smem_u32(smem + C::OFF_B + stage * C::B_STAGE);
+          // K-major: 16 of D are 32 bytes inside the 128-byte swizzle; MN-major:
+          // 64-column atoms 8 KB apart, 16 rows of D are 2 KB
+          const uint64_t ad = make_smem_desc(a0, 16, 1024, BWPP_SWIZZLE_128B);
+          const uint64_t bd = make_smem_desc(b0, B_MN ? B_BOX : 16, 1024, BWPP_SWIZZLE_128B);
+#pragma unroll
+          for (int ks = 0; ks < BK / 16; ++ks) {
+            const uint64_t as = desc_add(ad, ks * 32), bs = desc_add(bd, ks * (B_MN ? 2048 : 32));
+            const uint32_t accum = (kb | (uint32_t)ks) != 0 ? 1u : 0u;
+            if constexpr (PAIR) tc_mma_f16_ss_pair(tmem_base + acc * BN, as, bs, IDESC, accum);
+            else tc_mma_f16_ss(tmem_base + acc * BN, as, bs, IDESC, accum);
+          }
+          commit(&empty[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        commit(&tfull[acc]);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+      // every MMA issued here has finished before TMEM is freed
+      if constexpr (PAIR) tc_commit_pair(smem_u32(drain)); else tc_commit(drain);
+      mbar_wait(drain, 0, status);
+    }
+  } else {
+    const int q = warp & 3;            // TMEM lane quarter of this warp
+    const int ew = warp - 2;
+    const int sub = ew >> 2;           // columns [128 sub, 128 sub + 128) of the tile
+    const uint32_t tq = (uint32_t)(q * 32) << 16;
+    uint32_t acc = 0, acc_phase = 0;
+    for (uint32_t i = worker; i < tiles && !*abort_flag; i += workers) {
+      uint32_t mb, nb;
+      tile_at(i, tiles_m, tiles_n, mb, nb);
+      const uint32_t row0 = mb * C::TILE_M + rank * BM + q * 32, row = row0 + lane;
+      const uint32_t first = nb * BN + sub * 128;  // this warp's first column
+      const bool live_row = row < a.T;
+      const int32_t target = live_row && a.target ? __ldg(a.target + row) : -1;
+      // the target's column within this warp's 128, or beyond them
+      const uint32_t hit_col =
+          target >= 0 ? (uint32_t)target - a.v0 - first : 0xffffffffu;
+      float g = 0.0f, lse2 = 0.0f;
+      if constexpr (!FWD) {
+        if (live_row && (uint32_t)target < a.vocab) {
+          g = a.scale * (a.dloss ? __ldg(a.dloss + row) : 1.0f);
+          lse2 = __ldg(a.lse + row) * 1.44269504f;
+        }
+      }
+      const bool live = live_row && (uint32_t)target < a.vocab;
+      if (!mbar_wait(&tfull[acc], acc_phase, status)) {
+        *abort_flag = 1;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + tq + acc * BN + sub * 128;
+      if constexpr (FWD) {
+        if (first < a.V) {
+          float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t cs = first + k * 32;
+            if (cs >= a.V) break;
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(taddr + k * 32, r);
+            tc_wait_ld(r);
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * a.c;
+            if (hit_col - k * 32 < 32u) {
+              float h = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (hit_col - k * 32 == (uint32_t)j) h = __uint_as_float(r[j]);
+              a.hit[row] = h * a.scale;
+            }
+            if (cs + 32 > a.V) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (cs + j >= a.V) v[j] = -INFINITY;
+            }
+            float top = m;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
+            // only -inf so far, or +inf: the exponentials are taken against 0
+            const float base = fabsf(top) == INFINITY ? 0.0f : top;
+            s *= ex2(m - base);
+            float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s4[j & 3] += ex2(v[j] - base);
+            s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+            m = top;
+          }
+          if (live_row) a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);
+        }
+      } else {
+        uint8_t *stage_c = smem + C::OFF_C + ew * EPI_BUF;
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {  // 64 columns: 128 bytes of bf16
+          const uint32_t cs = first + k * 64;
+          if (cs >= a.V) break;
+          uint32_t out[32];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(taddr + k * 64 + h * 32, r);
+            tc_wait_ld(r);
+            float d[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) d[j] = ex2(__uint_as_float(r[j]) * a.c - lse2);
+            const uint32_t at = hit_col - (k * 64 + h * 32);
+            if (at < 32u) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (at == (uint32_t)j) d[j] -= 1.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              out[h * 16 + j] = live ? pack2_16<false>(g * d[2 * j], g * d[2 * j + 1]) : 0u;
+          }
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4 *>(stage_c + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < a.T) {
+            tma_store_2d(&tmOut, stage_c, (int32_t)cs, (int32_t)row0);
+            tma_store_commit();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(&tempty[acc], 0));
+        else mbar_arrive(&tempty[acc]);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (!FWD && lane == 0) tma_store_wait_all<0>();
+  }
+
+  // every wait is bounded, so both CTAs of a pair arrive here
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// lse and loss of 32 rows a block: lane = row, warp w folds the row's pairs
+// w, w + warps, ... and the warps' results meet in shared memory, in order.
+constexpr int COMBINE_WARPS = 16;
+__global__ void __launch_bounds__(32 * COMBINE_WARPS)
+    xent_combine_kernel(const float2 *__restrict__ part, uint32_t nparts, const float *__restrict__ hit,
+                        const int32_t *__restrict__ target, float *__restrict__ loss,
+                        float *__restrict__ lse, uint32_t T, uint32_t V, int *status) {
+  __shared__ float2 got[COMBINE_WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t t = blockIdx.x * 32 + lane;
+  auto fold = [](float2 &x, float2 y) {
+    const float top = fmaxf(x.x, y.x), base = fabsf(top) == INFINITY ? 0.0f : top;
+    x.y = x.y * ex2(x.x - base) + y.y * ex2(y.x - base);
+    x.x = top;
+  };
+  float2 x = make_float2(-INFINITY, 0.0f);
+  if (t < T)
+    for (uint32_t k = warp; k < nparts; k += COMBINE_WARPS) fold(x, __ldg(part + (size_t)k * T + t));
+  got[warp][lane] = x;
+  __syncthreads();
+  if (warp || t >= T) return;
+  for (int w = 1; w < COMBINE_WARPS; ++w) fold(x, got[w][lane]);
+  const float l = (x.x + log2f(x.y)) * 0.693147181f;
+  if (lse) lse[t] = l;
+  if (loss) {
+    const int32_t y = target[t];
+    float v = 0.0f;
+    if (y >= 0) {
+      if ((uint32_t)y < V) {
+        v = l - hit[t];
+      } else {
+        v = __int_as_float(0x7fc00000);
+        bwpp_report(status, BWPP_CUDA_ERR_ARG);
+      }
+    }
+    loss[t] = v;
+  }
+}
+
+bool g_smem_set[8][64] = {};
+int g_pairs[8][64] = {};  // resident CTA pairs per device (0: not asked yet)
+
+template <bool B_MN, bool PAIR, bool FWD>
+int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
+           const XentTile &a) {
+  using C = Cfg<PAIR>;
+  auto kern = xent_tc_kernel<B_MN, PAIR, FWD>;
+  const int v = (B_MN ? 1 : 0) + (PAIR ? 2 : 0) + (FWD ? 4 : 0), dev = ctx->device;
+  if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: device index >= 64");
+  if (!g_smem_set[v][dev]) {
+    const int rc = bwpp_check_cuda(
+        ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
+        "xent smem attribute");
+    if (rc) return rc;
+    g_smem_set[v][dev] = true;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctx->num_sms & ~1), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = ctx->stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  uint32_t cap = (uint32_t)ctx->num_sms;
+  if constexpr (PAIR) {
+    int &pairs = g_pairs[v][dev];
+    if (pairs == 0) {
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        pairs = -1;
+      } else {
+        pairs = n;
+      }
+    }
+    if (pairs < 0) return BWPP_CUDA_ERR_UNSUPPORTED;
+    cap = (uint32_t)pairs;
+  }
+  const uint64_t tiles = ((uint64_t)a.T + C::TILE_M - 1) / C::TILE_M * (((uint64_t)a.V + BN - 1) / BN);
+  if (tiles >= 0x80000000ull) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: T * V too large");
+  const uint32_t n = tiles < cap ? (uint32_t)tiles : cap;
+  cfg.gridDim = dim3((PAIR ? 2 : 1) * n, 1, 1);
+  int *status = ctx->status_word;
+  return bwpp_check_cuda(ctx, cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a, status),
+                         FWD ? "xent logits" : "xent dlogit");
+}
+
+template <bool FWD>
+int launch_any(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
+               const XentTile &a, bool vocab_major) {
+  if (a.T > (uint32_t)BM) {  // a pair's second CTA would otherwise have rows past T only
+    const int rc = vocab_major ? launch<false, true, FWD>(ctx, tx, tw, to, a)
+                               : launch<true, true, FWD>(ctx, tx, tw, to, a);
+    if (rc != BWPP_CUDA_ERR_UNSUPPORTED) return rc;
+  }
+  return vocab_major ? launch<false, false, FWD>(ctx, tx, tw, to, a)
+                     : launch<true, false, FWD>(ctx, tx, tw, to, a);
+}
+
+int operand_maps(BwppCudaCtx *ctx, const XentOperands &o, CUtensorMap *tx, CUtensorMap *tw) {
+  const auto BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const auto SW = CU_TENSOR_MAP_SWIZZLE_128B;
+  int rc = bwpp_make_tmap_2d(ctx, tx, o.x, BF, o.D, o.T, (uint64_t)o.ldx * 2, BK, BM, SW);
+  if (!rc)
+    rc = o.vocab_major ? bwpp_make_tmap_2d(ctx, tw, o.w, BF, o.D, o.V, (uint64_t)o.ldw * 2, BK, 64, SW)
+                       : bwpp_make_tmap_2d(ctx, tw, o.w, BF, o.V, o.D, (uint64_t)o.ldw * 2, 64, BK, SW);
+  return rc;
+}
+
+}  // namespace
+
+int bwpp_xent_stats_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_t *target,
+                           float2 *part, float *hit) {
+  CUtensorMap tx, tw;
+  const int rc = operand_maps(ctx, o, &tx, &tw);
+  if (rc) return rc;
+  XentTile a{};
+  a.T = o.T;
+  a.V = o.V;
+  a.D = o.D;
+  a.v0 = o.v0;
+  a.c = o.scale * 1.44269504f;
+  a.scale = o.scale;
+  a.target = target;
+  a.part = part;
+  a.hit = hit;
+  a.vocab = o.vocab;
+  return launch_any<true>(ctx, tx, tw, tx, a, o.vocab_major);
+}
+
+int bwpp_xent_combine_launch(BwppCudaCtx *ctx, const float2 *part, uint32_t nparts, const float *hit,
+                             const int32_t *target, float *loss, float *lse, uint32_t T, uint32_t V) {
+  xent_combine_kernel<<<(T + 31) / 32, 32 * COMBINE_WARPS, 0, ctx->stream>>>(
+      part, nparts, hit, target, loss, lse, T, V, ctx->status_word);
+  BWPP_LAUNCH_CHECK(ctx, "xent combine");
+  return BWPP_CUDA_OK;
+}
+
+int bwpp_xent_dlogit_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_t *target,
+                            const float *lse, const float *dloss, uint16_t *dlogit, uint32_t ld) {
+  CUtensorMap tx, tw, to;
+  int rc = operand_maps(ctx, o, &tx, &tw);
+  if (!rc)
+    rc = bwpp_make_tmap_2d(ctx, &to, dlogit, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, o.V, o.T,
+                           (uint64_t)ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc) return rc;
+  XentTile a{};
+  a.T = o.T;
+  a.V = o.V;
+  a.D = o.D;
+  a.v0 = o.v0;
+  a.c = o.scale * 1.44269504f;
+  a.scale = o.scale;
+  a.target = target;
+  a.lse = lse;
+  a.dloss = dloss;
+  a.vocab = o.vocab;
+  return launch_any<false>(ctx, tx, tw, to, a, o.vocab_major);
+}
