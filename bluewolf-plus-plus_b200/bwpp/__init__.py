@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_ROOT = os.path.dirname(_HERE)
@@ -136,19 +137,19 @@ _SIGS = {
     "bwpp_cuda_broadcast_f32": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, C.c_int]),
     "bwpp_cuda_cast_f32_bf16": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32]),
     "bwpp_cuda_xent_workspace_size": (_sz, [C.POINTER(XentParams), _i32]),
-    "bwpp_cuda_xent_fwd_bf16": (_i32, [_vp] * 6 + [C.POINTER(XentParams)]),
-    "bwpp_cuda_xent_bwd_bf16": (_i32, [_vp] * 8 + [C.POINTER(XentParams)]),
+    "bwpp_cuda_xent_fwd_bf16": (_i32, [_vp] * 7),
+    "bwpp_cuda_xent_bwd_bf16": (_i32, [_vp] * 9),
     "bwpp_cuda_rope_table": (_i32, [C.POINTER(RopeTable), C.POINTER(RopeConfig)]),
-    "bwpp_cuda_rope_bf16": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), C.POINTER(RopeParams)]),
-    "bwpp_cuda_rope_f16": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), C.POINTER(RopeParams)]),
-    "bwpp_cuda_rope_f32": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), C.POINTER(RopeParams)]),
-    "bwpp_cuda_junction_fwd_f32": (_i32, [_vp] * 8 + [C.POINTER(JunctionParams)]),
-    "bwpp_cuda_junction_fwd_bf16": (_i32, [_vp] * 8 + [C.POINTER(JunctionParams)]),
-    "bwpp_cuda_junction_fwd_f16": (_i32, [_vp] * 8 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_rope_bf16": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), _vp]),
+    "bwpp_cuda_rope_f16": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), _vp]),
+    "bwpp_cuda_rope_f32": (_i32, [_vp] * 6 + [C.POINTER(RopeTable), _vp]),
+    "bwpp_cuda_junction_fwd_f32": (_i32, [_vp] * 9),
+    "bwpp_cuda_junction_fwd_bf16": (_i32, [_vp] * 9),
+    "bwpp_cuda_junction_fwd_f16": (_i32, [_vp] * 9),
     "bwpp_cuda_junction_bwd_workspace_size": (_sz, [_vp, _u32, _u32, _u32]),
-    "bwpp_cuda_junction_bwd_f32": (_i32, [_vp] * 13 + [C.POINTER(JunctionParams)]),
-    "bwpp_cuda_junction_bwd_bf16": (_i32, [_vp] * 13 + [C.POINTER(JunctionParams)]),
-    "bwpp_cuda_junction_bwd_f16": (_i32, [_vp] * 13 + [C.POINTER(JunctionParams)]),
+    "bwpp_cuda_junction_bwd_f32": (_i32, [_vp] * 14),
+    "bwpp_cuda_junction_bwd_bf16": (_i32, [_vp] * 14),
+    "bwpp_cuda_junction_bwd_f16": (_i32, [_vp] * 14),
     "bwpp_cuda_comm_unique_id": (_i32, [_vp]),
     "bwpp_cuda_comm_create": (_i32, [C.POINTER(_vp), _vp, _i32, _i32, _i32]),
     "bwpp_cuda_comm_allreduce_sum_f32": (_i32, [_vp, _vp, _sz, _vp]),
@@ -247,11 +248,60 @@ def _ptr(t):
         return None
     if isinstance(t, int):
         return t
-    if hasattr(t, "data_ptr"):
+    try:
         return t.data_ptr()
+    except AttributeError:
+        pass
     if hasattr(t, "ctypes"):
         return t.ctypes.data
     raise TypeError(type(t))
+
+
+# The parameter structs as packed bytes: a fraction of a ctypes structure's
+# cost, and a value that does not fit its field is an error.
+_XENT = struct.Struct("@7I2if")       # XentParams
+_ROPE = struct.Struct("@9I5i")        # RopeParams
+_JUNCTION = struct.Struct("@7Ii4f")   # JunctionParams
+
+
+def _rope(name):
+    def rope(self, q, k, q_out, k_out, table, tokens, heads_q, heads_k, head_dim, ldq, ldk, ldq_out,
+             ldk_out, positions=None, seq=0, pos0=0, interleaved=0, inverse=0, head_major_in=0,
+             head_major_out=0):
+        rc = getattr(self.lib, name)(
+            self.handle, _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(positions), table,
+            _ROPE.pack(tokens, heads_q, heads_k, head_dim, ldq, ldk, ldq_out, ldk_out, seq, pos0,
+                       interleaved, inverse, head_major_in, head_major_out))
+        if rc:
+            self.check(rc, "rope")
+    return rope
+
+
+def _junction_fwd(name):
+    def junction_fwd(self, h, b, gain_post, gate, gain_pre, h_out, y, rows, cols, gate_rows=0,
+                     norm_after=1, scale_h=1.0, scale_b=1.0, eps_post=1e-5, eps_pre=1e-5, ldh=0, ldb=0,
+                     ldy=0, ldgate=0):
+        rc = getattr(self.lib, name)(
+            self.handle, _ptr(h), _ptr(b), _ptr(gain_post), _ptr(gate), _ptr(gain_pre), _ptr(h_out),
+            _ptr(y), _JUNCTION.pack(rows, cols, ldh or cols, ldb or cols, ldy or cols, ldgate or cols,
+                                    gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre))
+        if rc:
+            self.check(rc, "junction_fwd")
+    return junction_fwd
+
+
+def _junction_bwd(name):
+    def junction_bwd(self, h_out, b, gain_post, gate, gain_pre, dh_out, dy, dh, db, dgain_post, dgate,
+                     dgain_pre, rows, cols, gate_rows=0, norm_after=1, scale_h=1.0, scale_b=1.0,
+                     eps_post=1e-5, eps_pre=1e-5, ldh=0, ldb=0, ldy=0, ldgate=0):
+        rc = getattr(self.lib, name)(
+            self.handle, _ptr(h_out), _ptr(b), _ptr(gain_post), _ptr(gate), _ptr(gain_pre), _ptr(dh_out),
+            _ptr(dy), _ptr(dh), _ptr(db), _ptr(dgain_post), _ptr(dgate), _ptr(dgain_pre),
+            _JUNCTION.pack(rows, cols, ldh or cols, ldb or cols, ldy or cols, ldgate or cols, gate_rows,
+                           norm_after, scale_h, scale_b, eps_post, eps_pre))
+        if rc:
+            self.check(rc, "junction_bwd")
+    return junction_bwd
 
 
 class Ctx:
@@ -392,72 +442,29 @@ class Ctx:
 
     # training-step operators around a decoder block
     def xent_fwd(self, x, w, target, loss, lse, T, V, D, ldx, ldw, w_vocab_major=0, scale=1.0):
-        p = XentParams(T, V, D, ldx, ldw, 0, 0, int(w_vocab_major), 0, float(scale))
-        self.check(self.lib.bwpp_cuda_xent_fwd_bf16(self.handle, _ptr(x), _ptr(w), _ptr(target), _ptr(loss),
-                                                    _ptr(lse), C.byref(p)), "xent_fwd")
+        rc = self.lib.bwpp_cuda_xent_fwd_bf16(
+            self.handle, _ptr(x), _ptr(w), _ptr(target), _ptr(loss), _ptr(lse),
+            _XENT.pack(T, V, D, ldx, ldw, 0, 0, w_vocab_major, 0, scale))
+        if rc:
+            self.check(rc, "xent_fwd")
 
     def xent_bwd(self, x, w, target, lse, dloss, dx, dw, T, V, D, ldx, ldw, lddx, lddw, w_vocab_major=0,
                  scale=1.0, grads_bf16=0):
-        p = XentParams(T, V, D, ldx, ldw, lddx, lddw, int(w_vocab_major), int(grads_bf16), float(scale))
-        self.check(self.lib.bwpp_cuda_xent_bwd_bf16(self.handle, _ptr(x), _ptr(w), _ptr(target), _ptr(lse),
-                                                    _ptr(dloss), _ptr(dx), _ptr(dw), C.byref(p)), "xent_bwd")
+        rc = self.lib.bwpp_cuda_xent_bwd_bf16(
+            self.handle, _ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw),
+            _XENT.pack(T, V, D, ldx, ldw, lddx, lddw, w_vocab_major, grads_bf16, scale))
+        if rc:
+            self.check(rc, "xent_bwd")
 
-    def _rope(self, fn, q, k, q_out, k_out, table, tokens, heads_q, heads_k, head_dim, ldq, ldk, ldq_out,
-              ldk_out, positions=None, seq=0, pos0=0, interleaved=0, inverse=0, head_major_in=0,
-              head_major_out=0):
-        p = RopeParams(tokens, heads_q, heads_k, head_dim, ldq, ldk, ldq_out, ldk_out, seq, pos0,
-                       int(interleaved), int(inverse), int(head_major_in), int(head_major_out))
-        self.check(fn(self.handle, _ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), _ptr(positions),
-                      C.byref(table), C.byref(p)), "rope")
-
-    def rope_bf16(self, *args, **kw):
-        self._rope(self.lib.bwpp_cuda_rope_bf16, *args, **kw)
-
-    def rope_f16(self, *args, **kw):
-        self._rope(self.lib.bwpp_cuda_rope_f16, *args, **kw)
-
-    def rope_f32(self, *args, **kw):
-        self._rope(self.lib.bwpp_cuda_rope_f32, *args, **kw)
-
-    def _junction_params(self, rows, cols, gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre,
-                         ldh, ldb, ldy, ldgate):
-        return JunctionParams(rows, cols, ldh or cols, ldb or cols, ldy or cols, ldgate or cols, gate_rows,
-                              int(norm_after), scale_h, scale_b, eps_post, eps_pre)
-
-    def _junction_fwd(self, fn, h, b, gain_post, gate, gain_pre, h_out, y, rows, cols, gate_rows=0,
-                      norm_after=1, scale_h=1.0, scale_b=1.0, eps_post=1e-5, eps_pre=1e-5, ldh=0, ldb=0,
-                      ldy=0, ldgate=0):
-        p = self._junction_params(rows, cols, gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre,
-                                  ldh, ldb, ldy, ldgate)
-        self.check(fn(self.handle, _ptr(h), _ptr(b), _ptr(gain_post), _ptr(gate), _ptr(gain_pre),
-                      _ptr(h_out), _ptr(y), C.byref(p)), "junction_fwd")
-
-    def _junction_bwd(self, fn, h_out, b, gain_post, gate, gain_pre, dh_out, dy, dh, db, dgain_post, dgate,
-                      dgain_pre, rows, cols, gate_rows=0, norm_after=1, scale_h=1.0, scale_b=1.0,
-                      eps_post=1e-5, eps_pre=1e-5, ldh=0, ldb=0, ldy=0, ldgate=0):
-        p = self._junction_params(rows, cols, gate_rows, norm_after, scale_h, scale_b, eps_post, eps_pre,
-                                  ldh, ldb, ldy, ldgate)
-        self.check(fn(self.handle, _ptr(h_out), _ptr(b), _ptr(gain_post), _ptr(gate), _ptr(gain_pre),
-                      _ptr(dh_out), _ptr(dy), _ptr(dh), _ptr(db), _ptr(dgain_post), _ptr(dgate),
-                      _ptr(dgain_pre), C.byref(p)), "junction_bwd")
-
-    def junction_fwd_f32(self, *args, **kw):
-        self._junction_fwd(self.lib.bwpp_cuda_junction_fwd_f32, *args, **kw)
-
-    def junction_fwd_bf16(self, *args, **kw):
-        self._junction_fwd(self.lib.bwpp_cuda_junction_fwd_bf16, *args, **kw)
-
-    def junction_fwd_f16(self, *args, **kw):
-        self._junction_fwd(self.lib.bwpp_cuda_junction_fwd_f16, *args, **kw)
-
-    def junction_bwd_f32(self, *args, **kw):
-        self._junction_bwd(self.lib.bwpp_cuda_junction_bwd_f32, *args, **kw)
-
-    def junction_bwd_bf16(self, *args, **kw):
-        self._junction_bwd(self.lib.bwpp_cuda_junction_bwd_bf16, *args, **kw)
-
-    def junction_bwd_f16(self, *args, **kw):
-        self._junction_bwd(self.lib.bwpp_cuda_junction_bwd_f16, *args, **kw)
+    rope_bf16 = _rope("bwpp_cuda_rope_bf16")
+    rope_f16 = _rope("bwpp_cuda_rope_f16")
+    rope_f32 = _rope("bwpp_cuda_rope_f32")
+    junction_fwd_f32 = _junction_fwd("bwpp_cuda_junction_fwd_f32")
+    junction_fwd_bf16 = _junction_fwd("bwpp_cuda_junction_fwd_bf16")
+    junction_fwd_f16 = _junction_fwd("bwpp_cuda_junction_fwd_f16")
+    junction_bwd_f32 = _junction_bwd("bwpp_cuda_junction_bwd_f32")
+    junction_bwd_bf16 = _junction_bwd("bwpp_cuda_junction_bwd_bf16")
+    junction_bwd_f16 = _junction_bwd("bwpp_cuda_junction_bwd_f16")
 
 
 def xent_workspace_size(T, V, D, ldx, ldw, w_vocab_major=0, backward=0, grads_bf16=0) -> int:

@@ -40,6 +40,18 @@ struct Raw {
     }
   }
 
+  // From shared memory (VEC elements are 8 or 16 bytes).
+  __device__ __forceinline__ void load_shared(const uint8_t *p) {
+    static_assert(BYTES == 8 || BYTES == 16, "8 or 16 bytes");
+    if constexpr (BYTES == 16) {
+      const uint4 t = *reinterpret_cast<const uint4 *>(p);
+      w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
+    } else {
+      const uint2 t = *reinterpret_cast<const uint2 *>(p);
+      w[0] = t.x; w[1] = t.y;
+    }
+  }
+
   __device__ __forceinline__ void store(typename Elem<DT>::type *p) const {
     if constexpr (BYTES >= 16) {
 #pragma unroll

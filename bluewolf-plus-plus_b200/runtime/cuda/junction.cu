@@ -81,7 +81,7 @@ __device__ __forceinline__ void load_gain(const float *g, uint32_t c, float (&o)
   }
 }
 
-constexpr int block_threads(int tpr) { return tpr < 128 ? 128 : tpr; }
+constexpr int block_threads(int tpr) { return tpr == 32 ? 128 : tpr; }
 
 // ---- forward -----------------------------------------------------------------
 
@@ -231,25 +231,39 @@ __global__ void __launch_bounds__(block_threads(TPR))
 #pragma unroll
     for (int e = 0; e < VEC; ++e) acc_post[i][e] = acc_pre[i][e] = 0.0f;
 
+  // a row's loads are issued before the row in front of it is worked on
+  Raw<F32, VEC> hn[NV], dn[NV];
+  Raw<DT, VEC> bn[NV], yn[NV];
+  auto fetch = [&](uint32_t r) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * VEC;
+      hn[i].zero();
+      dn[i].zero();
+      bn[i].zero();
+      yn[i].zero();
+      if (c < p.cols && r < last) {
+        if (a.dy) {
+          hn[i].load(a.h + (size_t)r * p.ldh + c);
+          yn[i].load(static_cast<const T *>(a.dy) + (size_t)r * p.ldy + c);
+        }
+        if (a.dh_out) dn[i].load(a.dh_out + (size_t)r * p.ldh + c);
+        if (a.b) bn[i].load(static_cast<const T *>(a.b) + (size_t)r * p.ldb + c);
+      }
+    }
+  };
+  fetch(first + sub);
   for (uint32_t r = first + sub; r < last; r += RPB) {
     Raw<F32, VEC> hv[NV], dv[NV];
     Raw<DT, VEC> bv[NV], yv[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (t + i * TPR) * VEC;
-      hv[i].zero();
-      dv[i].zero();
-      bv[i].zero();
-      yv[i].zero();
-      if (c < p.cols) {
-        if (a.dy) {
-          hv[i].load(a.h + (size_t)r * p.ldh + c);
-          yv[i].load(static_cast<const T *>(a.dy) + (size_t)r * p.ldy + c);
-        }
-        if (a.dh_out) dv[i].load(a.dh_out + (size_t)r * p.ldh + c);
-        if (a.b) bv[i].load(static_cast<const T *>(a.b) + (size_t)r * p.ldb + c);
-      }
+      hv[i] = hn[i];
+      dv[i] = dn[i];
+      bv[i] = bn[i];
+      yv[i] = yn[i];
     }
+    fetch(r + RPB);
     float s[3] = {0.0f, 0.0f, 0.0f};  // sum h'^2, sum gain_pre dy h', sum b^2
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -355,6 +369,202 @@ __global__ void __launch_bounds__(block_threads(TPR))
   write(acc_pre, a.part_pre);
 }
 
+// The same for rows of 16-byte pieces, staged through shared memory: bulk
+// copies bring the rows of the next `stages` steps while this one is worked
+// on, so the loads in flight do not depend on the registers of the threads
+// that wait in the row's two reductions.  (32768 x 2048 bf16, 12 bytes read
+// and 6 written per element: 327 us with loads in the loop, 263 with the next
+// row's loads in registers, 205 staged, 5.9 TB/s)
+//
+// All threads of the block hold one row, thread t the four-element vectors t,
+// t + TPR, ....  TOKEN: a gate row per row (staged too), and its gradient.
+constexpr int kMaxStages = 3;
+
+template <int DT, int NV, int TPR, bool TOKEN>
+__global__ void __launch_bounds__(TPR)
+    junction_bwd_staged_kernel(const __grid_constant__ JunctionArgs a, uint32_t stages, int *status) {
+  using T = typename Elem<DT>::type;
+  constexpr int W = TPR / 32;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ float red[3][W], red1[W];
+  __shared__ volatile int expired;  // a wait ran out: the whole block leaves
+  const BwppCudaJunctionParams &p = a.p;
+  const uint32_t t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  uint32_t first, last;
+  chunk_range(a, blockIdx.x, first, last);
+  const float inv_c = 1.0f / (float)p.cols;
+  // a stage: h', dh', [gate], b, dy
+  const uint32_t wide = p.cols * 4, narrow = p.cols * (uint32_t)sizeof(T);
+  const uint32_t at_gate = 2 * wide, at_b = at_gate + (TOKEN ? wide : 0), at_y = at_b + narrow;
+  const uint32_t stage_bytes = at_y + narrow;
+  if (t == 0) {
+    for (uint32_t s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+    expired = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  auto fetch = [&](uint32_t r, uint32_t s) {  // one thread
+    uint8_t *to = ring + s * stage_bytes;
+    mbar_arrive_expect_tx(&full[s], (a.dy ? wide + narrow : 0) + (a.dh_out ? wide : 0) +
+                                        (TOKEN ? wide : 0) + (a.b ? narrow : 0));
+    if (a.dy) {
+      bulk_load(to, a.h + (size_t)r * p.ldh, wide, &full[s]);
+      bulk_load(to + at_y, static_cast<const T *>(a.dy) + (size_t)r * p.ldy, narrow, &full[s]);
+    }
+    if (a.dh_out) bulk_load(to + wide, a.dh_out + (size_t)r * p.ldh, wide, &full[s]);
+    if (TOKEN) bulk_load(to + at_gate, a.gate + (size_t)r * p.ldgate, wide, &full[s]);
+    if (a.b) bulk_load(to + at_b, static_cast<const T *>(a.b) + (size_t)r * p.ldb, narrow, &full[s]);
+  };
+  if (t == 0)
+    for (uint32_t s = 0; s < stages && first + s < last; ++s) fetch(first + s, s);
+
+  // gain_pre, and gain_post times the chunk's gate row
+  float gq[NV][4], gp[NV][4], acc_post[NV][4], acc_pre[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = (t + i * TPR) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc_post[i][e] = acc_pre[i][e] = gq[i][e] = gp[i][e] = 0.0f;
+    if (c >= p.cols || first >= last) continue;
+    load_gain<4>(a.gain_pre, c, gq[i]);
+    load_gain<4>(p.norm_after ? a.gain_post : nullptr, c, gp[i]);
+    if (!TOKEN && a.gate) {
+      float gt[4];
+      load_gain<4>(a.gate + (size_t)(first / p.gate_rows) * p.ldgate, c, gt);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) gp[i][e] *= gt[e];
+    }
+  }
+
+  uint32_t stage = 0, phase = 0;
+  for (uint32_t r = first; r < last; ++r) {
+    if (!mbar_wait(&full[stage], phase, status)) expired = 1;
+    const uint8_t *row = ring + stage * stage_bytes;
+    float hv[NV][4], dv[NV][4], gt[NV][4];
+    Raw<DT, 4> bv[NV], yv[NV];
+    float s[3] = {0.0f, 0.0f, 0.0f};  // sum h'^2, sum gain_pre dy h', sum b^2
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * 4;
+      bv[i].zero();
+      yv[i].zero();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hv[i][e] = dv[i][e] = gt[i][e] = 0.0f;
+      if (c >= p.cols) continue;
+      auto quad = [&](uint32_t at, float (&o)[4]) {
+        const float4 v = *reinterpret_cast<const float4 *>(row + at + c * 4);
+        o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+      };
+      if (a.dy) {
+        quad(0, hv[i]);
+        yv[i].load_shared(row + at_y + c * sizeof(T));
+      }
+      if (a.dh_out) quad(wide, dv[i]);
+      if (TOKEN) quad(at_gate, gt[i]);
+      if (a.b) bv[i].load_shared(row + at_b + c * sizeof(T));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float bb = bv[i].get(e);
+        s[0] += hv[i][e] * hv[i][e];
+        s[1] += gq[i][e] * yv[i].get(e) * hv[i][e];
+        s[2] += bb * bb;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+      if (lane == 0) red[j][warp] = s[j];
+    }
+    __syncthreads();  // every thread holds its part of the row: the stage is free
+    if (expired) {
+      if (t == 0)  // the copies still in flight, each with a limit again
+        for (uint32_t k = 1; k < stages && r + k < last; ++k)
+          mbar_wait(&full[(stage + k) % stages], phase ^ (stage + k >= stages ? 1u : 0u), status);
+      break;
+    }
+    if (t == 0 && r + stages < last) fetch(r + stages, stage);
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      s[j] = red[j][0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) s[j] += red[j][w];
+    }
+    const float rh = a.dy ? 1.0f / sqrtf(s[0] * inv_c + p.eps_pre) : 0.0f;
+    const float m2 = rh * s[1] * inv_c;  // mean(g hat)
+    const float rb = p.norm_after ? 1.0f / sqrtf(s[2] * inv_c + p.eps_post) : 1.0f;
+    float m = 0.0f;  // sum gain_post du bhat
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * 4;
+      if (c >= p.cols) continue;
+      float w[4], dg[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float hat = hv[i][e] * rh, dy = yv[i].get(e);
+        const float dH = dv[i][e] + rh * (gq[i][e] * dy - hat * m2);
+        const float bh = bv[i].get(e) * rb, ee = p.scale_b * dH;
+        const float gu = (TOKEN ? gp[i][e] * gt[i][e] : gp[i][e]) * ee;  // gain_post du
+        acc_pre[i][e] += dy * hat;
+        acc_post[i][e] += (TOKEN ? ee * gt[i][e] : ee) * bh;
+        m += gu * bh;
+        dg[e] = ee * bh * gp[i][e];
+        w[e] = p.scale_h * dH;
+        dv[i][e] = gu;
+      }
+      if (TOKEN && a.dgate) {
+        Raw<F32, 4> o;
+        o.set(dg);
+        o.store(a.dgate + (size_t)r * p.ldgate + c);
+      }
+      if (a.dh) {
+        Raw<F32, 4> o;
+        o.set(w);
+        o.store(a.dh + (size_t)r * p.ldh + c);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    if (lane == 0) red1[warp] = m;
+    __syncthreads();
+    if (!a.db) continue;
+    float m1 = 0.0f;
+    if (p.norm_after) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) m1 += red1[w];
+      m1 *= inv_c;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t c = (t + i * TPR) * 4;
+      if (c >= p.cols) continue;
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = rb * (dv[i][e] - bv[i].get(e) * rb * m1);
+      Raw<DT, 4> o;
+      o.set(w);
+      o.store(static_cast<T *>(a.db) + (size_t)r * p.ldb + c);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = (t + i * TPR) * 4;
+    if (c >= p.cols) continue;
+    const size_t at = (size_t)blockIdx.x * p.cols + c;
+    if (a.part_post)
+      *reinterpret_cast<float4 *>(a.part_post + at) =
+          make_float4(acc_post[i][0], acc_post[i][1], acc_post[i][2], acc_post[i][3]);
+    if (a.part_pre)
+      *reinterpret_cast<float4 *>(a.part_pre + at) =
+          make_float4(acc_pre[i][0], acc_pre[i][1], acc_pre[i][2], acc_pre[i][3]);
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kLoopThreads)
     junction_bwd_looped_kernel(const __grid_constant__ JunctionArgs a) {
@@ -448,7 +658,10 @@ struct JunctionSums {
   const float *gain_post, *gate;
   float *dgain_post, *dgain_pre, *dgate;
   uint32_t chunks, chunks_per_group, cols, ldgate;
-  int weighted;  // dgain_post: weight the partial rows with their gate rows
+  // dgain_post weights the partial rows with their gate rows: k / d is the high
+  // word of k * ceil(2^64 / d), exactly for k and d below 2^31 (0: not weighted;
+  // a divide for each term cost more than the sums, 4.3 us of 8.8)
+  uint64_t group_inv;
 };
 
 constexpr int kSumWarps = 32;
@@ -464,12 +677,24 @@ __global__ void __launch_bounds__(32 * kSumWarps) junction_sums_kernel(const Jun
   const uint32_t end = job < 2 ? a.chunks : begin + a.chunks_per_group;
   float acc = 0.0f;
   if (c < a.cols) {
-    if (job == 0 && a.weighted) {
-      for (uint32_t k = begin + warp; k < end; k += kSumWarps)
-        acc += part[(size_t)k * a.cols + c] * a.gate[(size_t)(k / a.chunks_per_group) * a.ldgate + c];
-    } else {
-#pragma unroll 4
-      for (uint32_t k = begin + warp; k < end; k += kSumWarps) acc += part[(size_t)k * a.cols + c];
+    constexpr int U = 8;  // rows in flight
+    for (uint32_t k0 = begin + warp; k0 < end; k0 += U * kSumWarps) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t k = k0 + u * kSumWarps;
+        v[u] = k < end ? __ldg(part + (size_t)k * a.cols + c) : 0.0f;
+      }
+      if (job == 0 && a.group_inv) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t k = k0 + u * kSumWarps;
+          const uint64_t g = a.chunks_per_group == 1 ? k : __umul64hi(k, a.group_inv);
+          if (k < end) v[u] *= __ldg(a.gate + g * a.ldgate + c);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc += v[u];
     }
   }
   sums[warp][lane] = acc;
@@ -493,9 +718,10 @@ struct Chunks {
 };
 
 // A chunk holds consecutive rows of one group (rows that share a gate row and
-// whose dgate is summed), about `per_sm` chunks per SM.
-bool make_chunks(BwppCudaCtx *ctx, uint32_t rows, uint32_t gate_rows, Chunks &k) {
-  constexpr uint32_t per_sm = 4;
+// whose dgate is summed), about `per_sm` chunks per SM (at most kMaxPerSm,
+// which the scratch is sized for).
+constexpr uint32_t kMaxPerSm = 8, kPerSm = 4;
+bool make_chunks(BwppCudaCtx *ctx, uint32_t rows, uint32_t gate_rows, uint32_t per_sm, Chunks &k) {
   k.group_rows = gate_rows <= 1 || gate_rows > rows ? rows : gate_rows;
   k.groups = (uint32_t)(((uint64_t)rows + k.group_rows - 1) / k.group_rows);
   const uint32_t want = (uint32_t)ctx->num_sms * per_sm;
@@ -534,6 +760,11 @@ template <int DT>
 void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
   const uint32_t cols = a.p.cols;
   cudaStream_t s = ctx->stream;
+  // Few threads with more of the row each keep more bytes in flight per SM and
+  // have less to wait for at the row's two reductions (32768 x 2048 bf16: 147 us
+  // with 256 threads, 130 with 128, 127 with 64, 140 with a warp); many threads
+  // finish a single row sooner (3.1 us with 256, 4.5 with 64).
+  const bool many = a.p.rows > (uint32_t)ctx->num_sms * 4;
 #define BWPP_FWD(VEC, NV, TPR)                                                             \
   junction_fwd_kernel<DT, VEC, NV, TPR>                                                    \
       <<<(a.p.rows + block_threads(TPR) / TPR - 1) / (block_threads(TPR) / TPR),           \
@@ -541,11 +772,15 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
   if (vectors<DT>(a)) {
     if (cols <= 256) BWPP_FWD(8, 1, 32);
     else if (cols <= 512) BWPP_FWD(8, 2, 32);
+    else if (cols <= 1024 && many) BWPP_FWD(8, 2, 64);
     else if (cols <= 1024) BWPP_FWD(8, 1, 128);
+    else if (cols <= 2048 && many) BWPP_FWD(8, 4, 64);
     else if (cols <= 2048) BWPP_FWD(8, 1, 256);
+    else if (cols <= 4096 && many) BWPP_FWD(8, 4, 128);
     else if (cols <= 4096) BWPP_FWD(8, 2, 256);
+    else if (cols <= 8192 && many) BWPP_FWD(8, 4, 256);
     else if (cols <= 8192) BWPP_FWD(8, 2, 512);
-    else if (cols <= 16384) BWPP_FWD(8, 2, 1024);
+    else if (cols <= 16384) BWPP_FWD(8, 4, 512);
     else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
   } else {
     if (cols <= 128) BWPP_FWD(1, 4, 32);
@@ -557,27 +792,82 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
 #undef BWPP_FWD
 }
 
+// How the staged backward takes a row width: stages and resident CTAs per SM
+// (stages 0: it does not take it).
+struct Staged {
+  uint32_t stages, per_sm, bytes;
+};
 template <int DT>
-void launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks) {
+Staged staged(const JunctionArgs &a) {
+  Staged g{0, kPerSm, 0};
+  const uint32_t cols = a.p.cols;
+  if (!vectors<DT>(a) || cols <= 256 || cols > 8192) return g;
+  const bool token = a.p.gate_rows == 1 && a.gate;
+  const uint32_t row = cols * (8 + (token ? 4 : 0) + 2 * (uint32_t)sizeof(typename Elem<DT>::type));
+  constexpr uint32_t sm = 220 * 1024;  // of an SM's 228 KB; 1 KB and the static part go with each CTA
+  // 16 warps per SM hide a row's two reductions (32768 x 2048 bf16: 323 us with
+  // one CTA of 8 warps, 205 with two, 218 with three, 227 with four); two or
+  // more stages make no difference then
+  const uint32_t want = cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1;
+  for (uint32_t per = want; per >= 1 && g.stages < 2; --per) {
+    g.per_sm = per;
+    g.stages = sm / per / row;
+  }
+  if (g.stages > (uint32_t)kMaxStages) g.stages = kMaxStages;
+  if (g.stages < 2) g = Staged{0, kPerSm, 0};
+  g.bytes = g.stages * row;
+  return g;
+}
+
+bool g_staged_set[64][32] = {};
+
+template <int DT, int NV, int TPR, bool TOKEN>
+int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Staged &g, int id) {
+  auto kern = junction_bwd_staged_kernel<DT, NV, TPR, TOKEN>;
+  const int dev = ctx->device;
+  if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction: device index >= 64");
+  bool &set = g_staged_set[dev][id * 6 + DT * 2 + (TOKEN ? 1 : 0)];
+  if (!set) {
+    const int rc = bwpp_check_cuda(
+        ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024),
+        "junction smem attribute");
+    if (rc) return rc;
+    set = true;
+  }
+  kern<<<chunks, TPR, g.bytes, ctx->stream>>>(a, g.stages, ctx->status_word);
+  return BWPP_CUDA_OK;
+}
+
+template <int DT, bool TOKEN>
+int launch_staged_any(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Staged &g) {
+  const uint32_t cols = a.p.cols;
+  if (cols <= 512) return launch_staged<DT, 2, 64, TOKEN>(ctx, a, chunks, g, 0);
+  if (cols <= 1024) return launch_staged<DT, 2, 128, TOKEN>(ctx, a, chunks, g, 1);
+  if (cols <= 2048) return launch_staged<DT, 2, 256, TOKEN>(ctx, a, chunks, g, 2);
+  if (cols <= 4096) return launch_staged<DT, 2, 512, TOKEN>(ctx, a, chunks, g, 3);
+  return launch_staged<DT, 4, 512, TOKEN>(ctx, a, chunks, g, 4);
+}
+
+template <int DT>
+int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Staged &g) {
   const uint32_t cols = a.p.cols;
   cudaStream_t s = ctx->stream;
+  if (g.stages)
+    return a.p.gate_rows == 1 && a.gate ? launch_staged_any<DT, true>(ctx, a, chunks, g)
+                                        : launch_staged_any<DT, false>(ctx, a, chunks, g);
 #define BWPP_BWD(VEC, NV, TPR) \
   junction_bwd_kernel<DT, VEC, NV, TPR><<<chunks, block_threads(TPR), 0, s>>>(a)
-  if (vectors<DT>(a)) {
-    if (cols <= 256) BWPP_BWD(8, 1, 32);
-    else if (cols <= 1024) BWPP_BWD(8, 1, 128);
-    else if (cols <= 2048) BWPP_BWD(8, 1, 256);
-    else if (cols <= 4096) BWPP_BWD(8, 1, 512);
-    else if (cols <= 8192) BWPP_BWD(8, 1, 1024);
-    else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
+  if (vectors<DT>(a) && cols <= 256) {
+    BWPP_BWD(8, 1, 32);
   } else {
     if (cols <= 128) BWPP_BWD(1, 4, 32);
-    else if (cols <= 1024) BWPP_BWD(1, 8, 128);
+    else if (cols <= 1024) BWPP_BWD(1, 4, 256);
     else if (cols <= 4096) BWPP_BWD(1, 8, 512);
     else if (cols <= 8192) BWPP_BWD(1, 8, 1024);
     else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
   }
 #undef BWPP_BWD
+  return BWPP_CUDA_OK;
 }
 
 template <int DT>
@@ -648,8 +938,9 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
   a.db = db;
   const bool per_row = a.p.gate_rows == 1;
   a.dgate = per_row ? dgate : nullptr;
+  const Staged g = staged<DT>(a);
   Chunks k;
-  if (!make_chunks(ctx, a.p.rows, a.p.gate_rows, k))
+  if (!make_chunks(ctx, a.p.rows, a.p.gate_rows, g.per_sm, k))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: too many gate rows");
   a.chunk_rows = k.chunk_rows;
   a.chunks_per_group = k.per_group;
@@ -664,7 +955,8 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
     if (sum_post) a.part_post = reinterpret_cast<float *>(scratch);
     if (dgain_pre) a.part_pre = reinterpret_cast<float *>(scratch) + part;
   }
-  launch_bwd<DT>(ctx, a, k.chunks);
+  rc = launch_bwd<DT>(ctx, a, k.chunks, g);
+  if (rc) return rc;
   BWPP_LAUNCH_CHECK(ctx, "junction bwd");
   if (sums) {
     JunctionSums q{};
@@ -679,7 +971,8 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
     q.chunks_per_group = k.per_group;
     q.cols = a.p.cols;
     q.ldgate = a.p.ldgate;
-    q.weighted = gate && !per_row;
+    q.group_inv = gate && !per_row ? ~0ull / k.per_group + 1 : 0;
+    if (gate && !per_row && k.per_group == 1) q.group_inv = 1;
     const dim3 grid(2 + (q.dgate ? k.groups : 0), (a.p.cols + 31) / 32);
     if (grid.y > 65535)
       return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: row too wide");
@@ -697,7 +990,7 @@ size_t bwpp_cuda_junction_bwd_workspace_size(BwppCudaCtx *ctx, uint32_t rows, ui
                                              uint32_t gate_rows) {
   if (!ctx || rows == 0 || cols == 0) return 0;
   Chunks k;
-  if (!make_chunks(ctx, rows, gate_rows ? gate_rows : rows, k)) return 0;
+  if (!make_chunks(ctx, rows, gate_rows ? gate_rows : rows, kMaxPerSm, k)) return 0;
   return 2 * (size_t)k.chunks * cols * sizeof(float) + BWPP_OP_SCRATCH_PAD;
 }
 

@@ -37,81 +37,106 @@ struct RopeArgs {
   uint32_t turn_slots, slots, lanes;
 };
 
+// Heads that a thread loads before it turns any: 128 bytes in flight.  (For
+// 32768 tokens x 32 heads x 128 bf16: 109 us with one head, 90 with two, 82.5
+// with four, 84 with eight.)
+constexpr int batch_of(bool one_vector) { return one_vector ? 8 : 4; }
+
 // A thread owns one slot (VEC pairs, or VEC columns behind R) of one token in
-// heads lane, lane + lanes, ...
+// heads lane, lane + lanes, ... of q and then of k: its sines and cosines are
+// computed once for all of them, behind the first loads.
 template <int DT, int VEC, bool IL>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
   using T = typename Elem<DT>::type;
+  constexpr bool ONE = IL && VEC > 1;  // a vector holds both sides of its pairs
+  constexpr int PAIRS = ONE ? VEC / 2 : VEC;
+  constexpr int kBatch = batch_of(ONE);
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   if (id >= a.units) return;
   const uint32_t per = a.slots * a.lanes;
-  const uint32_t t = a.token0 + id / per, rem = id % per;
-  const uint32_t lane = rem / a.slots, slot = rem % a.slots;
+  const uint32_t n = id / per, rem = id - n * per, t = a.token0 + n;
+  const uint32_t lane = rem / a.slots, slot = rem - lane * a.slots;
   const uint32_t b = t / a.seq, s = t - b * a.seq;
-  const uint32_t heads = a.p.heads_q + a.p.heads_k;
   const bool turns = slot < a.turn_slots;
-  const bool two = turns && !(IL && VEC > 1);  // the slot's pairs lie in two vectors
+  const bool two = !ONE && turns;
   const uint32_t half = a.table.pairs;
-  uint32_t c0, c1;
+  uint32_t c0, c1 = 0;  // columns of the slot's two vectors
   if (!turns) {
-    c0 = c1 = 2 * half + (slot - a.turn_slots) * VEC;
+    c0 = 2 * half + (slot - a.turn_slots) * VEC;
   } else if (IL) {
-    c0 = VEC > 1 ? slot * VEC : 2 * slot;
+    c0 = ONE ? slot * VEC : 2 * slot;
     c1 = c0 + 1;
   } else {
     c0 = slot * VEC;
     c1 = c0 + half;
   }
-  constexpr int PAIRS = IL && VEC > 1 ? VEC / 2 : VEC;
   float cs[PAIRS], sn[PAIRS];
-  if (turns) {
+  bool ready = !turns;
+  auto angles = [&]() {
     const int64_t pos =
-        a.positions ? (int64_t)a.positions[t] : (int64_t)a.p.pos0 + (int64_t)s;
+        a.positions ? (int64_t)__ldg(a.positions + t) : (int64_t)a.p.pos0 + (int64_t)s;
+    const float up = a.table.amplitude, side = a.p.inverse ? -up : up;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
       const uint64_t turn = (uint64_t)pos * a.table.turns[slot * PAIRS + i];
       sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &sn[i], &cs[i]);
-      cs[i] *= a.table.amplitude;
-      sn[i] *= a.p.inverse ? -a.table.amplitude : a.table.amplitude;
+      cs[i] *= up;
+      sn[i] *= side;
     }
-  }
-  for (uint32_t h = lane; h < heads; h += a.lanes) {
-    const bool isq = h < a.p.heads_q;
-    const uint32_t hh = isq ? h : h - a.p.heads_q, nh = isq ? a.p.heads_q : a.p.heads_k;
-    const size_t ldi = isq ? a.p.ldq : a.p.ldk, ldo = isq ? a.p.ldq_out : a.p.ldk_out;
-    const size_t at = a.p.head_major_in ? (((size_t)b * nh + hh) * a.seq + s) * ldi
-                                        : t * ldi + (size_t)hh * a.p.head_dim;
-    const size_t to = a.p.head_major_out ? (((size_t)b * nh + hh) * a.seq + s) * ldo
-                                         : t * ldo + (size_t)hh * a.p.head_dim;
-    const T *src = static_cast<const T *>(isq ? a.q : a.k) + at;
-    T *dst = static_cast<T *>(isq ? a.qo : a.ko) + to;
-    Raw<DT, VEC> x, y;
-    x.load(src + c0);
-    if (two) y.load(src + c1);
-    if (turns) {
-      float v[VEC], w[VEC];
-      if constexpr (IL && VEC > 1) {
+    ready = true;
+  };
+  auto pass = [&](const void *from, void *into, uint32_t heads, size_t ldi, size_t ldo) {
+    const size_t di = a.p.head_major_in ? (size_t)a.seq * ldi : a.p.head_dim;
+    const size_t dn = a.p.head_major_out ? (size_t)a.seq * ldo : a.p.head_dim;
+    const T *src = static_cast<const T *>(from) + c0 +
+                   (a.p.head_major_in ? (size_t)b * heads * di + s * ldi : t * ldi);
+    T *dst = static_cast<T *>(into) + c0 +
+             (a.p.head_major_out ? (size_t)b * heads * dn + s * ldo : t * ldo);
+    const uint32_t side = c1 - c0;
+    for (uint32_t h0 = lane; h0 < heads; h0 += kBatch * a.lanes) {
+      Raw<DT, VEC> x[kBatch], y[ONE ? 1 : kBatch];
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-          const float x0 = x.get(2 * i), x1 = x.get(2 * i + 1);
-          v[2 * i] = x0 * cs[i] - x1 * sn[i];
-          v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t h = h0 + u * a.lanes;
+        if (h < heads) {
+          x[u].load(src + h * di);
+          if constexpr (!ONE)
+            if (two) y[u].load(src + h * di + side);
         }
-        x.set(v);
-      } else {
+      }
+      if (!ready) angles();
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float x0 = x.get(i), x1 = y.get(i);
-          v[i] = x0 * cs[i] - x1 * sn[i];
-          w[i] = x1 * cs[i] + x0 * sn[i];
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t h = h0 + u * a.lanes;
+        if (h >= heads) break;
+        if (turns) {
+          float v[VEC];
+          if constexpr (ONE) {
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+              const float x0 = x[u].get(2 * i), x1 = x[u].get(2 * i + 1);
+              v[2 * i] = x0 * cs[i] - x1 * sn[i];
+              v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+            }
+          } else {
+            float w[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float x0 = x[u].get(i), x1 = y[u].get(i);
+              v[i] = x0 * cs[i] - x1 * sn[i];
+              w[i] = x1 * cs[i] + x0 * sn[i];
+            }
+            y[u].set(w);
+            y[u].store(dst + h * dn + side);
+          }
+          x[u].set(v);
         }
-        x.set(v);
-        y.set(w);
+        x[u].store(dst + h * dn);
       }
     }
-    x.store(dst + c0);
-    if (two) y.store(dst + c1);
-  }
+  };
+  pass(a.q, a.qo, a.p.heads_q, a.p.ldq, a.p.ldq_out);
+  pass(a.k, a.ko, a.p.heads_k, a.p.ldk, a.p.ldk_out);
 }
 
 template <int DT, int VEC>
@@ -122,7 +147,13 @@ int rope_launch(BwppCudaCtx *ctx, RopeArgs &a) {
   a.turn_slots = (pairs_in_one ? R : R / 2) / VEC;
   const bool in_place = a.qo == a.q && a.ko == a.k;
   a.slots = a.turn_slots + (in_place ? 0 : (p.head_dim - R) / VEC);
-  a.lanes = p.heads_q + p.heads_k;
+  // A thread per head and slot for few tokens, where latency counts; a thread
+  // takes a batch of heads of q and of k where that still leaves 1024 threads
+  // per SM (4084 tokens x 32 heads x 128 fp32: 33.7 us without, 23.2 with).
+  const uint32_t kBatch = batch_of(pairs_in_one);
+  a.lanes = p.heads_q > p.heads_k ? p.heads_q : p.heads_k;
+  if ((uint64_t)p.tokens * a.slots * a.lanes > (uint64_t)ctx->num_sms * 1024 * kBatch)
+    a.lanes = (a.lanes + kBatch - 1) / kBatch;
   const uint64_t per = (uint64_t)a.slots * a.lanes;
   const uint64_t most = (1u << 30) / per;  // tokens of a launch: unit ids stay in 31 bits
   if (most == 0)
