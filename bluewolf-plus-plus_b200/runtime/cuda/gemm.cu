@@ -343,16 +343,18 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + stage * A_STAGE);
           const uint32_t b0 = smem_u32(smem + Cfg::OFF_B + stage * Cfg::B_STAGE);
+          // K-major, 128-B swizzle: a K step of 16 bf16 is 32 bytes inside
+          // the swizzle atom; 8-row groups 1 KB apart (SBO).
+          // MN-major, 128-B swizzle: 64-element MN atoms 8 KB apart (LBO),
+          // 8-row K groups 1 KB apart (SBO); a K step of 16 rows is 2 KB.
+          // Built once a stage and stepped: 1.5-2% faster over seconds than
+          // four pairs built from the addresses.
+          const uint64_t ad0 = make_smem_desc(a0, A_MN ? B_SUB : 16, 1024, BWPP_SWIZZLE_128B);
+          const uint64_t bd0 = make_smem_desc(b0, B_MN ? B_SUB : 16, 1024, BWPP_SWIZZLE_128B);
 #pragma unroll
           for (int ks = 0; ks < BK / 16; ++ks) {
-            // K-major, 128-B swizzle: a K step of 16 bf16 is 32 bytes inside
-            // the swizzle atom; 8-row groups 1 KB apart (SBO).
-            // MN-major, 128-B swizzle: 64-element MN atoms 8 KB apart (LBO),
-            // 8-row K groups 1 KB apart (SBO); a K step of 16 rows is 2 KB.
-            const uint64_t ad = A_MN ? make_smem_desc(a0 + ks * 2048, B_SUB, 1024, BWPP_SWIZZLE_128B)
-                                     : make_smem_desc(a0 + ks * 32, 16, 1024, BWPP_SWIZZLE_128B);
-            const uint64_t bd = B_MN ? make_smem_desc(b0 + ks * 2048, B_SUB, 1024, BWPP_SWIZZLE_128B)
-                                     : make_smem_desc(b0 + ks * 32, 16, 1024, BWPP_SWIZZLE_128B);
+            const uint64_t ad = desc_add(ad0, ks * (A_MN ? 2048 : 32));
+            const uint64_t bd = desc_add(bd0, ks * (B_MN ? 2048 : 32));
             const uint32_t accum = (kb != x.kb0 || ks != 0) ? 1u : 0u;
             if constexpr (PAIR) tc_mma_f16_ss_pair(d_tmem, ad, bd, idesc, accum);
             else tc_mma_f16_ss(d_tmem, ad, bd, idesc, accum);

@@ -214,24 +214,61 @@ __device__ __forceinline__ void chunk_range(const JunctionArgs &a, uint32_t k, u
   last = (uint32_t)min(f + a.chunk_rows, end);
 }
 
+// Sums NV values over the TPR threads of a row with one barrier; `red` may be
+// used again once another barrier of the block has passed.
+template <int TPR, int NV>
+__device__ __forceinline__ void row_sum_once(float (&v)[NV], float (*red)[32]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) red[j][threadIdx.x >> 5] = v[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      v[j] = red[j][0];
+#pragma unroll
+      for (int w = 1; w < TPR / 32; ++w) v[j] += red[j][w];
+    }
+  }
+}
+
+// Rows in registers: narrow ones, a warp each, and those that 16-byte pieces
+// do not fit.  A row's loads are issued before the row in front of it is
+// worked on; gains and the chunk's gate row stay in registers.
 template <int DT, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(block_threads(TPR))
     junction_bwd_kernel(const __grid_constant__ JunctionArgs a) {
   using T = typename Elem<DT>::type;
   constexpr int RPB = block_threads(TPR) / TPR;  // rows that a block works on together
-  __shared__ float red[3 * 32];
+  __shared__ float red[3][32], red1[1][32];
   const BwppCudaJunctionParams &p = a.p;
   const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   uint32_t first, last;
   chunk_range(a, blockIdx.x, first, last);
   const float inv_c = 1.0f / (float)p.cols;
-  float acc_post[NV][VEC], acc_pre[NV][VEC];
+  const bool token = p.gate_rows == 1 && a.gate;
+  // gain_pre, and gain_post times the chunk's gate row
+  float gq[NV][VEC], gp[NV][VEC], acc_post[NV][VEC], acc_pre[NV][VEC];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t c = (t + i * TPR) * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc_post[i][e] = acc_pre[i][e] = 0.0f;
+    for (int e = 0; e < VEC; ++e) acc_post[i][e] = acc_pre[i][e] = gq[i][e] = gp[i][e] = 0.0f;
+    if (c >= p.cols || first >= last) continue;
+    load_gain<VEC>(a.gain_pre, c, gq[i]);
+    load_gain<VEC>(p.norm_after ? a.gain_post : nullptr, c, gp[i]);
+    if (!token && a.gate) {
+      float gt[VEC];
+      load_gain<VEC>(a.gate + (size_t)(first / p.gate_rows) * p.ldgate, c, gt);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) gp[i][e] *= gt[e];
+    }
+  }
 
-  // a row's loads are issued before the row in front of it is worked on
   Raw<F32, VEC> hn[NV], dn[NV];
   Raw<DT, VEC> bn[NV], yn[NV];
   auto fetch = [&](uint32_t r) {
@@ -266,62 +303,52 @@ __global__ void __launch_bounds__(block_threads(TPR))
     fetch(r + RPB);
     float s[3] = {0.0f, 0.0f, 0.0f};  // sum h'^2, sum gain_pre dy h', sum b^2
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t c = (t + i * TPR) * VEC;
-      if (c >= p.cols) continue;
-      float gq[VEC];
-      load_gain<VEC>(a.gain_pre, c, gq);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float hh = hv[i].get(e), bb = bv[i].get(e);
         s[0] += hh * hh;
-        s[1] += gq[e] * yv[i].get(e) * hh;
+        s[1] += gq[i][e] * yv[i].get(e) * hh;
         s[2] += bb * bb;
       }
-    }
-    row_sum<TPR, 3>(s, red);
+    row_sum_once<TPR, 3>(s, red);
     const float rh = a.dy ? 1.0f / sqrtf(s[0] * inv_c + p.eps_pre) : 0.0f;
     const float m2 = rh * s[1] * inv_c;  // mean(g hat)
     const float rb = p.norm_after ? 1.0f / sqrtf(s[2] * inv_c + p.eps_post) : 1.0f;
-    const float *gate = a.gate ? a.gate + (size_t)(r / p.gate_rows) * p.ldgate : nullptr;
-    float *dgate = a.dgate ? a.dgate + (size_t)r * p.ldgate : nullptr;
+    const float *gate = token ? a.gate + (size_t)r * p.ldgate : nullptr;
     float m[1] = {0.0f};  // sum gain_post du bhat
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * TPR) * VEC;
       if (c >= p.cols) continue;
-      float gq[VEC], gp[VEC], gt[VEC], w[VEC], dg[VEC];
-      load_gain<VEC>(a.gain_pre, c, gq);
-      load_gain<VEC>(p.norm_after ? a.gain_post : nullptr, c, gp);
+      float gt[VEC], w[VEC], dg[VEC], gu[VEC];
       load_gain<VEC>(gate, c, gt);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const float hat = hv[i].get(e) * rh, dy = yv[i].get(e);
-        const float dH = dv[i].get(e) + rh * (gq[e] * dy - hat * m2);
+        const float dH = dv[i].get(e) + rh * (gq[i][e] * dy - hat * m2);
         const float bh = bv[i].get(e) * rb, ee = p.scale_b * dH;
-        const float du = ee * gt[e];
+        gu[e] = gp[i][e] * gt[e] * ee;  // gain_post du
         acc_pre[i][e] += dy * hat;
-        acc_post[i][e] += (p.gate_rows == 1 ? du : ee) * bh;
-        m[0] += gp[e] * du * bh;
-        dg[e] = ee * bh * gp[e];
+        acc_post[i][e] += gt[e] * ee * bh;
+        m[0] += gu[e] * bh;
+        dg[e] = ee * bh * gp[i][e];
         w[e] = p.scale_h * dH;
-        // kept for the second pass: gain_post du in place of dh'
-        gp[e] *= du;
       }
-      if (dgate) {
+      if (token && a.dgate) {
         Raw<F32, VEC> o;
         o.set(dg);
-        o.store(dgate + c);
+        o.store(a.dgate + (size_t)r * p.ldgate + c);
       }
       if (a.dh) {
         Raw<F32, VEC> o;
         o.set(w);
         o.store(a.dh + (size_t)r * p.ldh + c);
       }
-      dv[i].set(gp);
+      dv[i].set(gu);  // in place of dh'
     }
+    row_sum_once<TPR, 1>(m, red1);
     if (!a.db) continue;
-    if (p.norm_after) row_sum<TPR, 1>(m, red);
     const float m1 = p.norm_after ? m[0] * inv_c : 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -658,10 +685,7 @@ struct JunctionSums {
   const float *gain_post, *gate;
   float *dgain_post, *dgain_pre, *dgate;
   uint32_t chunks, chunks_per_group, cols, ldgate;
-  // dgain_post weights the partial rows with their gate rows: k / d is the high
-  // word of k * ceil(2^64 / d), exactly for k and d below 2^31 (0: not weighted;
-  // a divide for each term cost more than the sums, 4.3 us of 8.8)
-  uint64_t group_inv;
+  int weighted;  // dgain_post: weight the partial rows with their gate rows
 };
 
 constexpr int kSumWarps = 32;
@@ -675,26 +699,39 @@ __global__ void __launch_bounds__(32 * kSumWarps) junction_sums_kernel(const Jun
   const float *part = job == 1 ? a.part_pre : a.part_post;
   const uint32_t begin = job < 2 ? 0 : (job - 2) * a.chunks_per_group;
   const uint32_t end = job < 2 ? a.chunks : begin + a.chunks_per_group;
-  float acc = 0.0f;
-  if (c < a.cols) {
-    constexpr int U = 8;  // rows in flight
-    for (uint32_t k0 = begin + warp; k0 < end; k0 += U * kSumWarps) {
-      float v[U];
+  // rows k, k + kSumWarps, ... below `to`, eight loads in flight; `weight(k)`
+  // is NULL or the gate row of chunk k
+  auto add = [&](uint32_t k, uint32_t to, auto weight) {
+    constexpr int U = 8;
+    float sum = 0.0f;
+    for (; k < to; k += U * kSumWarps) {
+      float v[U], w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const uint32_t k = k0 + u * kSumWarps;
-        v[u] = k < end ? __ldg(part + (size_t)k * a.cols + c) : 0.0f;
-      }
-      if (job == 0 && a.group_inv) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const uint32_t k = k0 + u * kSumWarps;
-          const uint64_t g = a.chunks_per_group == 1 ? k : __umul64hi(k, a.group_inv);
-          if (k < end) v[u] *= __ldg(a.gate + g * a.ldgate + c);
-        }
+        const uint32_t at = k + u * kSumWarps;
+        const float *g = weight(at);
+        v[u] = at < to ? __ldg(part + (size_t)at * a.cols + c) : 0.0f;
+        w[u] = g && at < to ? __ldg(g + c) : 1.0f;
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) acc += v[u];
+      for (int u = 0; u < U; ++u) sum += v[u] * w[u];
+    }
+    return sum;
+  };
+  auto plain = [](uint32_t) { return (const float *)nullptr; };
+  float acc = 0.0f;
+  if (c < a.cols) {
+    if (job || !a.weighted) {
+      acc = add(begin + warp, end, plain);
+    } else if (a.chunks_per_group >= (uint32_t)kSumWarps) {
+      // groups that keep every warp busy: one weight for each
+      for (uint32_t k = 0, g = 0; k < a.chunks; k += a.chunks_per_group, ++g) {
+        const float w = __ldg(a.gate + (size_t)g * a.ldgate + c);
+        acc += w * add(k + warp, k + a.chunks_per_group, plain);
+      }
+    } else {
+      acc = add(warp, a.chunks,
+                [&](uint32_t k) { return a.gate + (size_t)(k / a.chunks_per_group) * a.ldgate; });
     }
   }
   sums[warp][lane] = acc;
@@ -720,7 +757,7 @@ struct Chunks {
 // A chunk holds consecutive rows of one group (rows that share a gate row and
 // whose dgate is summed), about `per_sm` chunks per SM (at most kMaxPerSm,
 // which the scratch is sized for).
-constexpr uint32_t kMaxPerSm = 8, kPerSm = 4;
+constexpr uint32_t kMaxPerSm = 8;
 bool make_chunks(BwppCudaCtx *ctx, uint32_t rows, uint32_t gate_rows, uint32_t per_sm, Chunks &k) {
   k.group_rows = gate_rows <= 1 || gate_rows > rows ? rows : gate_rows;
   k.groups = (uint32_t)(((uint64_t)rows + k.group_rows - 1) / k.group_rows);
@@ -792,16 +829,19 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
 #undef BWPP_FWD
 }
 
-// How the staged backward takes a row width: stages and resident CTAs per SM
-// (stages 0: it does not take it).
-struct Staged {
+// How the backward takes a row width: CTAs per SM (as many as are resident:
+// 4055 x 1003 fp32 took 23.0 us with the 3 that fit, 26.8 with 4), and for rows
+// staged in shared memory the stages (else 0).
+struct Plan {
   uint32_t stages, per_sm, bytes;
 };
 template <int DT>
-Staged staged(const JunctionArgs &a) {
-  Staged g{0, kPerSm, 0};
+Plan plan_bwd(const JunctionArgs &a) {
   const uint32_t cols = a.p.cols;
-  if (!vectors<DT>(a) || cols <= 256 || cols > 8192) return g;
+  const bool vec = vectors<DT>(a);
+  const Plan held{0, vec && cols <= 256 ? 4u : cols <= 128 ? 6u : cols <= 1024 ? 3u : cols <= 4096 ? 1u : 2u, 0};
+  if (!vec || cols <= 256 || cols > 8192) return held;
+  Plan g{0, 0, 0};
   const bool token = a.p.gate_rows == 1 && a.gate;
   const uint32_t row = cols * (8 + (token ? 4 : 0) + 2 * (uint32_t)sizeof(typename Elem<DT>::type));
   constexpr uint32_t sm = 220 * 1024;  // of an SM's 228 KB; 1 KB and the static part go with each CTA
@@ -814,7 +854,7 @@ Staged staged(const JunctionArgs &a) {
     g.stages = sm / per / row;
   }
   if (g.stages > (uint32_t)kMaxStages) g.stages = kMaxStages;
-  if (g.stages < 2) g = Staged{0, kPerSm, 0};
+  if (g.stages < 2) return held;
   g.bytes = g.stages * row;
   return g;
 }
@@ -822,7 +862,7 @@ Staged staged(const JunctionArgs &a) {
 bool g_staged_set[64][32] = {};
 
 template <int DT, int NV, int TPR, bool TOKEN>
-int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Staged &g, int id) {
+int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Plan &g, int id) {
   auto kern = junction_bwd_staged_kernel<DT, NV, TPR, TOKEN>;
   const int dev = ctx->device;
   if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction: device index >= 64");
@@ -839,7 +879,7 @@ int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, cons
 }
 
 template <int DT, bool TOKEN>
-int launch_staged_any(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Staged &g) {
+int launch_staged_any(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Plan &g) {
   const uint32_t cols = a.p.cols;
   if (cols <= 512) return launch_staged<DT, 2, 64, TOKEN>(ctx, a, chunks, g, 0);
   if (cols <= 1024) return launch_staged<DT, 2, 128, TOKEN>(ctx, a, chunks, g, 1);
@@ -849,7 +889,7 @@ int launch_staged_any(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, 
 }
 
 template <int DT>
-int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Staged &g) {
+int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Plan &g) {
   const uint32_t cols = a.p.cols;
   cudaStream_t s = ctx->stream;
   if (g.stages)
@@ -863,7 +903,6 @@ int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const S
     if (cols <= 128) BWPP_BWD(1, 4, 32);
     else if (cols <= 1024) BWPP_BWD(1, 4, 256);
     else if (cols <= 4096) BWPP_BWD(1, 8, 512);
-    else if (cols <= 8192) BWPP_BWD(1, 8, 1024);
     else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
   }
 #undef BWPP_BWD
@@ -938,7 +977,7 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
   a.db = db;
   const bool per_row = a.p.gate_rows == 1;
   a.dgate = per_row ? dgate : nullptr;
-  const Staged g = staged<DT>(a);
+  const Plan g = plan_bwd<DT>(a);
   Chunks k;
   if (!make_chunks(ctx, a.p.rows, a.p.gate_rows, g.per_sm, k))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: too many gate rows");
@@ -971,8 +1010,7 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
     q.chunks_per_group = k.per_group;
     q.cols = a.p.cols;
     q.ldgate = a.p.ldgate;
-    q.group_inv = gate && !per_row ? ~0ull / k.per_group + 1 : 0;
-    if (gate && !per_row && k.per_group == 1) q.group_inv = 1;
+    q.weighted = gate && !per_row;
     const dim3 grid(2 + (q.dgate ? k.groups : 0), (a.p.cols + 31) / 32);
     if (grid.y > 65535)
       return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: row too wide");

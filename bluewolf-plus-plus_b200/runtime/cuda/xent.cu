@@ -38,65 +38,83 @@ using bwpp_elem::aligned_to;
 
 constexpr int kThreads = 256;
 
-// dst[r, c] = src[r, c] of 16-bit elements, eight a thread, into rows of 16
-// bytes (the last eight filled up with zeros).  With targets, rows that are
-// ignored become zero, and a target outside the vocabulary is reported.
+// Copies between rows of any pitch and rows of 16 bytes in scratch, for the
+// operands and results that TMA does not take as they are.  A warp takes
+// kSpan consecutive elements of a row.  (A thread with eight elements of its
+// own, as 2-byte accesses 16 bytes apart, took 60 us for 1001 x 10007 bf16.)
+constexpr uint32_t kSpan = 256;
+
+// dst[r, c] = src[r, c] of 16-bit elements; dst's rows are filled up with zeros
+// to a multiple of eight.  With targets, rows that are ignored become zero, and
+// a target outside the vocabulary is reported.
 __global__ void __launch_bounds__(kThreads)
     pack_rows_kernel(const uint16_t *__restrict__ src, uint16_t *__restrict__ dst, uint32_t rows,
                      uint32_t cols, size_t ld_src, size_t ld_dst, int wide, const int32_t *target,
                      uint32_t V, int *status) {
-  const uint32_t chunks = (cols + 7) / 8, i = blockIdx.x * kThreads + threadIdx.x;
-  if (i >= rows * chunks) return;
-  const uint32_t r = i / chunks, c = (i - r * chunks) * 8;
+  const uint32_t spans = (cols + kSpan - 1) / kSpan;
+  const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) / 32, lane = threadIdx.x & 31;
+  if (i >= rows * spans) return;
+  const uint32_t r = i / spans, c0 = (i - r * spans) * kSpan;
   bool live = true;
   if (target) {
     const int32_t y = target[r];
     live = (uint32_t)y < V;
-    if (y >= 0 && !live && c == 0) bwpp_report(status, BWPP_CUDA_ERR_ARG);
+    if (y >= 0 && !live && c0 + lane == 0) bwpp_report(status, BWPP_CUDA_ERR_ARG);
   }
-  uint4 t = make_uint4(0u, 0u, 0u, 0u);
-  if (live) {
-    const uint16_t *p = src + r * ld_src + c;
-    if (wide && c + 8 <= cols) {
-      t = __ldg(reinterpret_cast<const uint4 *>(p));
-    } else {
-      uint32_t w[8];
+  const uint16_t *from = src + r * ld_src;
+  uint16_t *to = dst + r * ld_dst;
+  const uint32_t padded = (cols + 7) & ~7u;
+  if (wide && c0 + kSpan <= cols) {
+    const uint32_t c = c0 + lane * 8;
+    *reinterpret_cast<uint4 *>(to + c) =
+        live ? __ldg(reinterpret_cast<const uint4 *>(from + c)) : make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  uint32_t v[kSpan / 64];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = c + e < cols ? __ldg(p + e) : 0u;
-      t = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-    }
+  for (uint32_t k = 0; k < kSpan / 64; ++k) {
+    const uint32_t c = c0 + k * 64 + lane * 2;
+    const uint32_t lo = live && c < cols ? __ldg(from + c) : 0u;
+    const uint32_t hi = live && c + 1 < cols ? __ldg(from + c + 1) : 0u;
+    v[k] = lo | hi << 16;
   }
-  *reinterpret_cast<uint4 *>(dst + r * ld_dst + c) = t;
+#pragma unroll
+  for (uint32_t k = 0; k < kSpan / 64; ++k) {
+    const uint32_t c = c0 + k * 64 + lane * 2;
+    if (c < padded) *reinterpret_cast<uint32_t *>(to + c) = v[k];
+  }
 }
 
-// Results from 16-byte rows of scratch into rows of any pitch, ES bytes an
-// element, 16 bytes a thread.
+// Results from rows of 16 bytes in scratch into rows of any pitch.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     unpack_rows_kernel(const T *__restrict__ src, T *__restrict__ dst, uint32_t rows, uint32_t cols,
                        size_t ld_src, size_t ld_dst) {
-  constexpr uint32_t N = 16 / sizeof(T);
-  const uint32_t chunks = (cols + N - 1) / N, i = blockIdx.x * kThreads + threadIdx.x;
-  if (i >= rows * chunks) return;
-  const uint32_t r = i / chunks, c = (i - r * chunks) * N;
-  union {
-    uint4 q;
-    T e[N];
-  } t;
-  t.q = *reinterpret_cast<const uint4 *>(src + r * ld_src + c);
+  const uint32_t spans = (cols + kSpan - 1) / kSpan;
+  const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) / 32, lane = threadIdx.x & 31;
+  if (i >= rows * spans) return;
+  const uint32_t r = i / spans, c0 = (i - r * spans) * kSpan;
+  T v[kSpan / 32];
 #pragma unroll
-  for (uint32_t e = 0; e < N; ++e)
-    if (c + e < cols) dst[r * ld_dst + c + e] = t.e[e];
+  for (uint32_t k = 0; k < kSpan / 32; ++k) {
+    const uint32_t c = c0 + k * 32 + lane;
+    if (c < cols) v[k] = __ldg(src + r * ld_src + c);
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kSpan / 32; ++k) {
+    const uint32_t c = c0 + k * 32 + lane;
+    if (c < cols) dst[r * ld_dst + c] = v[k];
+  }
 }
 
 int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t rows, uint32_t cols,
               uint32_t ld_src, uint32_t ld_dst, const int32_t *target, uint32_t V) {
-  const uint32_t chunks = (cols + 7) / 8;
+  const uint32_t spans = (cols + kSpan - 1) / kSpan;
   const int wide = ld_src % 8 == 0 && aligned_to(src, 16);
-  const uint32_t most = (1u << 30) / chunks;  // rows of a launch: indices stay in 31 bits
+  const uint32_t most = (1u << 25) / spans;  // rows of a launch: indices stay in 31 bits
   for (uint32_t r0 = 0; r0 < rows; r0 += most) {
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
-    pack_rows_kernel<<<(n * chunks + kThreads - 1) / kThreads, kThreads, 0, ctx->stream>>>(
+    pack_rows_kernel<<<(n * spans + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, ctx->stream>>>(
         src + (size_t)r0 * ld_src, dst + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst, wide,
         target ? target + r0 : nullptr, V, ctx->status_word);
     BWPP_LAUNCH_CHECK(ctx, "xent pack");
@@ -107,11 +125,11 @@ int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t row
 template <typename T>
 int unpack_rows(BwppCudaCtx *ctx, const void *src, void *dst, uint32_t rows, uint32_t cols,
                 uint32_t ld_src, uint32_t ld_dst) {
-  const uint32_t chunks = (cols + 16 / sizeof(T) - 1) / (16 / sizeof(T));
-  const uint32_t most = (1u << 30) / chunks;
+  const uint32_t spans = (cols + kSpan - 1) / kSpan;
+  const uint32_t most = (1u << 25) / spans;
   for (uint32_t r0 = 0; r0 < rows; r0 += most) {
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
-    unpack_rows_kernel<T><<<(n * chunks + kThreads - 1) / kThreads, kThreads, 0, ctx->stream>>>(
+    unpack_rows_kernel<T><<<(n * spans + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, ctx->stream>>>(
         static_cast<const T *>(src) + (size_t)r0 * ld_src, static_cast<T *>(dst) + (size_t)r0 * ld_dst,
         n, cols, ld_src, ld_dst);
     BWPP_LAUNCH_CHECK(ctx, "xent unpack");
@@ -136,14 +154,16 @@ uint32_t clamp_piece(uint64_t c, uint32_t V) {
   return (uint32_t)(c < all ? c : all);
 }
 
-// Vocabulary columns of a piece.  Backward: about 2^26 dlogit at a time.
+// Vocabulary columns of a piece.  Backward: about 2^27 dlogit at a time (T 8192,
+// V 32000, D 2048: 3300 us at 2^24, 2883 at 2^25, 2744 at 2^26, 2692 at 2^27,
+// where dx is read and written back once; 2659 with all of them kept).
 // Forward: the whole vocabulary, or about 2^25 weights at a time where they
 // are packed.
 Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool backward, bool stage_dx,
                  bool stage_dw) {
   Layout l{};
   l.dp = up8(p.D);
-  l.piece = backward ? clamp_piece((1ull << 26) / p.T, p.V)
+  l.piece = backward ? clamp_piece((1ull << 27) / p.T, p.V)
                      : clamp_piece(pack_w ? (1ull << 25) / l.dp : (uint64_t)p.V + 255, p.V);
   size_t at = 0;
   auto take = [&](size_t bytes) {

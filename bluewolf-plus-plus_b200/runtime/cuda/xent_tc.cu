@@ -60,6 +60,9 @@ struct XentTile {
   const float *lse, *dloss;
   float scale;
   uint32_t vocab;       // targets below it are live
+  // items [0, whole) are tiles, from there on each remaining tile is cut into
+  // two of 128 columns, so that a short last round spreads over twice the workers
+  uint32_t whole, items;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -76,6 +79,18 @@ __device__ __forceinline__ void tile_at(uint32_t i, uint32_t tiles_m, uint32_t t
   nb = r / gm;
 }
 
+// Item i: its row block, first column and width.
+__device__ __forceinline__ void item_at(const XentTile &a, uint32_t i, uint32_t tiles_m,
+                                        uint32_t tiles_n, uint32_t &mb, uint32_t &col,
+                                        uint32_t &width) {
+  const bool half = i >= a.whole;
+  const uint32_t j = i - a.whole;
+  uint32_t nb;
+  tile_at(half ? a.whole + j / 2 : i, tiles_m, tiles_n, mb, nb);
+  width = half ? BN / 2 : BN;
+  col = nb * BN + (half ? (j & 1) * (BN / 2) : 0);
+}
+
 template <bool B_MN, bool PAIR, bool FWD>
 __global__ void __launch_bounds__(THREADS, 1)
     xent_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -83,7 +98,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   using C = Cfg<PAIR>;
   constexpr int STAGES = C::STAGES;
   constexpr uint32_t IDESC = make_idesc_bf16_f32(C::TILE_M, BN, 0u, B_MN ? 1u : 0u);
-  constexpr int B_BOXES = C::B_STAGE / B_BOX;
+  constexpr uint32_t IDESC_HALF = make_idesc_bf16_f32(C::TILE_M, BN / 2, 0u, B_MN ? 1u : 0u);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t *smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -100,7 +115,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t worker = PAIR ? cluster_id_x() : blockIdx.x;
   const uint32_t workers = PAIR ? cluster_count_x() : gridDim.x;
   const uint32_t tiles_m = (a.T + C::TILE_M - 1) / C::TILE_M, tiles_n = (a.V + BN - 1) / BN;
-  const uint32_t tiles = tiles_m * tiles_n, num_kb = (a.D + BK - 1) / BK;
+  const uint32_t num_kb = (a.D + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -135,11 +150,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
-      for (uint32_t i = worker; i < tiles && !*abort_flag; i += workers) {
-        uint32_t mb, nb;
-        tile_at(i, tiles_m, tiles_n, mb, nb);
+      for (uint32_t i = worker; i < a.items && !*abort_flag; i += workers) {
+        uint32_t mb, col, width;
+        item_at(a, i, tiles_m, tiles_n, mb, col, width);
+        const uint32_t mine = PAIR ? width / 2 : width;  // columns that this CTA loads
         const int32_t row0 = (int32_t)(mb * C::TILE_M + rank * BM);
-        const int32_t col0 = (int32_t)(nb * BN + rank * (BN / 2));  // rank is 0 for one CTA
+        const int32_t col0 = (int32_t)(col + rank * mine);
         for (uint32_t kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, status)) {
             *abort_flag = 1;
@@ -147,7 +163,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           // both CTAs' bytes count on rank 0's barrier
           if (rank == 0)
-            mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * (A_STAGE + C::B_STAGE));
+            mbar_arrive_expect_tx(&full[stage], (PAIR ? 2 : 1) * (A_STAGE + mine * BK * 2));
           uint32_t fbar = 0;
           if constexpr (PAIR) fbar = cluster_addr(&full[stage], 0);
           auto load = [&](void *dst, const CUtensorMap *map, int32_t x, int32_t y) {
@@ -157,10 +173,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int32_t k0 = (int32_t)(kb * BK);
           uint8_t *sb = smem + C::OFF_B + stage * C::B_STAGE;
           load(smem + stage * A_STAGE, &tmX, k0, row0);
-#pragma unroll
-          for (int j = 0; j < B_BOXES; ++j) {
-            if (B_MN) load(sb + j * B_BOX, &tmW, col0 + j * 64, k0);
-            else load(sb + j * B_BOX, &tmW, k0, col0 + j * 64);
+          for (uint32_t j = 0; j < mine / 64; ++j) {
+            if (B_MN) load(sb + j * B_BOX, &tmW, col0 + (int32_t)j * 64, k0);
+            else load(sb + j * B_BOX, &tmW, k0, col0 + (int32_t)j * 64);
           }
           if (++stage == STAGES) {
             stage = 0;
@@ -180,12 +195,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       };
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      for (uint32_t i = worker; i < tiles && !*abort_flag; i += workers) {
+      for (uint32_t i = worker; i < a.items && !*abort_flag; i += workers) {
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status)) {
           *abort_flag = 1;
           break;
         }
         tc_fence_after();
+        uint32_t mb, col, width;
+        item_at(a, i, tiles_m, tiles_n, mb, col, width);
+        const uint32_t idesc = width == BN ? IDESC : IDESC_HALF;
         bool ok = true;
         for (uint32_t kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&full[stage], phase, status)) {
@@ -204,8 +222,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int ks = 0; ks < BK / 16; ++ks) {
             const uint64_t as = desc_add(ad, ks * 32), bs = desc_add(bd, ks * (B_MN ? 2048 : 32));
             const uint32_t accum = (kb | (uint32_t)ks) != 0 ? 1u : 0u;
-            if constexpr (PAIR) tc_mma_f16_ss_pair(tmem_base + acc * BN, as, bs, IDESC, accum);
-            else tc_mma_f16_ss(tmem_base + acc * BN, as, bs, IDESC, accum);
+            if constexpr (PAIR) tc_mma_f16_ss_pair(tmem_base + acc * BN, as, bs, idesc, accum);
+            else tc_mma_f16_ss(tmem_base + acc * BN, as, bs, idesc, accum);
           }
           commit(&empty[stage]);
           if (++stage == STAGES) {
@@ -228,11 +246,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int sub = ew >> 2;           // columns [128 sub, 128 sub + 128) of the tile
     const uint32_t tq = (uint32_t)(q * 32) << 16;
     uint32_t acc = 0, acc_phase = 0;
-    for (uint32_t i = worker; i < tiles && !*abort_flag; i += workers) {
-      uint32_t mb, nb;
-      tile_at(i, tiles_m, tiles_n, mb, nb);
+    for (uint32_t i = worker; i < a.items && !*abort_flag; i += workers) {
+      uint32_t mb, col, width;
+      item_at(a, i, tiles_m, tiles_n, mb, col, width);
       const uint32_t row0 = mb * C::TILE_M + rank * BM + q * 32, row = row0 + lane;
-      const uint32_t first = nb * BN + sub * 128;  // this warp's first column
+      const uint32_t first = col + sub * 128;  // this warp's first column
+      const uint32_t end = min(a.V, col + width);
       const bool live_row = row < a.T;
       const int32_t target = live_row && a.target ? __ldg(a.target + row) : -1;
       // the target's column within this warp's 128, or beyond them
@@ -253,12 +272,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
       const uint32_t taddr = tmem_base + tq + acc * BN + sub * 128;
       if constexpr (FWD) {
-        if (first < a.V) {
+        if (first < end) {
           float m = -INFINITY, s = 0.0f;
 #pragma unroll 1
           for (int k = 0; k < 4; ++k) {
             const uint32_t cs = first + k * 32;
-            if (cs >= a.V) break;
+            if (cs >= end) break;
             uint32_t r[32];
             tmem_ld_32x32b_x32(taddr + k * 32, r);
             tc_wait_ld(r);
@@ -296,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
         for (int k = 0; k < 2; ++k) {  // 64 columns: 128 bytes of bf16
           const uint32_t cs = first + k * 64;
-          if (cs >= a.V) break;
+          if (cs >= end) break;
           uint32_t out[32];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -436,10 +455,15 @@ int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const
   }
   const uint64_t tiles = ((uint64_t)a.T + C::TILE_M - 1) / C::TILE_M * (((uint64_t)a.V + BN - 1) / BN);
   if (tiles >= 0x80000000ull) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: T * V too large");
-  const uint32_t n = tiles < cap ? (uint32_t)tiles : cap;
+  XentTile b = a;
+  const uint32_t tail = (uint32_t)(tiles % cap);
+  const bool halve = tail > 0 && 2 * tail <= cap;
+  b.whole = (uint32_t)tiles - (halve ? tail : 0);
+  b.items = (uint32_t)tiles + (halve ? tail : 0);
+  const uint32_t n = b.items < cap ? b.items : cap;
   cfg.gridDim = dim3((PAIR ? 2 : 1) * n, 1, 1);
   int *status = ctx->status_word;
-  return bwpp_check_cuda(ctx, cudaLaunchKernelEx(&cfg, kern, tx, tw, to, a, status),
+  return bwpp_check_cuda(ctx, cudaLaunchKernelEx(&cfg, kern, tx, tw, to, b, status),
                          FWD ? "xent logits" : "xent dlogit");
 }
 
