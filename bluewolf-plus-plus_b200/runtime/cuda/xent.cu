@@ -9,8 +9,8 @@
 // The products run on the tensor cores (xent_tc.cu): the forward's logits are
 // folded into a (maximum, sum) pair per row and 128 columns in the product's
 // epilogue.  The backward computes them again, a piece of the vocabulary at a
-// time, and writes bf16 dlogit; two GEMMs add the piece's share to dx (in
-// fp32) and write its part of dW.
+// time, and writes bf16 dlogit; one launch of two products (xent_grad.cu) adds
+// the piece's share to dx (in fp32) and writes its part of dW.
 //
 // A negative target ignores its row: loss 0, no share in any gradient (its x
 // may hold anything, so the backward reads a copy of x with such rows zeroed:
@@ -24,13 +24,6 @@
 #include "bwpp_cuda_internal.cuh"
 #include "elem.cuh"
 #include "xent.cuh"
-
-int bwpp_gemm_launch_dt(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint32_t lda,
-                        const uint16_t *b, int b_mn, uint32_t ldb, void *c,
-                        uint32_t ldc, uint32_t M, uint32_t N, uint32_t K,
-                        const float *bias, int silu, const void *residual,
-                        uint32_t ldr, int out_bf16, int force_simt, int ab_f16,
-                        int out_f16, int res16);
 
 namespace {
 
@@ -144,7 +137,9 @@ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct Layout {
   uint32_t piece;             // vocabulary columns of a piece
   uint32_t dp;                // D rounded up
-  size_t part, hit, x, w, dlogit, dx, dx16, dw, total;
+  uint32_t part_rows;         // rows of one K part of dx
+  uint32_t most_parts;        // K parts of dx that scratch has room for
+  size_t part, hit, x, w, dlogit, dx, dw, total;
 };
 
 uint32_t clamp_piece(uint64_t c, uint32_t V) {
@@ -165,6 +160,10 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
   l.dp = up8(p.D);
   l.piece = backward ? clamp_piece((1ull << 27) / p.T, p.V)
                      : clamp_piece(pack_w ? (1ull << 25) / l.dp : (uint64_t)p.V + 255, p.V);
+  l.part_rows = (p.T + 255) & ~255u;
+  // parts of dx only where they take little memory (and few tiles need them)
+  const uint64_t fit = (64ull << 20) / ((uint64_t)l.part_rows * l.dp * 4);
+  l.most_parts = fit < 1 ? 1 : fit > 8 ? 8 : (uint32_t)fit;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -179,10 +178,7 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
     l.hit = take((size_t)p.T * 4);
   } else {
     l.dlogit = take((size_t)p.T * l.piece * 2);
-    if (stage_dx) {
-      l.dx = take((size_t)p.T * l.dp * 4);
-      l.dx16 = take((size_t)p.T * l.dp * 2);
-    }
+    if (stage_dx) l.dx = take((size_t)l.most_parts * l.part_rows * l.dp * 4);
     if (stage_dw) l.dw = take((size_t)l.piece * l.dp * es);
   }
   l.total = at;
@@ -286,14 +282,44 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   if (!x || !w || !target || !lse)
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent bwd: NULL buffer");
   const bool pack_w = needs_pack(w, p.ldw);
-  const uint32_t piece = layout_of(p, true, pack_w, true, true, true).piece;
-  const bool one = piece >= p.V;
   auto tma_out = [&](const void *q, uint32_t ld) { return (size_t)ld * es % 16 == 0 && aligned_to(q, 16); };
-  // dx is summed over the pieces in fp32: in place where the caller's rows
-  // are fp32 and TMA takes them
-  const bool stage_dx = dx && (!tma_out(dx, p.lddx) || (p.grads_bf16 && !one));
-  const bool stage_dw = dw && !tma_out(dw, p.lddw);
-  const Layout l = layout_of(p, true, pack_w, true, stage_dx, stage_dw);
+  const bool dx_out = dx && tma_out(dx, p.lddx), stage_dw = dw && !tma_out(dw, p.lddw);
+  const Layout probe = layout_of(p, true, pack_w, true, true, true);
+  const uint32_t piece = probe.piece, pieces = (p.V - 1) / piece + 1;
+  const bool vm = p.w_vocab_major != 0;
+  const uint32_t ld_w = pack_w ? (vm ? probe.dp : piece) : p.ldw;
+  // The products of the piece [v0, v0 + n), with no addresses yet.
+  auto products = [&](uint32_t n, XentProduct &px, XentProduct &pw) {
+    px = XentProduct{};
+    px.M = p.T;
+    px.N = p.D;
+    px.K = n;
+    px.lda = piece;
+    px.ldb = ld_w;
+    px.b_mn = vm;  // W's rows are K here
+    px.ldc = px.ld_add = probe.dp;
+    px.part_rows = probe.part_rows;
+    pw = XentProduct{};
+    pw.M = vm ? n : p.D;
+    pw.N = vm ? p.D : n;
+    pw.K = p.T;
+    pw.lda = vm ? piece : probe.dp;
+    pw.ldb = vm ? probe.dp : piece;
+    pw.a_mn = pw.b_mn = true;
+    pw.ldc = stage_dw ? (vm ? probe.dp : piece) : p.lddw;
+    pw.bf16 = p.grads_bf16 != 0;
+  };
+  XentProduct px, pw;
+  products(piece < p.V ? piece : p.V, px, pw);
+  uint32_t parts = 1;
+  if (dx) {  // the same whether dW is wanted or not, so that dx is the same too
+    rc = bwpp_xent_dx_parts(ctx, px, pw, probe.most_parts, &parts);
+    if (rc) return rc;
+  }
+  // dx is summed in scratch, unless the caller's rows take it: all of it in one
+  // piece, or fp32 sums
+  const bool direct = dx_out && parts == 1 && (pieces == 1 || !p.grads_bf16);
+  const Layout l = layout_of(p, true, pack_w, true, dx && !direct, stage_dw);
   uint8_t *scratch;
   rc = bwpp_op_scratch(ctx, l.total, "xent bwd", &scratch);
   if (rc) return rc;
@@ -301,55 +327,42 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   rc = pack_rows(ctx, x, xp, p.T, p.D, p.ldx, l.dp, target, p.V);
   if (rc) return rc;
   uint16_t *dlogit = reinterpret_cast<uint16_t *>(scratch + l.dlogit);
-  float *dx32 = reinterpret_cast<float *>(scratch + l.dx);
   for (uint32_t v0 = 0; v0 < p.V; v0 += piece) {
     const uint32_t n = p.V - v0 < piece ? p.V - v0 : piece;
     const bool last = v0 + n == p.V;
     Piece w1;
     rc = piece_w(ctx, p, w, pack_w, reinterpret_cast<uint16_t *>(scratch + l.w), v0, n,
-                 p.w_vocab_major ? l.dp : piece, w1);
-    const XentOperands o{xp, w1.w, p.T, n, p.D, l.dp, w1.ld, v0, p.V, p.w_vocab_major != 0, p.scale};
+                 vm ? l.dp : piece, w1);
+    const XentOperands o{xp, w1.w, p.T, n, p.D, l.dp, w1.ld, v0, p.V, vm, p.scale};
     if (!rc) rc = bwpp_xent_dlogit_launch(ctx, o, target, lse, dloss, dlogit, piece);
     if (rc) return rc;
-    if (dx) {
-      // dx (+)= dlogit W: the last piece leaves the sum in the caller's rows
-      // where TMA can store them
-      const bool to_user = !stage_dx || (last && tma_out(dx, p.lddx));
-      const bool bf16_out = p.grads_bf16 && last;
-      void *out = to_user ? dx : bf16_out ? static_cast<void *>(scratch + l.dx16) : dx32;
-      const uint32_t ldo = to_user ? p.lddx : l.dp;
-      const float *sum = v0 == 0 ? nullptr : stage_dx ? dx32 : static_cast<float *>(dx);
-      rc = bwpp_gemm_launch_dt(ctx, dlogit, 0, piece, w1.w, p.w_vocab_major ? 1 : 0, w1.ld, out, ldo,
-                               p.T, p.D, n, nullptr, 0, sum, stage_dx ? l.dp : p.lddx,
-                               bf16_out ? 1 : 0, 0, 0, 0, 0);
+    products(n, px, pw);
+    px.a = dlogit;
+    px.b = w1.w;
+    px.accumulate = v0 > 0;
+    // the last piece leaves the sum in the caller's rows where it can
+    const bool to_user = direct || (dx_out && parts == 1 && last);
+    px.add = direct ? dx : static_cast<void *>(scratch + l.dx);
+    px.ld_add = direct ? p.lddx : l.dp;
+    px.c = to_user ? dx : static_cast<void *>(scratch + l.dx);
+    px.ldc = to_user ? p.lddx : l.dp;
+    px.bf16 = to_user && p.grads_bf16;
+    uint8_t *user_w = static_cast<uint8_t *>(dw) + (vm ? (size_t)v0 * p.lddw : (size_t)v0) * es;
+    pw.a = vm ? dlogit : xp;
+    pw.b = vm ? xp : dlogit;
+    pw.c = stage_dw ? static_cast<void *>(scratch + l.dw) : static_cast<void *>(user_w);
+    rc = bwpp_xent_grad_launch(ctx, dx ? &px : nullptr, dw ? &pw : nullptr, parts);
+    if (rc) return rc;
+    if (stage_dw) {
+      rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw)
+                        : unpack_rows<float>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw);
       if (rc) return rc;
-      if (!to_user && last) {
-        rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, out, dx, p.T, p.D, l.dp, p.lddx)
-                          : unpack_rows<float>(ctx, out, dx, p.T, p.D, l.dp, p.lddx);
-        if (rc) return rc;
-      }
-    }
-    if (dw) {
-      uint8_t *user = static_cast<uint8_t *>(dw) +
-                      (p.w_vocab_major ? (size_t)v0 * p.lddw : (size_t)v0) * es;
-      const uint32_t ld_staged = p.w_vocab_major ? l.dp : piece;
-      void *out = stage_dw ? static_cast<void *>(scratch + l.dw) : user;
-      const uint32_t ldo = stage_dw ? ld_staged : p.lddw;
-      if (p.w_vocab_major)  // [n, D] = dlogit^T x
-        rc = bwpp_gemm_launch_dt(ctx, dlogit, 1, piece, xp, 1, l.dp, out, ldo, n, p.D, p.T, nullptr, 0,
-                                 nullptr, 0, p.grads_bf16 ? 1 : 0, 0, 0, 0, 0);
-      else  // [D, n] = x^T dlogit
-        rc = bwpp_gemm_launch_dt(ctx, xp, 1, l.dp, dlogit, 1, piece, out, ldo, p.D, n, p.T, nullptr, 0,
-                                 nullptr, 0, p.grads_bf16 ? 1 : 0, 0, 0, 0, 0);
-      if (rc) return rc;
-      if (stage_dw) {
-        const uint32_t rows = p.w_vocab_major ? n : p.D, cols = p.w_vocab_major ? p.D : n;
-        rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, out, user, rows, cols, ldo, p.lddw)
-                          : unpack_rows<float>(ctx, out, user, rows, cols, ldo, p.lddw);
-        if (rc) return rc;
-      }
     }
   }
+  if (dx && !direct && !(dx_out && parts == 1))
+    return bwpp_xent_sum_parts_launch(ctx, reinterpret_cast<const float *>(scratch + l.dx), parts,
+                                      (size_t)l.part_rows * l.dp, dx, p.T, p.D, l.dp, p.lddx,
+                                      p.grads_bf16);
   return BWPP_CUDA_OK;
 }
 

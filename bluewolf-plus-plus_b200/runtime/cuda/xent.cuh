@@ -1,7 +1,10 @@
-// Tensor-core launches of the vocabulary cross entropy (xent_tc.cu).
+// Tensor-core launches of the vocabulary cross entropy.
+
 #pragma once
 
 #include "bwpp_cuda_internal.cuh"
+
+// ---- xent_tc.cu ----
 
 // x [T, D] and vocabulary columns [v0, v0 + V) of the weight, both with row
 // pitches of 16 bytes and 16-byte aligned bases.
@@ -23,3 +26,30 @@ int bwpp_xent_combine_launch(BwppCudaCtx *ctx, const float2 *part, uint32_t npar
 // bf16 scale * dlogit [T, ld] of the columns.
 int bwpp_xent_dlogit_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_t *target,
                             const float *lse, const float *dloss, uint16_t *dlogit, uint32_t ld);
+
+// ---- xent_grad.cu ----
+
+// C [M, N] = A [M, K] B [K, N] (+ add), bf16 operands, K-major or MN-major.
+struct XentProduct {
+  const uint16_t *a, *b;
+  void *c;
+  uint32_t M, N, K, lda, ldb, ldc;
+  bool a_mn, b_mn;
+  bool bf16;          // C bf16, else fp32
+  bool accumulate;    // add fp32 rows `add` (pitch ld_add; may be C)
+  const void *add;
+  uint32_t ld_add;
+  uint32_t part_rows; // with K parts: rows from one part's C to the next, >= M
+                      // rounded up to 256
+};
+
+// K parts of dx, at most `most`, that a launch of both would best have.
+int bwpp_xent_dx_parts(BwppCudaCtx *ctx, const XentProduct &dx, const XentProduct &dw, uint32_t most,
+                       uint32_t *parts);
+// Either may be NULL.
+int bwpp_xent_grad_launch(BwppCudaCtx *ctx, const XentProduct *dx, const XentProduct *dw,
+                          uint32_t parts);
+// out [rows, ld_out] = the sum over parts, in order, of part + s * part_stride.
+int bwpp_xent_sum_parts_launch(BwppCudaCtx *ctx, const float *part, uint32_t parts,
+                               size_t part_stride, void *out, uint32_t rows, uint32_t cols,
+                               uint32_t ld, uint32_t ld_out, int bf16);
