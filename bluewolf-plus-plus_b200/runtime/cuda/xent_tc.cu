@@ -71,6 +71,35 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Maximum and sum of exponentials over it of 2 P logits in powers of two,
+// folded into (m, s).  Paired fp32 operations, and max of three: the epilogue
+// warps share their issue slots with the thread that feeds the tensor core.
+template <int P>
+__device__ __forceinline__ void fold_logits(uint64_t (&t)[P], float &m, float &s) {
+  float top = m;
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    float x, y;
+    f2unpack(t[j], x, y);
+    asm("max.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(x), "f"(y));
+  }
+  // only -inf so far, or +inf: the exponentials are taken against 0
+  const float base = fabsf(top) == INFINITY ? 0.0f : top;
+  s *= ex2(m - base);
+  const uint64_t less = f2pack(-base, -base);
+  uint64_t sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    float x, y;
+    f2unpack(f2add(t[j], less), x, y);
+    sum[j & 3] = f2add(sum[j & 3], f2pack(ex2(x), ex2(y)));
+  }
+  float x, y;
+  f2unpack(f2add(f2add(sum[0], sum[1]), f2add(sum[2], sum[3])), x, y);
+  s += x + y;
+  m = top;
+}
+
 // Tiles go down the row blocks of a group, then to the next 256 columns.
 __device__ __forceinline__ void tile_at(uint32_t i, uint32_t group, uint32_t tiles_m,
                                         uint32_t tiles_n, uint32_t &mb, uint32_t &nb) {
@@ -92,7 +121,14 @@ __device__ __forceinline__ void item_at(const XentTile &a, uint32_t i, uint32_t 
   col = nb * BN + (half ? (j & 1) * (BN / 2) : 0);
 }
 
-template <bool B_MN, bool PAIR, bool FWD>
+// The forward's sums over D are cut into chunks of this many K blocks, each
+// summed in TMEM from zero and added to the others in registers: the tensor
+// core truncates its running sum at each addition, and over D = 4096 the
+// errors, all towards zero, reached 2e-6 of lse (6e-7 at D = 1024).
+constexpr uint32_t CHUNK = 16;
+
+// CHUNKED (FWD, D > 1024): see CHUNK.
+template <bool B_MN, bool PAIR, bool FWD, bool CHUNKED>
 __global__ void __launch_bounds__(THREADS, 1)
     xent_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ CUtensorMap tmOut, const XentTile a, int *status) {
@@ -207,6 +243,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t idesc = width == BN ? IDESC : IDESC_HALF;
         bool ok = true;
         for (uint32_t kb = 0; kb < num_kb; ++kb) {
+          if (CHUNKED && kb && kb % CHUNK == 0) {  // the next accumulator takes over
+            commit(&tfull[acc]);
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+            if (!mbar_wait(&tempty[acc], acc_phase ^ 1, status)) {
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
           if (!mbar_wait(&full[stage], phase, status)) {
             *abort_flag = 1;
             ok = false;
@@ -222,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int ks = 0; ks < BK / 16; ++ks) {
             const uint64_t as = desc_add(ad, ks * 32), bs = desc_add(bd, ks * (B_MN ? 2048 : 32));
-            const uint32_t accum = (kb | (uint32_t)ks) != 0 ? 1u : 0u;
+            const uint32_t accum = ((CHUNKED ? kb % CHUNK : kb) | (uint32_t)ks) != 0 ? 1u : 0u;
             if constexpr (PAIR) tc_mma_f16_ss_pair(tmem_base + acc * BN, as, bs, idesc, accum);
             else tc_mma_f16_ss(tmem_base + acc * BN, as, bs, idesc, accum);
           }
@@ -266,6 +313,75 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       const bool live = live_row && (uint32_t)target < a.vocab;
+      auto release = [&]() {  // the accumulator has been read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(&tempty[acc], 0));
+          else mbar_arrive(&tempty[acc]);
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      };
+      if constexpr (CHUNKED) {
+        uint64_t v[64];  // pairs of columns
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = 0ull;
+        bool ok = true;
+#pragma unroll 1
+        for (uint32_t kb = 0; kb < num_kb; kb += CHUNK) {
+          if (!mbar_wait(&tfull[acc], acc_phase, status)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          // 16 columns at a time: 32 more registers would not fit
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(tmem_base + tq + acc * BN + sub * 128 + k * 16, r);
+            tc_wait_ld16(r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[8 * k + j] = f2add(v[8 * k + j], f2pack(__uint_as_float(r[2 * j]),
+                                                        __uint_as_float(r[2 * j + 1])));
+          }
+          release();
+        }
+        if (!ok) break;
+        if (first < end) {
+          if (hit_col < 128u) {
+            float h = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+              float x, y;
+              f2unpack(v[j], x, y);
+              if (hit_col == 2u * j) h = x;
+              if (hit_col == 2u * j + 1) h = y;
+            }
+            a.hit[row] = h * a.scale;
+          }
+          const uint64_t c2 = f2pack(a.c, a.c);
+#pragma unroll
+          for (int j = 0; j < 64; ++j) v[j] = f2mul(v[j], c2);
+          if (first + 128 > end) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+              float x, y;
+              f2unpack(v[j], x, y);
+              if (first + 2 * j >= end) x = -INFINITY;
+              if (first + 2 * j + 1 >= end) y = -INFINITY;
+              v[j] = f2pack(x, y);
+            }
+          }
+          float m = -INFINITY, s = 0.0f;
+          fold_logits(v, m, s);
+          if (live_row)
+            a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);
+        }
+        continue;
+      }
       if (!mbar_wait(&tfull[acc], acc_phase, status)) {
         *abort_flag = 1;
         break;
@@ -282,9 +398,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t r[32];
             tmem_ld_32x32b_x32(taddr + k * 32, r);
             tc_wait_ld(r);
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * a.c;
             if (hit_col - k * 32 < 32u) {
               float h = 0.0f;
 #pragma unroll
@@ -292,22 +405,18 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (hit_col - k * 32 == (uint32_t)j) h = __uint_as_float(r[j]);
               a.hit[row] = h * a.scale;
             }
-            if (cs + 32 > a.V) {
+            if (cs + 32 > end) {
+              // below any logit, whatever the sign of the scale
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (cs + j >= a.V) v[j] = -INFINITY;
+                if (cs + j >= end) r[j] = __float_as_uint(a.c < 0 ? INFINITY : -INFINITY);
             }
-            float top = m;
+            const uint64_t c2 = f2pack(a.c, a.c);
+            uint64_t v[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
-            // only -inf so far, or +inf: the exponentials are taken against 0
-            const float base = fabsf(top) == INFINITY ? 0.0f : top;
-            s *= ex2(m - base);
-            float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int j = 0; j < 32; ++j) s4[j & 3] += ex2(v[j] - base);
-            s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            m = top;
+            for (int j = 0; j < 16; ++j)
+              v[j] = f2mul(f2pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2);
+            fold_logits(v, m, s);
           }
           if (live_row) a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);
         }
@@ -324,17 +433,27 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_ld_32x32b_x32(taddr + k * 64 + h * 32, r);
             tc_wait_ld(r);
             float d[32];
+            const uint64_t c2 = f2pack(a.c, a.c), l2 = f2pack(-lse2, -lse2);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) d[j] = ex2(__uint_as_float(r[j]) * a.c - lse2);
+            for (int j = 0; j < 32; j += 2) {
+              f2unpack(f2fma(f2pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), c2, l2), d[j],
+                       d[j + 1]);
+              d[j] = ex2(d[j]);
+              d[j + 1] = ex2(d[j + 1]);
+            }
             const uint32_t at = hit_col - (k * 64 + h * 32);
             if (at < 32u) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 if (at == (uint32_t)j) d[j] -= 1.0f;
             }
+            const uint64_t g2 = f2pack(g, g);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              out[h * 16 + j] = live ? pack2_16<false>(g * d[2 * j], g * d[2 * j + 1]) : 0u;
+            for (int j = 0; j < 16; ++j) {
+              float x, y;
+              f2unpack(f2mul(f2pack(d[2 * j], d[2 * j + 1]), g2), x, y);
+              out[h * 16 + j] = live ? pack2_16<false>(x, y) : 0u;
+            }
           }
           if (lane == 0) tma_store_wait_read<0>();
           __syncwarp();
@@ -350,14 +469,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(&tempty[acc], 0));
-        else mbar_arrive(&tempty[acc]);
-      }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1;
+      release();
     }
     if (!FWD && lane == 0) tma_store_wait_all<0>();
   }
@@ -411,15 +523,15 @@ __global__ void __launch_bounds__(32 * COMBINE_WARPS)
   }
 }
 
-bool g_smem_set[8][64] = {};
-int g_pairs[8][64] = {};  // resident CTA pairs per device (0: not asked yet)
+bool g_smem_set[16][64] = {};
+int g_pairs[16][64] = {};  // resident CTA pairs per device (0: not asked yet)
 
-template <bool B_MN, bool PAIR, bool FWD>
+template <bool B_MN, bool PAIR, bool FWD, bool CHUNKED>
 int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
            const XentTile &a) {
   using C = Cfg<PAIR>;
-  auto kern = xent_tc_kernel<B_MN, PAIR, FWD>;
-  const int v = (B_MN ? 1 : 0) + (PAIR ? 2 : 0) + (FWD ? 4 : 0), dev = ctx->device;
+  auto kern = xent_tc_kernel<B_MN, PAIR, FWD, CHUNKED>;
+  const int v = (B_MN ? 1 : 0) + (PAIR ? 2 : 0) + (FWD ? 4 : 0) + (CHUNKED ? 8 : 0), dev = ctx->device;
   if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: device index >= 64");
   if (!g_smem_set[v][dev]) {
     const int rc = bwpp_check_cuda(
@@ -473,16 +585,16 @@ int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const
                          FWD ? "xent logits" : "xent dlogit");
 }
 
-template <bool FWD>
+template <bool FWD, bool CHUNKED>
 int launch_any(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
                const XentTile &a, bool vocab_major) {
   if (a.T > (uint32_t)BM) {  // a pair's second CTA would otherwise have rows past T only
-    const int rc = vocab_major ? launch<false, true, FWD>(ctx, tx, tw, to, a)
-                               : launch<true, true, FWD>(ctx, tx, tw, to, a);
+    const int rc = vocab_major ? launch<false, true, FWD, CHUNKED>(ctx, tx, tw, to, a)
+                               : launch<true, true, FWD, CHUNKED>(ctx, tx, tw, to, a);
     if (rc != BWPP_CUDA_ERR_UNSUPPORTED) return rc;
   }
-  return vocab_major ? launch<false, false, FWD>(ctx, tx, tw, to, a)
-                     : launch<true, false, FWD>(ctx, tx, tw, to, a);
+  return vocab_major ? launch<false, false, FWD, CHUNKED>(ctx, tx, tw, to, a)
+                     : launch<true, false, FWD, CHUNKED>(ctx, tx, tw, to, a);
 }
 
 int operand_maps(BwppCudaCtx *ctx, const XentOperands &o, CUtensorMap *tx, CUtensorMap *tw) {
@@ -513,7 +625,8 @@ int bwpp_xent_stats_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_
   a.part = part;
   a.hit = hit;
   a.vocab = o.vocab;
-  return launch_any<true>(ctx, tx, tw, tx, a, o.vocab_major);
+  return o.D > CHUNK * BK ? launch_any<true, true>(ctx, tx, tw, tx, a, o.vocab_major)
+                          : launch_any<true, false>(ctx, tx, tw, tx, a, o.vocab_major);
 }
 
 int bwpp_xent_combine_launch(BwppCudaCtx *ctx, const float2 *part, uint32_t nparts, const float *hit,
@@ -543,5 +656,5 @@ int bwpp_xent_dlogit_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32
   a.lse = lse;
   a.dloss = dloss;
   a.vocab = o.vocab;
-  return launch_any<false>(ctx, tx, tw, to, a, o.vocab_major);
+  return launch_any<false, false>(ctx, tx, tw, to, a, o.vocab_major);
 }
