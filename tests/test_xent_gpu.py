@@ -93,7 +93,9 @@ def check(ctx, T, V, D, vocab_major, scale=1.0, bf16=1, pad=0, seed=0, ones=Fals
 @pytest.mark.parametrize("T,V,D", [(1, 1, 1), (1, 2, 8), (1, 1000, 64), (3, 257, 16), (5, 255, 33), (64, 256, 64),
                                    (127, 1000, 72), (128, 512, 128), (129, 513, 65), (200, 3001, 100),
                                    (257, 770, 256), (300, 5000, 520), (1, 32000, 256), (777, 1009, 101),
-                                   (140, 700, 1096), (33, 1500, 2500), (260, 300, 4096)])
+                                   (140, 700, 1096), (33, 1500, 2500), (260, 300, 4096),
+                                   (2, 333, 40), (2, 1001, 129), (1, 130, 264), (2, 4097, 1000), (2, 600, 7000),
+                                   (1, 50000, 16), (7, 20000, 8), (1, 200, 30000), (2, 90, 50000)])
 def test_sizes(ctx, T, V, D, vocab_major):
     check(ctx, T, V, D, vocab_major, ignored=0.0 if T == 1 else 0.2)
 
