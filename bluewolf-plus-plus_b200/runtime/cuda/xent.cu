@@ -137,16 +137,22 @@ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct Layout {
   uint32_t piece;             // vocabulary columns of a piece
   uint32_t dp;                // D rounded up
-  uint32_t part_rows;         // rows of one K part of dx
-  uint32_t most_parts;        // K parts of dx that scratch has room for
+  // K parts of dx and of dW that scratch has room for, and the rows of one
+  uint32_t dx_rows, dx_parts, dw_rows, dw_parts;
   size_t part, hit, x, w, dlogit, dx, dw, total;
 };
 
-uint32_t clamp_piece(uint64_t c, uint32_t V) {
-  c &= ~255ull;
+// Equal pieces of about c columns, whole 256s, at least 1024.
+uint32_t piece_of(uint64_t c, uint32_t V) {
   if (c < 1024) c = 1024;
-  const uint64_t all = ((uint64_t)V + 255) & ~255ull;
-  return (uint32_t)(c < all ? c : all);
+  const uint64_t pieces = (V + c - 1) / c;
+  return (uint32_t)((((uint64_t)V + pieces - 1) / pieces + 255) & ~255ull);
+}
+
+// K parts of a [rows, ld] product that fit 64 MB, at most eight.
+uint32_t parts_that_fit(uint64_t rows, uint64_t ld) {
+  const uint64_t fit = (64ull << 20) / (rows * ld * 4);
+  return fit < 1 ? 1 : fit > 8 ? 8 : (uint32_t)fit;
 }
 
 // Vocabulary columns of a piece.  Backward: about 2^27 dlogit at a time (T 8192,
@@ -158,12 +164,12 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
                  bool stage_dw) {
   Layout l{};
   l.dp = up8(p.D);
-  l.piece = backward ? clamp_piece((1ull << 27) / p.T, p.V)
-                     : clamp_piece(pack_w ? (1ull << 25) / l.dp : (uint64_t)p.V + 255, p.V);
-  l.part_rows = (p.T + 255) & ~255u;
-  // parts of dx only where they take little memory (and few tiles need them)
-  const uint64_t fit = (64ull << 20) / ((uint64_t)l.part_rows * l.dp * 4);
-  l.most_parts = fit < 1 ? 1 : fit > 8 ? 8 : (uint32_t)fit;
+  l.piece = backward ? piece_of((1ull << 27) / p.T, p.V)
+                     : piece_of(pack_w ? (1ull << 25) / l.dp : (uint64_t)p.V, p.V);
+  l.dx_rows = (uint32_t)up256(p.T);
+  l.dx_parts = parts_that_fit(l.dx_rows, l.dp);
+  l.dw_rows = (uint32_t)up256(p.w_vocab_major ? l.piece : p.D);
+  l.dw_parts = parts_that_fit(l.dw_rows, p.w_vocab_major ? l.dp : l.piece);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -178,8 +184,10 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
     l.hit = take((size_t)p.T * 4);
   } else {
     l.dlogit = take((size_t)p.T * l.piece * 2);
-    if (stage_dx) l.dx = take((size_t)l.most_parts * l.part_rows * l.dp * 4);
-    if (stage_dw) l.dw = take((size_t)l.piece * l.dp * es);
+    if (stage_dx) l.dx = take((size_t)l.dx_parts * l.dx_rows * l.dp * 4);
+    if (stage_dw || l.dw_parts > 1)
+      l.dw = take((size_t)l.dw_parts * l.dw_rows * (p.w_vocab_major ? l.dp : l.piece) *
+                  (l.dw_parts > 1 ? 4 : es));
   }
   l.total = at;
   return l;
@@ -298,7 +306,7 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     px.ldb = ld_w;
     px.b_mn = vm;  // W's rows are K here
     px.ldc = px.ld_add = probe.dp;
-    px.part_rows = probe.part_rows;
+    px.part_rows = probe.dx_rows;
     pw = XentProduct{};
     pw.M = vm ? n : p.D;
     pw.N = vm ? p.D : n;
@@ -306,19 +314,18 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     pw.lda = vm ? piece : probe.dp;
     pw.ldb = vm ? probe.dp : piece;
     pw.a_mn = pw.b_mn = true;
-    pw.ldc = stage_dw ? (vm ? probe.dp : piece) : p.lddw;
-    pw.bf16 = p.grads_bf16 != 0;
+    pw.part_rows = probe.dw_rows;
   };
   XentProduct px, pw;
   products(piece < p.V ? piece : p.V, px, pw);
-  uint32_t parts = 1;
-  if (dx) {  // the same whether dW is wanted or not, so that dx is the same too
-    rc = bwpp_xent_dx_parts(ctx, px, pw, probe.most_parts, &parts);
-    if (rc) return rc;
-  }
+  // K parts, the same whether both gradients are wanted or one, so that each
+  // comes out the same
+  uint32_t dx_parts, dw_parts;
+  rc = bwpp_xent_parts(ctx, px, pw, probe.dx_parts, probe.dw_parts, &dx_parts, &dw_parts);
+  if (rc) return rc;
   // dx is summed in scratch, unless the caller's rows take it: all of it in one
   // piece, or fp32 sums
-  const bool direct = dx_out && parts == 1 && (pieces == 1 || !p.grads_bf16);
+  const bool direct = dx_out && dx_parts == 1 && (pieces == 1 || !p.grads_bf16);
   const Layout l = layout_of(p, true, pack_w, true, dx && !direct, stage_dw);
   uint8_t *scratch;
   rc = bwpp_op_scratch(ctx, l.total, "xent bwd", &scratch);
@@ -341,27 +348,33 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     px.b = w1.w;
     px.accumulate = v0 > 0;
     // the last piece leaves the sum in the caller's rows where it can
-    const bool to_user = direct || (dx_out && parts == 1 && last);
+    const bool to_user = direct || (dx_out && dx_parts == 1 && last);
     px.add = direct ? dx : static_cast<void *>(scratch + l.dx);
     px.ld_add = direct ? p.lddx : l.dp;
     px.c = to_user ? dx : static_cast<void *>(scratch + l.dx);
     px.ldc = to_user ? p.lddx : l.dp;
     px.bf16 = to_user && p.grads_bf16;
-    uint8_t *user_w = static_cast<uint8_t *>(dw) + (vm ? (size_t)v0 * p.lddw : (size_t)v0) * es;
+    uint8_t *user_w =
+        dw ? static_cast<uint8_t *>(dw) + (vm ? (size_t)v0 * p.lddw : (size_t)v0) * es : nullptr;
+    const bool own_w = stage_dw || dw_parts > 1;  // dW's part goes through scratch
     pw.a = vm ? dlogit : xp;
     pw.b = vm ? xp : dlogit;
-    pw.c = stage_dw ? static_cast<void *>(scratch + l.dw) : static_cast<void *>(user_w);
-    rc = bwpp_xent_grad_launch(ctx, dx ? &px : nullptr, dw ? &pw : nullptr, parts);
-    if (rc) return rc;
-    if (stage_dw) {
+    pw.c = own_w ? static_cast<void *>(scratch + l.dw) : static_cast<void *>(user_w);
+    pw.ldc = own_w ? (vm ? l.dp : piece) : p.lddw;
+    pw.bf16 = p.grads_bf16 && dw_parts == 1;
+    rc = bwpp_xent_grad_launch(ctx, dx ? &px : nullptr, dw ? &pw : nullptr, dx_parts, dw_parts);
+    if (!rc && dw && dw_parts > 1)
+      rc = bwpp_xent_sum_parts_launch(ctx, static_cast<const float *>(pw.c), dw_parts,
+                                      (size_t)l.dw_rows * pw.ldc, user_w, pw.M, pw.N, pw.ldc, p.lddw,
+                                      p.grads_bf16);
+    else if (!rc && stage_dw)
       rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw)
                         : unpack_rows<float>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw);
-      if (rc) return rc;
-    }
+    if (rc) return rc;
   }
-  if (dx && !direct && !(dx_out && parts == 1))
-    return bwpp_xent_sum_parts_launch(ctx, reinterpret_cast<const float *>(scratch + l.dx), parts,
-                                      (size_t)l.part_rows * l.dp, dx, p.T, p.D, l.dp, p.lddx,
+  if (dx && !direct && !(dx_out && dx_parts == 1))
+    return bwpp_xent_sum_parts_launch(ctx, reinterpret_cast<const float *>(scratch + l.dx), dx_parts,
+                                      (size_t)l.dx_rows * l.dp, dx, p.T, p.D, l.dp, p.lddx,
                                       p.grads_bf16);
   return BWPP_CUDA_OK;
 }

@@ -43,12 +43,13 @@ struct XentProduct {
                       // rounded up to 256
 };
 
-// K parts of dx, at most `most`, that a launch of both would best have.
-int bwpp_xent_dx_parts(BwppCudaCtx *ctx, const XentProduct &dx, const XentProduct &dw, uint32_t most,
-                       uint32_t *parts);
+// K parts of dx and dw, at most `most_dx` and `most_dw`, that a launch of both
+// would best have.
+int bwpp_xent_parts(BwppCudaCtx *ctx, const XentProduct &dx, const XentProduct &dw, uint32_t most_dx,
+                    uint32_t most_dw, uint32_t *dx_parts, uint32_t *dw_parts);
 // Either may be NULL.
 int bwpp_xent_grad_launch(BwppCudaCtx *ctx, const XentProduct *dx, const XentProduct *dw,
-                          uint32_t parts);
+                          uint32_t dx_parts, uint32_t dw_parts);
 // out [rows, ld_out] = the sum over parts, in order, of part + s * part_stride.
 int bwpp_xent_sum_parts_launch(BwppCudaCtx *ctx, const float *part, uint32_t parts,
                                size_t part_stride, void *out, uint32_t rows, uint32_t cols,

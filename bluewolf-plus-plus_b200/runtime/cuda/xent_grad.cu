@@ -8,7 +8,7 @@
 // (T 8192, V 32000, D 2048, a piece of 16384: 774 us, 1.42 PFLOP/s.  Half the
 // workers on each product balance as well, but the tiles that run together then
 // share less in L2: 830 us.)
-// A dx whose few tiles have a long K is cut into K parts, each summed on its
+// A product of few tiles with a long K is cut into K parts, each summed on its
 // own in fp32; a last kernel adds the parts in order, so the result does not
 // depend on which part ends first.
 //
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// dx from its K parts, added in order, into rows of any pitch.  A warp takes
+// A product from its K parts, added in order, into rows of any pitch.  A warp takes
 // 256 columns of a row.
 __global__ void __launch_bounds__(256)
     xent_sum_parts_kernel(const float *__restrict__ part, uint32_t parts, size_t part_stride,
@@ -392,17 +392,23 @@ __global__ void __launch_bounds__(256)
   const uint32_t i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
   if (i >= rows * spans) return;
   const uint32_t r = i / spans, c0 = (i - r * spans) * 256 + lane;
+  float v[8];
+#pragma unroll
+  for (uint32_t k = 0; k < 8; ++k) v[k] = 0.0f;
+  for (uint32_t s = 0; s < parts; ++s) {
+    const float *p = part + s * part_stride + r * ld;
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k)
+      if (c0 + k * 32 < cols) v[k] += __ldg(p + c0 + k * 32);
+  }
 #pragma unroll
   for (uint32_t k = 0; k < 8; ++k) {
     const uint32_t c = c0 + k * 32;
     if (c >= cols) break;
-    const float *p = part + r * ld + c;
-    float v = __ldg(p);
-    for (uint32_t s = 1; s < parts; ++s) v += __ldg(p + s * part_stride);
     if (bf16)
-      static_cast<uint16_t *>(out)[r * ld_out + c] = (uint16_t)(pack2_16<false>(v, 0.0f) & 0xFFFFu);
+      static_cast<uint16_t *>(out)[r * ld_out + c] = (uint16_t)(pack2_16<false>(v[k], 0.0f) & 0xFFFFu);
     else
-      static_cast<float *>(out)[r * ld_out + c] = v;
+      static_cast<float *>(out)[r * ld_out + c] = v[k];
   }
 }
 
@@ -503,8 +509,8 @@ uint32_t tile_time(uint32_t num_kb, uint32_t parts) { return ceil_div(num_kb, pa
 
 }  // namespace
 
-int bwpp_xent_dx_parts(BwppCudaCtx *ctx, const XentProduct &dx, const XentProduct &dw, uint32_t most,
-                       uint32_t *parts) {
+int bwpp_xent_parts(BwppCudaCtx *ctx, const XentProduct &dx, const XentProduct &dw, uint32_t most_dx,
+                    uint32_t most_dw, uint32_t *dx_parts, uint32_t *dw_parts) {
   int pairs;
   const int rc = resident_pairs(ctx, &pairs);
   if (rc) return rc;
@@ -512,43 +518,46 @@ int bwpp_xent_dx_parts(BwppCudaCtx *ctx, const XentProduct &dx, const XentProduc
   const uint32_t tile_m = pairs > 0 ? 2 * BM : BM;
   const uint64_t tx = (uint64_t)ceil_div(dx.M, tile_m) * ceil_div(dx.N, BN);
   const uint64_t tw = (uint64_t)ceil_div(dw.M, tile_m) * ceil_div(dw.N, BN);
-  const uint32_t kx = ceil_div(dx.K, BK), cw = tile_time(ceil_div(dw.K, BK), 1);
+  const uint32_t kx = ceil_div(dx.K, BK), kw = ceil_div(dw.K, BK);
   uint64_t best = ~0ull;
-  *parts = 1;
-  for (uint32_t s = 1; s <= most && s <= kx; ++s) {
-    const uint64_t items = tx * s, late = items % cap, cx = tile_time(kx, s);
-    const uint64_t ahead = late ? cx / cw * (cap - late) : 0;
-    uint64_t t = (items + cap - 1) / cap * cx;
-    if (tw > ahead) t += (tw - ahead + cap - 1) / cap * cw;
-    t *= s > 1 ? 9 : 8;  // the parts' sums are written and read once more: worth an eighth
-    if (t < best) {
-      best = t;
-      *parts = s;
+  *dx_parts = *dw_parts = 1;
+  for (uint32_t s = 1; s <= most_dx && s <= kx; ++s)
+    for (uint32_t q = 1; q <= most_dw && q <= kw; ++q) {
+      const uint64_t late = tx * s % cap, cx = tile_time(kx, s), cw = tile_time(kw, q);
+      const uint64_t ahead = late ? cx / cw * (cap - late) : 0;
+      uint64_t t = (tx * s + cap - 1) / cap * cx;
+      if (tw * q > ahead) t += (tw * q - ahead + cap - 1) / cap * cw;
+      // parts' sums are written and read once more: worth an eighth of the time
+      t = t * (8 + (s > 1) + (q > 1));
+      if (t < best) {
+        best = t;
+        *dx_parts = s;
+        *dw_parts = q;
+      }
     }
-  }
   return BWPP_CUDA_OK;
 }
 
 int bwpp_xent_grad_launch(BwppCudaCtx *ctx, const XentProduct *dx, const XentProduct *dw,
-                          uint32_t parts) {
+                          uint32_t dx_parts, uint32_t dw_parts) {
   int pairs;
   int rc = resident_pairs(ctx, &pairs);
   if (rc) return rc;
   const uint32_t cap = pairs > 0 ? (uint32_t)pairs : (uint32_t)ctx->num_sms;
   const uint32_t tile_m = pairs > 0 ? 2 * BM : BM;
   // a last, short piece may have fewer K blocks than parts
-  if (dx && parts > ceil_div(dx->K, BK)) parts = ceil_div(dx->K, BK);
+  if (dx && dx_parts > ceil_div(dx->K, BK)) dx_parts = ceil_div(dx->K, BK);
   Work work{};
   Product &p0 = work.product[0], &p1 = work.product[1];
-  if (dx) rc = make_product(ctx, *dx, tile_m, parts, work.maps[0], p0);
-  if (!rc && dw) rc = make_product(ctx, *dw, tile_m, 1, work.maps[1], p1);
+  if (dx) rc = make_product(ctx, *dx, tile_m, dx_parts, work.maps[0], p0);
+  if (!rc && dw) rc = make_product(ctx, *dw, tile_m, dw_parts, work.maps[1], p1);
   if (rc) return rc;
   const uint64_t items = (uint64_t)p0.items + p1.items;
   const uint32_t n = items < cap ? (uint32_t)items : cap;
   work.workers = n;
   work.late = p0.items % n;
   if (work.late && dw)
-    work.ahead = tile_time(p0.num_kb, p0.parts) / tile_time(p1.num_kb, 1);
+    work.ahead = tile_time(p0.num_kb, p0.parts) / tile_time(p1.num_kb, p1.parts);
   if (dx) p0.group = group_of(p0, n);
   if (dw) p1.group = group_of(p1, n);
   cudaLaunchAttribute attr[1];

@@ -95,7 +95,8 @@ def check(ctx, T, V, D, vocab_major, scale=1.0, bf16=1, pad=0, seed=0, ones=Fals
                                    (257, 770, 256), (300, 5000, 520), (1, 32000, 256), (777, 1009, 101),
                                    (140, 700, 1096), (33, 1500, 2500), (260, 300, 4096),
                                    (2, 333, 40), (2, 1001, 129), (1, 130, 264), (2, 4097, 1000), (2, 600, 7000),
-                                   (1, 50000, 16), (7, 20000, 8), (1, 200, 30000), (2, 90, 50000)])
+                                   (1, 50000, 16), (7, 20000, 8), (1, 200, 30000), (2, 90, 50000),
+                                   (5000, 300, 40), (4001, 700, 136), (2100, 64, 520)])
 def test_sizes(ctx, T, V, D, vocab_major):
     check(ctx, T, V, D, vocab_major, ignored=0.0 if T == 1 else 0.2)
 
