@@ -987,6 +987,8 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
   const bool sum_post = dgain_post || (dgate && !per_row);
   const bool sums = sum_post || dgain_pre;
   if (sums) {
+    if ((a.p.cols - 1) / 32 >= 65535)  // blocks of 32 columns in a grid's second dimension
+      return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: row too wide");
     uint8_t *scratch;
     const size_t part = (size_t)k.chunks * a.p.cols;
     rc = bwpp_op_scratch(ctx, 2 * part * sizeof(float), "junction bwd", &scratch);
@@ -1012,8 +1014,6 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
     q.ldgate = a.p.ldgate;
     q.weighted = gate && !per_row;
     const dim3 grid(2 + (q.dgate ? k.groups : 0), (a.p.cols + 31) / 32);
-    if (grid.y > 65535)
-      return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: row too wide");
     junction_sums_kernel<<<grid, 32 * kSumWarps, 0, s>>>(q);
     BWPP_LAUNCH_CHECK(ctx, "junction sums");
   }

@@ -101,6 +101,20 @@ __device__ __forceinline__ void fold_logits(uint64_t (&t)[P], float &m, float &s
   m = top;
 }
 
+// Columns from `end` on drop out.
+template <int P>
+__device__ __forceinline__ void mask_logits(uint64_t (&t)[P], uint32_t col, uint32_t end) {
+  if (col + 2 * P <= end) return;
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    float x, y;
+    f2unpack(t[j], x, y);
+    if (col + 2 * j >= end) x = -INFINITY;
+    if (col + 2 * j + 1 >= end) y = -INFINITY;
+    t[j] = f2pack(x, y);
+  }
+}
+
 // Tiles go down the row blocks of a group, then to the next 256 columns.
 __device__ __forceinline__ void tile_at(uint32_t i, uint32_t group, uint32_t tiles_m,
                                         uint32_t tiles_n, uint32_t &mb, uint32_t &nb) {
@@ -366,16 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint64_t c2 = f2pack(a.c, a.c);
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = f2mul(v[j], c2);
-          if (first + 128 > end) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              float x, y;
-              f2unpack(v[j], x, y);
-              if (first + 2 * j >= end) x = -INFINITY;
-              if (first + 2 * j + 1 >= end) y = -INFINITY;
-              v[j] = f2pack(x, y);
-            }
-          }
+          mask_logits(v, first, end);
           float m = -INFINITY, s = 0.0f;
           fold_logits(v, m, s);
           if (live_row)
@@ -406,17 +411,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (hit_col - k * 32 == (uint32_t)j) h = __uint_as_float(r[j]);
               a.hit[row] = h * a.scale;
             }
-            if (cs + 32 > end) {
-              // below any logit, whatever the sign of the scale
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (cs + j >= end) r[j] = __float_as_uint(a.c < 0 ? INFINITY : -INFINITY);
-            }
             const uint64_t c2 = f2pack(a.c, a.c);
             uint64_t v[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
               v[j] = f2mul(f2pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2);
+            mask_logits(v, cs, end);
             fold_logits(v, m, s);
           }
           if (live_row) a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);

@@ -338,7 +338,9 @@ int bwpp_cuda_cast_f32_bf16(BwppCudaCtx *ctx, const float *src, uint16_t *dst,
  * captured graph keeps the scratch's address, so a call that needs scratch
  * and is made while the ctx's stream is capturing needs a caller's workspace
  * (BWPP_CUDA_ERR_UNSUPPORTED without one); graphs that share a workspace must
- * not run at the same time. */
+ * not run at the same time.  All calls of a ctx share its scratch: after
+ * bwpp_cuda_ctx_set_stream, work of the stream before has to be done, or the
+ * new stream has to wait for it. */
 
 /* Softmax cross entropy over a vocabulary of V, from hidden states x [T, ldx]
  * and the vocabulary weight, without keeping the T x V logits:

@@ -265,6 +265,9 @@ def test_zero_rows_and_refusals(ctx):
     refused(b, None, z, None, None, None, z, z, z, None, None, None, None, 4, 16)
     refused(b, z, z, None, None, None, z, z, z, None, None, z, None, 4, 16)  # dgate without a gate
     refused(b, z, z, None, None, None, z, z, z, None, g, None, None, 4, 16, norm_after=0)
+    with pytest.raises(bwpp.BwppError) as e:  # 32 columns a block, 65535 blocks
+        b(z, z, None, None, None, None, z, None, None, None, None, g, 1, 32 * 65535 + 1)
+    assert e.value.status == bwpp.ERR_UNSUPPORTED
 
 
 def test_zero_rows_of_b_and_eps_zero(ctx):

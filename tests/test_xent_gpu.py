@@ -102,7 +102,7 @@ def test_sizes(ctx, T, V, D, vocab_major):
 
 
 @pytest.mark.parametrize("vocab_major", [0, 1])
-@pytest.mark.parametrize("kw", [dict(scale=0.125), dict(scale=-3.0), dict(bf16=0), dict(pad=8), dict(pad=3),
+@pytest.mark.parametrize("kw", [dict(scale=0.125), dict(scale=0.0), dict(scale=-3.0), dict(bf16=0), dict(pad=8), dict(pad=3),
                                 dict(pad=3, bf16=0), dict(ones=True), dict(sharp=30.0), dict(ignored=1.0)])
 def test_options(ctx, vocab_major, kw):
     check(ctx, 150, 1111, 136, vocab_major, **kw)
