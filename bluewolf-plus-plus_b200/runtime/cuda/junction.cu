@@ -54,11 +54,11 @@ struct JunctionArgs {
 // Sums NV values over the TPR threads of a row.
 template <int TPR, int NV>
 __device__ __forceinline__ void row_sum(float (&v)[NV], float *red) {
-  if constexpr (TPR == 32) {
+  if constexpr (TPR <= 32) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+      for (int o = TPR / 2; o > 0; o >>= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
   } else {
     block_sum<NV>(v, red);
   }
@@ -81,7 +81,8 @@ __device__ __forceinline__ void load_gain(const float *g, uint32_t c, float (&o)
   }
 }
 
-constexpr int block_threads(int tpr) { return tpr == 32 ? 128 : tpr; }
+// Rows of up to 32 threads share a block of 128.
+constexpr int block_threads(int tpr) { return tpr <= 32 ? 128 : tpr; }
 
 // ---- forward -----------------------------------------------------------------
 
@@ -92,8 +93,9 @@ __global__ void __launch_bounds__(block_threads(TPR))
   using T = typename Elem<DT>::type;
   __shared__ float red[32];
   const BwppCudaJunctionParams &p = a.p;
-  const uint32_t r = blockIdx.x * (block_threads(TPR) / TPR) + threadIdx.x / TPR;
-  if (r >= p.rows) return;  // a whole warp (TPR 32), or none
+  const uint32_t at = blockIdx.x * (block_threads(TPR) / TPR) + threadIdx.x / TPR;
+  const bool live = at < p.rows;  // threads past the last row go along with it
+  const uint32_t r = live ? at : p.rows - 1;
   const uint32_t t = threadIdx.x % TPR;
   const float *h = a.h + (size_t)r * p.ldh;
   const T *b = static_cast<const T *>(a.b) + (size_t)r * p.ldb;
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(block_threads(TPR))
       ss[0] += v[e] * v[e];
     }
     hv[i].set(v);
-    hv[i].store(a.h_out + (size_t)r * p.ldh + c);
+    if (live) hv[i].store(a.h_out + (size_t)r * p.ldh + c);
   }
   if (!a.y) return;
   row_sum<TPR, 1>(ss, red);
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(block_threads(TPR))
     for (int e = 0; e < VEC; ++e) v[e] = hv[i].get(e) * rh * gq[e];
     Raw<DT, VEC> o;
     o.set(v);
-    o.store(static_cast<T *>(a.y) + (size_t)r * p.ldy + c);
+    if (live) o.store(static_cast<T *>(a.y) + (size_t)r * p.ldy + c);
   }
 }
 
@@ -221,7 +223,8 @@ __device__ __forceinline__ void row_sum_once(float (&v)[NV], float (*red)[32]) {
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
+      v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
   if constexpr (TPR > 32) {
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
@@ -290,7 +293,9 @@ __global__ void __launch_bounds__(block_threads(TPR))
     }
   };
   fetch(first + sub);
-  for (uint32_t r = first + sub; r < last; r += RPB) {
+  for (uint32_t r0 = first; r0 < last; r0 += RPB) {
+    const uint32_t r = r0 + sub;
+    const bool live = r < last;  // the others go along: their rows read as zero
     Raw<F32, VEC> hv[NV], dv[NV];
     Raw<DT, VEC> bv[NV], yv[NV];
 #pragma unroll
@@ -315,12 +320,12 @@ __global__ void __launch_bounds__(block_threads(TPR))
     const float rh = a.dy ? 1.0f / sqrtf(s[0] * inv_c + p.eps_pre) : 0.0f;
     const float m2 = rh * s[1] * inv_c;  // mean(g hat)
     const float rb = p.norm_after ? 1.0f / sqrtf(s[2] * inv_c + p.eps_post) : 1.0f;
-    const float *gate = token ? a.gate + (size_t)r * p.ldgate : nullptr;
+    const float *gate = token && live ? a.gate + (size_t)r * p.ldgate : nullptr;
     float m[1] = {0.0f};  // sum gain_post du bhat
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * TPR) * VEC;
-      if (c >= p.cols) continue;
+      if (c >= p.cols || !live) continue;
       float gt[VEC], w[VEC], dg[VEC], gu[VEC];
       load_gain<VEC>(gate, c, gt);
 #pragma unroll
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(block_threads(TPR))
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint32_t c = (t + i * TPR) * VEC;
-      if (c >= p.cols) continue;
+      if (c >= p.cols || !live) continue;
       float w[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) w[e] = rb * (dv[i].get(e) - bv[i].get(e) * rb * m1);
@@ -757,7 +762,7 @@ struct Chunks {
 // A chunk holds consecutive rows of one group (rows that share a gate row and
 // whose dgate is summed), about `per_sm` chunks per SM (at most kMaxPerSm,
 // which the scratch is sized for).
-constexpr uint32_t kMaxPerSm = 8;
+constexpr uint32_t kMaxPerSm = 12;
 bool make_chunks(BwppCudaCtx *ctx, uint32_t rows, uint32_t gate_rows, uint32_t per_sm, Chunks &k) {
   k.group_rows = gate_rows <= 1 || gate_rows > rows ? rows : gate_rows;
   k.groups = (uint32_t)(((uint64_t)rows + k.group_rows - 1) / k.group_rows);
@@ -807,7 +812,9 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
       <<<(a.p.rows + block_threads(TPR) / TPR - 1) / (block_threads(TPR) / TPR),           \
          block_threads(TPR), 0, s>>>(a)
   if (vectors<DT>(a)) {
-    if (cols <= 256) BWPP_FWD(8, 1, 32);
+    if (cols <= 64) BWPP_FWD(8, 1, 8);
+    else if (cols <= 128) BWPP_FWD(8, 1, 16);
+    else if (cols <= 256) BWPP_FWD(8, 1, 32);
     else if (cols <= 512) BWPP_FWD(8, 2, 32);
     else if (cols <= 1024 && many) BWPP_FWD(8, 2, 64);
     else if (cols <= 1024) BWPP_FWD(8, 1, 128);
@@ -815,13 +822,19 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
     else if (cols <= 2048) BWPP_FWD(8, 1, 256);
     else if (cols <= 4096 && many) BWPP_FWD(8, 4, 128);
     else if (cols <= 4096) BWPP_FWD(8, 2, 256);
+    else if (cols <= 6144 && many) BWPP_FWD(8, 3, 256);
     else if (cols <= 8192 && many) BWPP_FWD(8, 4, 256);
     else if (cols <= 8192) BWPP_FWD(8, 2, 512);
+    else if (cols <= 12288) BWPP_FWD(8, 3, 512);
     else if (cols <= 16384) BWPP_FWD(8, 4, 512);
     else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
   } else {
-    if (cols <= 128) BWPP_FWD(1, 4, 32);
+    if (cols <= 64) BWPP_FWD(1, 8, 8);
+    else if (cols <= 128) BWPP_FWD(1, 8, 16);
+    else if (cols <= 256) BWPP_FWD(1, 8, 32);
+    else if (cols <= 512) BWPP_FWD(1, 8, 64);
     else if (cols <= 1024) BWPP_FWD(1, 8, 128);
+    else if (cols <= 2048) BWPP_FWD(1, 8, 256);
     else if (cols <= 4096) BWPP_FWD(1, 8, 512);
     else if (cols <= 16384) BWPP_FWD(1, 16, 1024);
     else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
@@ -839,16 +852,21 @@ template <int DT>
 Plan plan_bwd(const JunctionArgs &a) {
   const uint32_t cols = a.p.cols;
   const bool vec = vectors<DT>(a);
-  const Plan held{0, vec && cols <= 256 ? 4u : cols <= 128 ? 6u : cols <= 1024 ? 3u : cols <= 4096 ? 1u : 2u, 0};
+  // threads of a block: 128 (VEC 8, or up to 128 columns), then a fourth of the
+  // columns up to 512; about 80 registers a thread, 128 in the widest
+  const uint32_t per = vec && cols <= 256 ? 4 : cols <= 128 ? 6 : cols <= 256 ? 12 : cols <= 512 ? 6
+                       : cols <= 1024 ? 3 : cols <= 4096 ? 1 : 2;
+  const Plan held{0, per, 0};
   if (!vec || cols <= 256 || cols > 8192) return held;
   Plan g{0, 0, 0};
   const bool token = a.p.gate_rows == 1 && a.gate;
   const uint32_t row = cols * (8 + (token ? 4 : 0) + 2 * (uint32_t)sizeof(typename Elem<DT>::type));
   constexpr uint32_t sm = 220 * 1024;  // of an SM's 228 KB; 1 KB and the static part go with each CTA
   // 16 warps per SM hide a row's two reductions (32768 x 2048 bf16: 323 us with
-  // one CTA of 8 warps, 205 with two, 218 with three, 227 with four); two or
-  // more stages make no difference then
-  const uint32_t want = cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1;
+  // one CTA of 8 warps, 205 with two, 218 with three, 227 with four; 8192 x 2560
+  // bf16: 115 us with one CTA of 16 warps, 77 with two of 8); two or more stages
+  // make no difference then
+  const uint32_t want = cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 4096 ? 2 : 1;
   for (uint32_t per = want; per >= 1 && g.stages < 2; --per) {
     g.per_sm = per;
     g.stages = sm / per / row;
@@ -884,7 +902,7 @@ int launch_staged_any(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, 
   if (cols <= 512) return launch_staged<DT, 2, 64, TOKEN>(ctx, a, chunks, g, 0);
   if (cols <= 1024) return launch_staged<DT, 2, 128, TOKEN>(ctx, a, chunks, g, 1);
   if (cols <= 2048) return launch_staged<DT, 2, 256, TOKEN>(ctx, a, chunks, g, 2);
-  if (cols <= 4096) return launch_staged<DT, 2, 512, TOKEN>(ctx, a, chunks, g, 3);
+  if (cols <= 4096) return launch_staged<DT, 4, 256, TOKEN>(ctx, a, chunks, g, 3);
   return launch_staged<DT, 4, 512, TOKEN>(ctx, a, chunks, g, 4);
 }
 
@@ -898,10 +916,16 @@ int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const P
 #define BWPP_BWD(VEC, NV, TPR) \
   junction_bwd_kernel<DT, VEC, NV, TPR><<<chunks, block_threads(TPR), 0, s>>>(a)
   if (vectors<DT>(a) && cols <= 256) {
-    BWPP_BWD(8, 1, 32);
+    if (cols <= 64) BWPP_BWD(8, 1, 8);
+    else if (cols <= 128) BWPP_BWD(8, 1, 16);
+    else BWPP_BWD(8, 1, 32);
   } else {
-    if (cols <= 128) BWPP_BWD(1, 4, 32);
+    if (cols <= 64) BWPP_BWD(1, 4, 16);
+    else if (cols <= 128) BWPP_BWD(1, 4, 32);
+    else if (cols <= 256) BWPP_BWD(1, 4, 64);
+    else if (cols <= 512) BWPP_BWD(1, 4, 128);
     else if (cols <= 1024) BWPP_BWD(1, 4, 256);
+    else if (cols <= 2048) BWPP_BWD(1, 4, 512);
     else if (cols <= 4096) BWPP_BWD(1, 8, 512);
     else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
   }
