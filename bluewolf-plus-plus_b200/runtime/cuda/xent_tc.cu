@@ -608,7 +608,8 @@ int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const
   // in L2 (T 8192, V 32000, D 2048 over seconds: 1277 TFLOP/s with groups of 8
   // blocks, 1305 with 16, 1343 with all 32)
   const uint64_t block = (uint64_t)C::TILE_M * a.D * 2, fit = (32ull << 20) / block;
-  b.group = fit < 8 ? 8u : fit > 4096 ? 4096u : (uint32_t)fit;
+  const uint64_t blocks = ((uint64_t)a.T + C::TILE_M - 1) / C::TILE_M;
+  b.group = (uint32_t)(fit < 8 ? 8 : fit > blocks ? blocks : fit);
   const uint32_t n = b.items < cap ? b.items : cap;
   cfg.gridDim = dim3((PAIR ? 2 : 1) * n, 1, 1);
   int *status = ctx->status_word;

@@ -100,3 +100,20 @@ def test_struct_layouts():
     assert C.sizeof(bwpp.RopeTable) == 8 + 8 * bwpp.ROPE_MAX_PAIRS
     assert C.sizeof(bwpp.RopeParams) == 56
     assert C.sizeof(bwpp.JunctionParams) == 48
+
+
+def test_packed_parameters_are_the_structs():
+    xent = bwpp.XentParams.from_buffer_copy(bwpp._XENT.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 0.5))
+    assert [getattr(xent, n) for n, _ in xent._fields_] == [1, 2, 3, 4, 5, 6, 7, 8, 9, 0.5]
+    rope = bwpp.RopeParams.from_buffer_copy(bwpp._ROPE.pack(*range(1, 10), -3, 11, 12, 13, 14))
+    assert [getattr(rope, n) for n, _ in rope._fields_] == [*range(1, 10), -3, 11, 12, 13, 14]
+    junction = bwpp.JunctionParams.from_buffer_copy(bwpp._JUNCTION.pack(*range(1, 9), 0.5, 1.5, 2.5, 3.5))
+    assert [getattr(junction, n) for n, _ in junction._fields_] == [*range(1, 9), 0.5, 1.5, 2.5, 3.5]
+
+
+def test_sizes_that_do_not_fit_their_field_are_errors():
+    """2^32 rows would read as none."""
+    with pytest.raises(Exception):
+        bwpp._JUNCTION.pack(1 << 32, *range(7), 1.0, 1.0, 0.0, 0.0)
+    with pytest.raises(Exception):
+        bwpp._ROPE.pack(*range(9), 1 << 31, 0, 0, 0, 0)

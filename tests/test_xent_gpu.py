@@ -281,10 +281,11 @@ def test_rows_past_32_bits(ctx):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
-def test_captured_and_replayed(ctx):
+@pytest.mark.parametrize("T", [1, 30, 400])
+def test_captured_and_replayed(ctx, T):
     """Forward and gradient in one graph with a caller's workspace, replayed on
     new inputs; without a workspace the capture is refused."""
-    T, V, D = 400, 2100, 128
+    V, D = 2100, 128
     stream = torch.cuda.Stream()
     c = bwpp.Ctx(0, stream.cuda_stream)
     x, w, target, dloss, xs, ws = make(T, V, D, 0, 15)
