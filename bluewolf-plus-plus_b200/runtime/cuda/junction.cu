@@ -72,12 +72,12 @@ __device__ __forceinline__ void load_gain(const float *g, uint32_t c, float (&o)
   } else if constexpr (VEC >= 4) {
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
-      const float4 t = __ldg(reinterpret_cast<const float4 *>(g + c) + i);
+      const float4 t = *(reinterpret_cast<const float4 *>(g + c) + i);
       o[4 * i] = t.x; o[4 * i + 1] = t.y; o[4 * i + 2] = t.z; o[4 * i + 3] = t.w;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = __ldg(g + c + e);
+    for (int e = 0; e < VEC; ++e) o[e] = g[c + e];
   }
 }
 
@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(block_threads(TPR))
     junction_fwd_kernel(const __grid_constant__ JunctionArgs a) {
   using T = typename Elem<DT>::type;
   __shared__ float red[32];
+  dependent_wait();
   const BwppCudaJunctionParams &p = a.p;
   const uint32_t at = blockIdx.x * (block_threads(TPR) / TPR) + threadIdx.x / TPR;
   const bool live = at < p.rows;  // threads past the last row go along with it
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(kLoopThreads)
     junction_fwd_looped_kernel(const __grid_constant__ JunctionArgs a) {
   using T = typename Elem<DT>::type;
   __shared__ float red[32];
+  dependent_wait();
   const BwppCudaJunctionParams &p = a.p;
   const uint32_t r = blockIdx.x;
   const float *h = a.h + (size_t)r * p.ldh;
@@ -248,6 +250,7 @@ __global__ void __launch_bounds__(block_threads(TPR))
   using T = typename Elem<DT>::type;
   constexpr int RPB = block_threads(TPR) / TPR;  // rows that a block works on together
   __shared__ float red[3][32], red1[1][32];
+  dependent_wait();
   const BwppCudaJunctionParams &p = a.p;
   const uint32_t t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   uint32_t first, last;
@@ -436,6 +439,7 @@ __global__ void __launch_bounds__(TPR)
     fence_mbar_init();
   }
   __syncthreads();
+  dependent_wait();
   auto fetch = [&](uint32_t r, uint32_t s) {  // one thread
     uint8_t *to = ring + s * stage_bytes;
     mbar_arrive_expect_tx(&full[s], (a.dy ? wide + narrow : 0) + (a.dh_out ? wide : 0) +
@@ -602,6 +606,7 @@ __global__ void __launch_bounds__(kLoopThreads)
     junction_bwd_looped_kernel(const __grid_constant__ JunctionArgs a) {
   using T = typename Elem<DT>::type;
   __shared__ float red[3 * 32];
+  dependent_wait();
   const BwppCudaJunctionParams &p = a.p;
   uint32_t first, last;
   chunk_range(a, blockIdx.x, first, last);
@@ -697,6 +702,7 @@ constexpr int kSumWarps = 32;
 __global__ void __launch_bounds__(32 * kSumWarps) junction_sums_kernel(const JunctionSums a) {
   const uint32_t job = blockIdx.x;
   float *out = job == 0 ? a.dgain_post : job == 1 ? a.dgain_pre : a.dgate;
+  dependent_wait();
   if (!out) return;
   __shared__ float sums[kSumWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -715,8 +721,8 @@ __global__ void __launch_bounds__(32 * kSumWarps) junction_sums_kernel(const Jun
       for (int u = 0; u < U; ++u) {
         const uint32_t at = k + u * kSumWarps;
         const float *g = weight(at);
-        v[u] = at < to ? __ldg(part + (size_t)at * a.cols + c) : 0.0f;
-        w[u] = g && at < to ? __ldg(g + c) : 1.0f;
+        v[u] = at < to ? part[(size_t)at * a.cols + c] : 0.0f;
+        w[u] = g && at < to ? g[c] : 1.0f;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) sum += v[u] * w[u];
@@ -731,7 +737,7 @@ __global__ void __launch_bounds__(32 * kSumWarps) junction_sums_kernel(const Jun
     } else if (a.chunks_per_group >= (uint32_t)kSumWarps) {
       // groups that keep every warp busy: one weight for each
       for (uint32_t k = 0, g = 0; k < a.chunks; k += a.chunks_per_group, ++g) {
-        const float w = __ldg(a.gate + (size_t)g * a.ldgate + c);
+        const float w = a.gate[(size_t)g * a.ldgate + c];
         acc += w * add(k + warp, k + a.chunks_per_group, plain);
       }
     } else {
@@ -799,18 +805,20 @@ bool vectors(const JunctionArgs &a) {
 }
 
 template <int DT>
-void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
+int launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
   const uint32_t cols = a.p.cols;
   cudaStream_t s = ctx->stream;
+  cudaError_t rc;
   // Few threads with more of the row each keep more bytes in flight per SM and
   // have less to wait for at the row's two reductions (32768 x 2048 bf16: 147 us
   // with 256 threads, 130 with 128, 127 with 64, 140 with a warp); many threads
   // finish a single row sooner (3.1 us with 256, 4.5 with 64).
   const bool many = a.p.rows > (uint32_t)ctx->num_sms * 4;
 #define BWPP_FWD(VEC, NV, TPR)                                                             \
-  junction_fwd_kernel<DT, VEC, NV, TPR>                                                    \
-      <<<(a.p.rows + block_threads(TPR) / TPR - 1) / (block_threads(TPR) / TPR),           \
-         block_threads(TPR), 0, s>>>(a)
+  rc = bwpp_launch_dependent(                                                              \
+      junction_fwd_kernel<DT, VEC, NV, TPR>,                                               \
+      dim3((a.p.rows + block_threads(TPR) / TPR - 1) / (block_threads(TPR) / TPR)),        \
+      dim3(block_threads(TPR)), 0, s, a)
   if (vectors<DT>(a)) {
     if (cols <= 64) BWPP_FWD(8, 1, 8);
     else if (cols <= 128) BWPP_FWD(8, 1, 16);
@@ -827,7 +835,7 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
     else if (cols <= 8192) BWPP_FWD(8, 2, 512);
     else if (cols <= 12288) BWPP_FWD(8, 3, 512);
     else if (cols <= 16384) BWPP_FWD(8, 4, 512);
-    else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
+    else rc = bwpp_launch_dependent(junction_fwd_looped_kernel<DT>, dim3(a.p.rows), dim3(kLoopThreads), 0, s, a);
   } else {
     if (cols <= 64) BWPP_FWD(1, 8, 8);
     else if (cols <= 128) BWPP_FWD(1, 8, 16);
@@ -837,9 +845,10 @@ void launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
     else if (cols <= 2048) BWPP_FWD(1, 8, 256);
     else if (cols <= 4096) BWPP_FWD(1, 8, 512);
     else if (cols <= 16384) BWPP_FWD(1, 16, 1024);
-    else junction_fwd_looped_kernel<DT><<<a.p.rows, kLoopThreads, 0, s>>>(a);
+    else rc = bwpp_launch_dependent(junction_fwd_looped_kernel<DT>, dim3(a.p.rows), dim3(kLoopThreads), 0, s, a);
   }
 #undef BWPP_FWD
+  return bwpp_check_cuda(ctx, rc, "junction fwd");
 }
 
 // How the backward takes a row width: CTAs per SM (as many as are resident:
@@ -873,7 +882,10 @@ Plan plan_bwd(const JunctionArgs &a) {
   }
   if (g.stages > (uint32_t)kMaxStages) g.stages = kMaxStages;
   if (g.stages < 2) return held;
-  g.bytes = g.stages * row;
+  // A CTA asks for its whole share of shared memory: one more on an SM would
+  // leave another SM with one less, which happens when the kernel in front still
+  // holds SMs as these are placed (32768 x 2048 bf16: 263 us instead of 211).
+  g.bytes = sm / g.per_sm;
   return g;
 }
 
@@ -892,8 +904,10 @@ int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, cons
     if (rc) return rc;
     set = true;
   }
-  kern<<<chunks, TPR, g.bytes, ctx->stream>>>(a, g.stages, ctx->status_word);
-  return BWPP_CUDA_OK;
+  return bwpp_check_cuda(ctx,
+                         bwpp_launch_dependent(kern, dim3(chunks), dim3(TPR), g.bytes, ctx->stream, a,
+                                               g.stages, ctx->status_word),
+                         "junction bwd");
 }
 
 template <int DT, bool TOKEN>
@@ -913,8 +927,10 @@ int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const P
   if (g.stages)
     return a.p.gate_rows == 1 && a.gate ? launch_staged_any<DT, true>(ctx, a, chunks, g)
                                         : launch_staged_any<DT, false>(ctx, a, chunks, g);
-#define BWPP_BWD(VEC, NV, TPR) \
-  junction_bwd_kernel<DT, VEC, NV, TPR><<<chunks, block_threads(TPR), 0, s>>>(a)
+  cudaError_t rc;
+#define BWPP_BWD(VEC, NV, TPR)                                                              \
+  rc = bwpp_launch_dependent(junction_bwd_kernel<DT, VEC, NV, TPR>, dim3(chunks),           \
+                             dim3(block_threads(TPR)), 0, s, a)
   if (vectors<DT>(a) && cols <= 256) {
     if (cols <= 64) BWPP_BWD(8, 1, 8);
     else if (cols <= 128) BWPP_BWD(8, 1, 16);
@@ -927,10 +943,10 @@ int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const P
     else if (cols <= 1024) BWPP_BWD(1, 4, 256);
     else if (cols <= 2048) BWPP_BWD(1, 4, 512);
     else if (cols <= 4096) BWPP_BWD(1, 8, 512);
-    else junction_bwd_looped_kernel<DT><<<chunks, kLoopThreads, 0, s>>>(a);
+    else rc = bwpp_launch_dependent(junction_bwd_looped_kernel<DT>, dim3(chunks), dim3(kLoopThreads), 0, s, a);
   }
 #undef BWPP_BWD
-  return BWPP_CUDA_OK;
+  return bwpp_check_cuda(ctx, rc, "junction bwd");
 }
 
 template <int DT>
@@ -953,9 +969,7 @@ int junction_fwd(BwppCudaCtx *ctx, const float *h, const void *b, const float *g
   a.gain_pre = gain_pre;
   a.h_out = h_out;
   a.y = y;
-  launch_fwd<DT>(ctx, a);
-  BWPP_LAUNCH_CHECK(ctx, "junction fwd");
-  return BWPP_CUDA_OK;
+  return launch_fwd<DT>(ctx, a);
 }
 
 template <int DT>
@@ -1022,7 +1036,6 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
   }
   rc = launch_bwd<DT>(ctx, a, k.chunks, g);
   if (rc) return rc;
-  BWPP_LAUNCH_CHECK(ctx, "junction bwd");
   if (sums) {
     JunctionSums q{};
     q.part_post = a.part_post;
@@ -1038,8 +1051,10 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
     q.ldgate = a.p.ldgate;
     q.weighted = gate && !per_row;
     const dim3 grid(2 + (q.dgate ? k.groups : 0), (a.p.cols + 31) / 32);
-    junction_sums_kernel<<<grid, 32 * kSumWarps, 0, s>>>(q);
-    BWPP_LAUNCH_CHECK(ctx, "junction sums");
+    rc = bwpp_check_cuda(
+        ctx, bwpp_launch_dependent(junction_sums_kernel, grid, dim3(32 * kSumWarps), 0, s, q),
+        "junction sums");
+    if (rc) return rc;
   }
   return BWPP_CUDA_OK;
 }

@@ -51,6 +51,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   constexpr bool ONE = IL && VEC > 1;  // a vector holds both sides of its pairs
   constexpr int PAIRS = ONE ? VEC / 2 : VEC;
   constexpr int kBatch = batch_of(ONE);
+  dependent_wait();
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   if (id >= a.units) return;
   const uint32_t per = a.slots * a.lanes;
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   bool ready = !turns;
   auto angles = [&]() {
     const int64_t pos =
-        a.positions ? (int64_t)__ldg(a.positions + t) : (int64_t)a.p.pos0 + (int64_t)s;
+        a.positions ? (int64_t)a.positions[t] : (int64_t)a.p.pos0 + (int64_t)s;
     const float up = a.table.amplitude, side = a.p.inverse ? -up : up;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
@@ -163,9 +164,12 @@ int rope_launch(BwppCudaCtx *ctx, RopeArgs &a) {
     a.token0 = (uint32_t)t0;
     a.units = (uint32_t)(n * per);
     const uint32_t grid = (a.units + kThreads - 1) / kThreads;
-    if (p.interleaved) rope_kernel<DT, VEC, true><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else rope_kernel<DT, VEC, false><<<grid, kThreads, 0, ctx->stream>>>(a);
-    BWPP_LAUNCH_CHECK(ctx, "rope");
+    const int rc = bwpp_check_cuda(
+        ctx,
+        bwpp_launch_dependent(p.interleaved ? rope_kernel<DT, VEC, true> : rope_kernel<DT, VEC, false>,
+                              dim3(grid), dim3(kThreads), 0, ctx->stream, a),
+        "rope");
+    if (rc) return rc;
   }
   return BWPP_CUDA_OK;
 }

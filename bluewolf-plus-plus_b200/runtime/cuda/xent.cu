@@ -41,9 +41,10 @@ constexpr uint32_t kSpan = 256;
 // to a multiple of eight.  With targets, rows that are ignored become zero, and
 // a target outside the vocabulary is reported.
 __global__ void __launch_bounds__(kThreads)
-    pack_rows_kernel(const uint16_t *__restrict__ src, uint16_t *__restrict__ dst, uint32_t rows,
+    pack_rows_kernel(const uint16_t *src, uint16_t *dst, uint32_t rows,
                      uint32_t cols, size_t ld_src, size_t ld_dst, int wide, const int32_t *target,
                      uint32_t V, int *status) {
+  dependent_wait();
   const uint32_t spans = (cols + kSpan - 1) / kSpan;
   const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) / 32, lane = threadIdx.x & 31;
   if (i >= rows * spans) return;
@@ -60,15 +61,15 @@ __global__ void __launch_bounds__(kThreads)
   if (wide && c0 + kSpan <= cols) {
     const uint32_t c = c0 + lane * 8;
     *reinterpret_cast<uint4 *>(to + c) =
-        live ? __ldg(reinterpret_cast<const uint4 *>(from + c)) : make_uint4(0u, 0u, 0u, 0u);
+        live ? *reinterpret_cast<const uint4 *>(from + c) : make_uint4(0u, 0u, 0u, 0u);
     return;
   }
   uint32_t v[kSpan / 64];
 #pragma unroll
   for (uint32_t k = 0; k < kSpan / 64; ++k) {
     const uint32_t c = c0 + k * 64 + lane * 2;
-    const uint32_t lo = live && c < cols ? __ldg(from + c) : 0u;
-    const uint32_t hi = live && c + 1 < cols ? __ldg(from + c + 1) : 0u;
+    const uint32_t lo = live && c < cols ? from[c] : 0u;
+    const uint32_t hi = live && c + 1 < cols ? from[c + 1] : 0u;
     v[k] = lo | hi << 16;
   }
 #pragma unroll
@@ -81,8 +82,9 @@ __global__ void __launch_bounds__(kThreads)
 // Results from rows of 16 bytes in scratch into rows of any pitch.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    unpack_rows_kernel(const T *__restrict__ src, T *__restrict__ dst, uint32_t rows, uint32_t cols,
+    unpack_rows_kernel(const T *src, T *dst, uint32_t rows, uint32_t cols,
                        size_t ld_src, size_t ld_dst) {
+  dependent_wait();
   const uint32_t spans = (cols + kSpan - 1) / kSpan;
   const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) / 32, lane = threadIdx.x & 31;
   if (i >= rows * spans) return;
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (uint32_t k = 0; k < kSpan / 32; ++k) {
     const uint32_t c = c0 + k * 32 + lane;
-    if (c < cols) v[k] = __ldg(src + r * ld_src + c);
+    if (c < cols) v[k] = src[r * ld_src + c];
   }
 #pragma unroll
   for (uint32_t k = 0; k < kSpan / 32; ++k) {
@@ -107,10 +109,14 @@ int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t row
   const uint32_t most = (1u << 25) / spans;  // rows of a launch: indices stay in 31 bits
   for (uint32_t r0 = 0; r0 < rows; r0 += most) {
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
-    pack_rows_kernel<<<(n * spans + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, ctx->stream>>>(
-        src + (size_t)r0 * ld_src, dst + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst, wide,
-        target ? target + r0 : nullptr, V, ctx->status_word);
-    BWPP_LAUNCH_CHECK(ctx, "xent pack");
+    const int rc = bwpp_check_cuda(
+        ctx,
+        bwpp_launch_dependent(pack_rows_kernel, dim3((n * spans + kThreads / 32 - 1) / (kThreads / 32)),
+                              dim3(kThreads), 0, ctx->stream, src + (size_t)r0 * ld_src,
+                              dst + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst, wide,
+                              target ? target + r0 : nullptr, V, ctx->status_word),
+        "xent pack");
+    if (rc) return rc;
   }
   return BWPP_CUDA_OK;
 }
@@ -122,10 +128,14 @@ int unpack_rows(BwppCudaCtx *ctx, const void *src, void *dst, uint32_t rows, uin
   const uint32_t most = (1u << 25) / spans;
   for (uint32_t r0 = 0; r0 < rows; r0 += most) {
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
-    unpack_rows_kernel<T><<<(n * spans + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, ctx->stream>>>(
-        static_cast<const T *>(src) + (size_t)r0 * ld_src, static_cast<T *>(dst) + (size_t)r0 * ld_dst,
-        n, cols, ld_src, ld_dst);
-    BWPP_LAUNCH_CHECK(ctx, "xent unpack");
+    const int rc = bwpp_check_cuda(
+        ctx,
+        bwpp_launch_dependent(unpack_rows_kernel<T>,
+                              dim3((n * spans + kThreads / 32 - 1) / (kThreads / 32)), dim3(kThreads), 0,
+                              ctx->stream, static_cast<const T *>(src) + (size_t)r0 * ld_src,
+                              static_cast<T *>(dst) + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst),
+        "xent unpack");
+    if (rc) return rc;
   }
   return BWPP_CUDA_OK;
 }

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  dependent_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -385,9 +386,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 // A product from its K parts, added in order, into rows of any pitch.  A warp takes
 // 256 columns of a row.
 __global__ void __launch_bounds__(256)
-    xent_sum_parts_kernel(const float *__restrict__ part, uint32_t parts, size_t part_stride,
-                          void *__restrict__ out, uint32_t rows, uint32_t cols, size_t ld,
+    xent_sum_parts_kernel(const float *part, uint32_t parts, size_t part_stride, void *out, uint32_t rows, uint32_t cols, size_t ld,
                           size_t ld_out, int bf16) {
+  dependent_wait();
   const uint32_t spans = (cols + 255) / 256;
   const uint32_t i = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x & 31;
   if (i >= rows * spans) return;
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(256)
     const float *p = part + s * part_stride + r * ld;
 #pragma unroll
     for (uint32_t k = 0; k < 8; ++k)
-      if (c0 + k * 32 < cols) v[k] += __ldg(p + c0 + k * 32);
+      if (c0 + k * 32 < cols) v[k] += p[c0 + k * 32];
   }
 #pragma unroll
   for (uint32_t k = 0; k < 8; ++k) {
@@ -560,17 +561,19 @@ int bwpp_xent_grad_launch(BwppCudaCtx *ctx, const XentProduct *dx, const XentPro
     work.ahead = tile_time(p0.num_kb, p0.parts) / tile_time(p1.num_kb, p1.parts);
   if (dx) p0.group = group_of(p0, n);
   if (dw) p1.group = group_of(p1, n);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = pairs > 0 ? 2 : 1;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((pairs > 0 ? 2 : 1) * n, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = pairs > 0 ? Cfg<true>::SMEM : Cfg<false>::SMEM;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
-  cfg.numAttrs = pairs > 0 ? 1 : 0;
+  cfg.numAttrs = 2;
   int *status = ctx->status_word;
   return bwpp_check_cuda(
       ctx,
@@ -586,9 +589,12 @@ int bwpp_xent_sum_parts_launch(BwppCudaCtx *ctx, const float *part, uint32_t par
   for (uint32_t r0 = 0; r0 < rows; r0 += most) {
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
     uint8_t *to = static_cast<uint8_t *>(out) + (size_t)r0 * ld_out * (bf16 ? 2 : 4);
-    xent_sum_parts_kernel<<<(n * spans + 7) / 8, 256, 0, ctx->stream>>>(
-        part + (size_t)r0 * ld, parts, part_stride, to, n, cols, ld, ld_out, bf16);
-    BWPP_LAUNCH_CHECK(ctx, "xent sum");
+    const int rc = bwpp_check_cuda(
+        ctx,
+        bwpp_launch_dependent(xent_sum_parts_kernel, dim3((n * spans + 7) / 8), dim3(256), 0, ctx->stream,
+                              part + (size_t)r0 * ld, parts, part_stride, to, n, cols, ld, ld_out, bf16),
+        "xent sum");
+    if (rc) return rc;
   }
   return BWPP_CUDA_OK;
 }

@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  dependent_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -316,15 +317,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t first = col + sub * 128;  // this warp's first column
       const uint32_t end = min(a.V, col + width);
       const bool live_row = row < a.T;
-      const int32_t target = live_row && a.target ? __ldg(a.target + row) : -1;
+      const int32_t target = live_row && a.target ? __ldcg(a.target + row) : -1;
       // the target's column within this warp's 128, or beyond them
       const uint32_t hit_col =
           target >= 0 ? (uint32_t)target - a.v0 - first : 0xffffffffu;
       float g = 0.0f, lse2 = 0.0f;
       if constexpr (!FWD) {
         if (live_row && (uint32_t)target < a.vocab) {
-          g = a.scale * (a.dloss ? __ldg(a.dloss + row) : 1.0f);
-          lse2 = __ldg(a.lse + row) * 1.44269504f;
+          g = a.scale * (a.dloss ? __ldcg(a.dloss + row) : 1.0f);
+          lse2 = __ldcg(a.lse + row) * 1.44269504f;
         }
       }
       const bool live = live_row && (uint32_t)target < a.vocab;
@@ -516,15 +517,15 @@ __device__ __forceinline__ void finish_row(uint32_t t, float2 x, const float *hi
 // ... and the warps' results meet in shared memory, in order.
 constexpr int COMBINE_WARPS = 16;
 __global__ void __launch_bounds__(32 * COMBINE_WARPS)
-    xent_combine_kernel(const float2 *__restrict__ part, uint32_t nparts, const float *__restrict__ hit,
-                        const int32_t *__restrict__ target, float *__restrict__ loss,
-                        float *__restrict__ lse, uint32_t T, uint32_t V, int *status) {
+    xent_combine_kernel(const float2 *part, uint32_t nparts, const float *hit, const int32_t *target, float *loss,
+                        float *lse, uint32_t T, uint32_t V, int *status) {
   __shared__ float2 got[COMBINE_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t t = blockIdx.x * 32 + lane;
+  dependent_wait();
   float2 x = make_float2(-INFINITY, 0.0f);
   if (t < T)
-    for (uint32_t k = warp; k < nparts; k += COMBINE_WARPS) fold_pair(x, __ldg(part + (size_t)k * T + t));
+    for (uint32_t k = warp; k < nparts; k += COMBINE_WARPS) fold_pair(x, part[(size_t)k * T + t]);
   got[warp][lane] = x;
   __syncthreads();
   if (warp || t >= T) return;
@@ -532,8 +533,7 @@ __global__ void __launch_bounds__(32 * COMBINE_WARPS)
   finish_row(t, x, hit, target, loss, lse, V, status);
 }
 
-// Few rows: a block a row, its threads share the pairs.  Launched while the
-// kernel that writes them still runs; waits for its end before it reads.
+// Few rows: a block a row, its threads share the pairs.
 constexpr int FEW_THREADS = 256;
 __global__ void __launch_bounds__(FEW_THREADS)
     xent_combine_few_kernel(const float2 *part, uint32_t nparts, const float *hit, const int32_t *target,
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
   __shared__ float2 got[FEW_THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t t = blockIdx.x;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  dependent_wait();
   float2 x = make_float2(-INFINITY, 0.0f);
   for (uint32_t k = threadIdx.x; k < nparts; k += FEW_THREADS) fold_pair(x, part[(size_t)k * T + t]);
 #pragma unroll
@@ -571,17 +571,19 @@ int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const
     if (rc) return rc;
     g_smem_set[v][dev] = true;
   }
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = PAIR ? 2 : 1;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ctx->num_sms & ~1), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = 1;
   uint32_t cap = (uint32_t)ctx->num_sms;
   if constexpr (PAIR) {
     int &pairs = g_pairs[v][dev];
@@ -612,6 +614,7 @@ int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const
   b.group = (uint32_t)(fit < 8 ? 8 : fit > blocks ? blocks : fit);
   const uint32_t n = b.items < cap ? b.items : cap;
   cfg.gridDim = dim3((PAIR ? 2 : 1) * n, 1, 1);
+  cfg.numAttrs = 2;
   int *status = ctx->status_word;
   return bwpp_check_cuda(ctx, cudaLaunchKernelEx(&cfg, kern, tx, tw, to, b, status),
                          FWD ? "xent logits" : "xent dlogit");
@@ -670,26 +673,13 @@ int bwpp_xent_stats_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_
 
 int bwpp_xent_combine_launch(BwppCudaCtx *ctx, const float2 *part, uint32_t nparts, const float *hit,
                              const int32_t *target, float *loss, float *lse, uint32_t T, uint32_t V) {
-  if (T > 32) {
-    xent_combine_kernel<<<(T + 31) / 32, 32 * COMBINE_WARPS, 0, ctx->stream>>>(
-        part, nparts, hit, target, loss, lse, T, V, ctx->status_word);
-    BWPP_LAUNCH_CHECK(ctx, "xent combine");
-    return BWPP_CUDA_OK;
-  }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(T, 1, 1);
-  cfg.blockDim = dim3(FEW_THREADS, 1, 1);
-  cfg.stream = ctx->stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int *status = ctx->status_word;
-  return bwpp_check_cuda(ctx,
-                         cudaLaunchKernelEx(&cfg, xent_combine_few_kernel, part, nparts, hit, target,
-                                            loss, lse, T, V, status),
-                         "xent combine");
+  const bool few = T <= 32;
+  return bwpp_check_cuda(
+      ctx,
+      bwpp_launch_dependent(few ? xent_combine_few_kernel : xent_combine_kernel,
+                            dim3(few ? T : (T + 31) / 32), dim3(few ? FEW_THREADS : 32 * COMBINE_WARPS),
+                            0, ctx->stream, part, nparts, hit, target, loss, lse, T, V, ctx->status_word),
+      "xent combine");
 }
 
 int bwpp_xent_dlogit_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_t *target,
