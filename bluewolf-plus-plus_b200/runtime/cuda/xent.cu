@@ -37,20 +37,72 @@ constexpr int kThreads = 256;
 // own, as 2-byte accesses 16 bytes apart, took 60 us for 1001 x 10007 bf16.)
 constexpr uint32_t kSpan = 256;
 
+// The dloss that all live rows share, if they do: out = {scale * dloss, 1}, or
+// {1, 0} where they differ.  The gradients' products then take p - hit, and this
+// factor goes onto their results: with a mean loss, the usual one, a rounding
+// of scale * dloss * (p - hit) would round the same mantissa, that of 1 / rows,
+// in every row, up to 2^-8 of all targets' entries at once.
+struct Common {
+  const float *dloss;  // NULL: ones
+  uint32_t T;
+  float scale;
+  float *out;          // NULL: not wanted
+};
+
+// One block.
+__device__ __forceinline__ void find_common(const Common &a, const int32_t *target, uint32_t V) {
+  __shared__ float lows[kThreads / 32], highs[kThreads / 32];
+  float low = INFINITY, high = -INFINITY;
+  bool odd = false;  // NaN: no two are alike
+#pragma unroll 4
+  for (uint32_t t = threadIdx.x; t < a.T; t += kThreads) {
+    const bool live = (uint32_t)target[t] < V;
+    const float g = a.dloss ? a.dloss[t] : 1.0f;
+    odd |= live && g != g;
+    low = live ? fminf(low, g) : low;
+    high = live ? fmaxf(high, g) : high;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  }
+  if ((threadIdx.x & 31) == 0) {
+    lows[threadIdx.x >> 5] = low;
+    highs[threadIdx.x >> 5] = high;
+  }
+  odd = __syncthreads_or(odd);
+  if (threadIdx.x) return;
+  for (int w = 1; w < kThreads / 32; ++w) {
+    low = fminf(low, lows[w]);
+    high = fmaxf(high, highs[w]);
+  }
+  const bool same = !odd && low == high && low - low == 0.0f;  // one finite value
+  a.out[0] = same ? a.scale * low : 1.0f;
+  a.out[1] = same ? 1.0f : 0.0f;
+}
+
 // dst[r, c] = src[r, c] of 16-bit elements; dst's rows are filled up with zeros
 // to a multiple of eight.  With targets, rows that are ignored become zero, and
-// a target outside the vocabulary is reported.
+// a target outside the vocabulary is reported.  again > 0: the rows have a
+// second copy `again` rows below, and rows from `live_rows` on are zero.  The
+// block behind the rows' finds the common dloss: a launch of its own cost 2.7 us.
 __global__ void __launch_bounds__(kThreads)
     pack_rows_kernel(const uint16_t *src, uint16_t *dst, uint32_t rows,
                      uint32_t cols, size_t ld_src, size_t ld_dst, int wide, const int32_t *target,
-                     uint32_t V, int *status) {
+                     uint32_t V, uint32_t live_rows, uint32_t again, const Common common,
+                     int *status) {
   dependent_wait();
+  if (common.out && blockIdx.x == gridDim.x - 1) {
+    find_common(common, target, V);
+    return;
+  }
   const uint32_t spans = (cols + kSpan - 1) / kSpan;
   const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) / 32, lane = threadIdx.x & 31;
   if (i >= rows * spans) return;
   const uint32_t r = i / spans, c0 = (i - r * spans) * kSpan;
-  bool live = true;
-  if (target) {
+  bool live = r < live_rows;
+  if (live && target) {
     const int32_t y = target[r];
     live = (uint32_t)y < V;
     if (y >= 0 && !live && c0 + lane == 0) bwpp_report(status, BWPP_CUDA_ERR_ARG);
@@ -60,8 +112,9 @@ __global__ void __launch_bounds__(kThreads)
   const uint32_t padded = (cols + 7) & ~7u;
   if (wide && c0 + kSpan <= cols) {
     const uint32_t c = c0 + lane * 8;
-    *reinterpret_cast<uint4 *>(to + c) =
-        live ? *reinterpret_cast<const uint4 *>(from + c) : make_uint4(0u, 0u, 0u, 0u);
+    const uint4 t = live ? *reinterpret_cast<const uint4 *>(from + c) : make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<uint4 *>(to + c) = t;
+    if (again) *reinterpret_cast<uint4 *>(to + again * ld_dst + c) = t;
     return;
   }
   uint32_t v[kSpan / 64];
@@ -75,7 +128,9 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (uint32_t k = 0; k < kSpan / 64; ++k) {
     const uint32_t c = c0 + k * 64 + lane * 2;
-    if (c < padded) *reinterpret_cast<uint32_t *>(to + c) = v[k];
+    if (c >= padded) continue;
+    *reinterpret_cast<uint32_t *>(to + c) = v[k];
+    if (again) *reinterpret_cast<uint32_t *>(to + again * ld_dst + c) = v[k];
   }
 }
 
@@ -103,7 +158,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t rows, uint32_t cols,
-              uint32_t ld_src, uint32_t ld_dst, const int32_t *target, uint32_t V) {
+              uint32_t ld_src, uint32_t ld_dst, const int32_t *target, uint32_t V,
+              uint32_t live_rows = 0xffffffffu, uint32_t again = 0, Common common = Common{}) {
   const uint32_t spans = (cols + kSpan - 1) / kSpan;
   const int wide = ld_src % 8 == 0 && aligned_to(src, 16);
   const uint32_t most = (1u << 25) / spans;  // rows of a launch: indices stay in 31 bits
@@ -111,12 +167,15 @@ int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t row
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
     const int rc = bwpp_check_cuda(
         ctx,
-        bwpp_launch_dependent(pack_rows_kernel, dim3((n * spans + kThreads / 32 - 1) / (kThreads / 32)),
+        bwpp_launch_dependent(pack_rows_kernel,
+                              dim3((n * spans + kThreads / 32 - 1) / (kThreads / 32) + (common.out != nullptr)),
                               dim3(kThreads), 0, ctx->stream, src + (size_t)r0 * ld_src,
                               dst + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst, wide,
-                              target ? target + r0 : nullptr, V, ctx->status_word),
+                              target ? target + r0 : nullptr, V, live_rows > r0 ? live_rows - r0 : 0, again,
+                              common, ctx->status_word),
         "xent pack");
     if (rc) return rc;
+    common.out = nullptr;  // the first launch found it, from all rows
   }
   return BWPP_CUDA_OK;
 }
@@ -149,7 +208,8 @@ struct Layout {
   uint32_t dp;                // D rounded up
   // K parts of dx and of dW that scratch has room for, and the rows of one
   uint32_t dx_rows, dx_parts, dw_rows, dw_parts;
-  size_t part, hit, x, w, dlogit, dx, dw, total;
+  uint32_t k_rows;            // backward: rows of x and dlogit in scratch
+  size_t part, hit, x, w, dlogit, dx, dw, common, total;
 };
 
 // Equal pieces of about c columns, whole 256s, at least 1024.
@@ -176,7 +236,8 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
   l.dp = up8(p.D);
   l.piece = backward ? piece_of((1ull << 27) / p.T, p.V)
                      : piece_of(pack_w ? (1ull << 25) / l.dp : (uint64_t)p.V, p.V);
-  l.dx_rows = (uint32_t)up256(p.T);
+  l.k_rows = p.T <= XENT_EXACT_ROWS ? 2 * XENT_EXACT_ROWS : p.T;
+  l.dx_rows = (uint32_t)up256(l.k_rows);
   l.dx_parts = parts_that_fit(l.dx_rows, l.dp);
   l.dw_rows = (uint32_t)up256(p.w_vocab_major ? l.piece : p.D);
   l.dw_parts = parts_that_fit(l.dw_rows, p.w_vocab_major ? l.dp : l.piece);
@@ -187,13 +248,14 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
     return here;
   };
   const size_t es = p.grads_bf16 ? 2 : 4;
-  if (pack_x || backward) l.x = take((size_t)p.T * l.dp * 2);
+  if (pack_x || backward) l.x = take((size_t)(backward ? l.k_rows : p.T) * l.dp * 2);
   if (pack_w) l.w = take((size_t)l.piece * l.dp * 2);
   if (!backward) {
     l.part = take((((size_t)p.V + 127) / 128) * p.T * sizeof(float2));
     l.hit = take((size_t)p.T * 4);
   } else {
-    l.dlogit = take((size_t)p.T * l.piece * 2);
+    l.common = take(2 * sizeof(float));
+    l.dlogit = take((size_t)l.k_rows * l.piece * 2);
     if (stage_dx) l.dx = take((size_t)l.dx_parts * l.dx_rows * l.dp * 4);
     if (stage_dw || l.dw_parts > 1)
       l.dw = take((size_t)l.dw_parts * l.dw_rows * (p.w_vocab_major ? l.dp : l.piece) *
@@ -272,7 +334,8 @@ int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     rc = piece_w(ctx, p, w, pack_w, reinterpret_cast<uint16_t *>(scratch + l.w), v0, n,
                  p.w_vocab_major ? l.dp : l.piece, w1);
     const XentOperands o{x, w1.w, p.T, n, p.D, ldx, w1.ld, v0, p.V, p.w_vocab_major != 0, p.scale};
-    if (!rc) rc = bwpp_xent_stats_launch(ctx, o, loss ? target : nullptr, part + (size_t)(v0 / 128) * p.T, hit);
+    if (!rc)
+      rc = bwpp_xent_stats_launch(ctx, o, loss ? target : nullptr, part + (size_t)(v0 / 128) * p.T, hit);
     if (rc) return rc;
   }
   return bwpp_xent_combine_launch(ctx, part, (p.V + 127) / 128, hit, target, loss, lse, p.T, p.V);
@@ -309,7 +372,7 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   // The products of the piece [v0, v0 + n), with no addresses yet.
   auto products = [&](uint32_t n, XentProduct &px, XentProduct &pw) {
     px = XentProduct{};
-    px.M = p.T;
+    px.M = probe.k_rows;
     px.N = p.D;
     px.K = n;
     px.lda = piece;
@@ -320,7 +383,7 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     pw = XentProduct{};
     pw.M = vm ? n : p.D;
     pw.N = vm ? p.D : n;
-    pw.K = p.T;
+    pw.K = probe.k_rows;
     pw.lda = vm ? piece : probe.dp;
     pw.ldb = vm ? probe.dp : piece;
     pw.a_mn = pw.b_mn = true;
@@ -333,15 +396,21 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   uint32_t dx_parts, dw_parts;
   rc = bwpp_xent_parts(ctx, px, pw, probe.dx_parts, probe.dw_parts, &dx_parts, &dw_parts);
   if (rc) return rc;
+  // few rows: two bf16 for each dlogit, XENT_EXACT_ROWS apart, which are summed here
+  const bool exact = p.T <= XENT_EXACT_ROWS;
   // dx is summed in scratch, unless the caller's rows take it: all of it in one
   // piece, or fp32 sums
-  const bool direct = dx_out && dx_parts == 1 && (pieces == 1 || !p.grads_bf16);
+  const bool one_sum = dx_out && dx_parts == 1 && !exact;
+  const bool direct = one_sum && (pieces == 1 || !p.grads_bf16);
   const Layout l = layout_of(p, true, pack_w, true, dx && !direct, stage_dw);
   uint8_t *scratch;
   rc = bwpp_op_scratch(ctx, l.total, "xent bwd", &scratch);
   if (rc) return rc;
   uint16_t *xp = reinterpret_cast<uint16_t *>(scratch + l.x);
-  rc = pack_rows(ctx, x, xp, p.T, p.D, p.ldx, l.dp, target, p.V);
+  float *common = exact ? nullptr : reinterpret_cast<float *>(scratch + l.common);
+  rc = exact ? pack_rows(ctx, x, xp, XENT_EXACT_ROWS, p.D, p.ldx, l.dp, target, p.V, p.T, XENT_EXACT_ROWS)
+             : pack_rows(ctx, x, xp, p.T, p.D, p.ldx, l.dp, target, p.V, p.T, 0,
+                         Common{dloss, p.T, p.scale, common});
   if (rc) return rc;
   uint16_t *dlogit = reinterpret_cast<uint16_t *>(scratch + l.dlogit);
   for (uint32_t v0 = 0; v0 < p.V; v0 += piece) {
@@ -351,19 +420,20 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     rc = piece_w(ctx, p, w, pack_w, reinterpret_cast<uint16_t *>(scratch + l.w), v0, n,
                  vm ? l.dp : piece, w1);
     const XentOperands o{xp, w1.w, p.T, n, p.D, l.dp, w1.ld, v0, p.V, vm, p.scale};
-    if (!rc) rc = bwpp_xent_dlogit_launch(ctx, o, target, lse, dloss, dlogit, piece);
+    if (!rc) rc = bwpp_xent_dlogit_launch(ctx, o, target, lse, dloss, common, dlogit, piece);
     if (rc) return rc;
     products(n, px, pw);
     px.a = dlogit;
     px.b = w1.w;
     px.accumulate = v0 > 0;
     // the last piece leaves the sum in the caller's rows where it can
-    const bool to_user = direct || (dx_out && dx_parts == 1 && last);
+    const bool to_user = direct || (one_sum && last);
     px.add = direct ? dx : static_cast<void *>(scratch + l.dx);
     px.ld_add = direct ? p.lddx : l.dp;
     px.c = to_user ? dx : static_cast<void *>(scratch + l.dx);
     px.ldc = to_user ? p.lddx : l.dp;
-    px.bf16 = to_user && p.grads_bf16;
+    px.bf16 = to_user && last && p.grads_bf16;
+    px.factor = to_user && last ? common : nullptr;
     uint8_t *user_w =
         dw ? static_cast<uint8_t *>(dw) + (vm ? (size_t)v0 * p.lddw : (size_t)v0) * es : nullptr;
     const bool own_w = stage_dw || dw_parts > 1;  // dW's part goes through scratch
@@ -372,20 +442,22 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     pw.c = own_w ? static_cast<void *>(scratch + l.dw) : static_cast<void *>(user_w);
     pw.ldc = own_w ? (vm ? l.dp : piece) : p.lddw;
     pw.bf16 = p.grads_bf16 && dw_parts == 1;
+    pw.factor = dw_parts == 1 ? common : nullptr;
     rc = bwpp_xent_grad_launch(ctx, dx ? &px : nullptr, dw ? &pw : nullptr, dx_parts, dw_parts);
     if (!rc && dw && dw_parts > 1)
       rc = bwpp_xent_sum_parts_launch(ctx, static_cast<const float *>(pw.c), dw_parts,
-                                      (size_t)l.dw_rows * pw.ldc, user_w, pw.M, pw.N, pw.ldc, p.lddw,
-                                      p.grads_bf16);
+                                      (size_t)l.dw_rows * pw.ldc, 0, common, user_w, pw.M, pw.N, pw.ldc,
+                                      p.lddw, p.grads_bf16);
     else if (!rc && stage_dw)
       rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw)
                         : unpack_rows<float>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw);
     if (rc) return rc;
   }
-  if (dx && !direct && !(dx_out && dx_parts == 1))
+  if (dx && !one_sum) {
     return bwpp_xent_sum_parts_launch(ctx, reinterpret_cast<const float *>(scratch + l.dx), dx_parts,
-                                      (size_t)l.dx_rows * l.dp, dx, p.T, p.D, l.dp, p.lddx,
-                                      p.grads_bf16);
+                                      (size_t)l.dx_rows * l.dp, exact ? XENT_EXACT_ROWS * (size_t)l.dp : 0,
+                                      common, dx, p.T, p.D, l.dp, p.lddx, p.grads_bf16);
+  }
   return BWPP_CUDA_OK;
 }
 

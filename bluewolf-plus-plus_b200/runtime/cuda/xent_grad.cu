@@ -55,6 +55,7 @@ struct Product {
   uint32_t part_rows;       // rows from one part's C to the next
   const float *add;         // fp32 rows added to C (pitch ld_add; may be C), or NULL
   uint32_t ld_add;
+  const float *factor;      // multiplies C, or NULL
   uint32_t bf16;            // C is bf16, else fp32
 };
 
@@ -306,6 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t row0 = mb * C::TILE_M + rank * BM + q * 32, row = row0 + lane;
       const uint32_t out_row = part * p.part_rows + row0;
       const float *add = p.add && row < M ? p.add + (size_t)(out_row + lane) * p.ld_add : nullptr;
+      const float factor = p.factor ? __ldcg(p.factor) : 1.0f;
       if (!mbar_wait(&tfull[acc], acc_phase, status)) {
         *abort_flag = 1;
         break;
@@ -338,14 +340,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (cs + j < N) r[j] = __float_as_uint(__uint_as_float(r[j]) + add[cs + j]);
             }
           }
-          if (out16) {
+          const uint64_t f2 = f2pack(factor, factor);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              out[h * 16 + j] =
-                  pack2_16<false>(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) out[j] = r[j];
+          for (int j = 0; j < 16; ++j) {
+            float x, y;
+            f2unpack(f2mul(f2pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), f2), x, y);
+            if (out16) {
+              out[h * 16 + j] = pack2_16<false>(x, y);
+            } else {
+              out[2 * j] = __float_as_uint(x);
+              out[2 * j + 1] = __float_as_uint(y);
+            }
           }
         }
         if (lane == 0) tma_store_wait_read<0>();
@@ -383,10 +388,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// A product from its K parts, added in order, into rows of any pitch.  A warp takes
-// 256 columns of a row.
+// A product from its K parts, added in order, into rows of any pitch.  second: a
+// part has two terms, so many elements apart.  A warp takes 256 columns of a row.
 __global__ void __launch_bounds__(256)
-    xent_sum_parts_kernel(const float *part, uint32_t parts, size_t part_stride, void *out, uint32_t rows, uint32_t cols, size_t ld,
+    xent_sum_parts_kernel(const float *part, uint32_t parts, size_t part_stride, size_t second,
+                          const float *factor, void *out, uint32_t rows, uint32_t cols, size_t ld,
                           size_t ld_out, int bf16) {
   dependent_wait();
   const uint32_t spans = (cols + 255) / 256;
@@ -400,12 +406,14 @@ __global__ void __launch_bounds__(256)
     const float *p = part + s * part_stride + r * ld;
 #pragma unroll
     for (uint32_t k = 0; k < 8; ++k)
-      if (c0 + k * 32 < cols) v[k] += p[c0 + k * 32];
+      if (c0 + k * 32 < cols) v[k] += second ? p[c0 + k * 32] + p[second + c0 + k * 32] : p[c0 + k * 32];
   }
+  const float f = factor ? *factor : 1.0f;
 #pragma unroll
   for (uint32_t k = 0; k < 8; ++k) {
     const uint32_t c = c0 + k * 32;
     if (c >= cols) break;
+    v[k] *= f;
     if (bf16)
       static_cast<uint16_t *>(out)[r * ld_out + c] = (uint16_t)(pack2_16<false>(v[k], 0.0f) & 0xFFFFu);
     else
@@ -482,6 +490,7 @@ int make_product(BwppCudaCtx *ctx, const XentProduct &s, uint32_t tile_m, uint32
   p.part_rows = s.part_rows;
   p.add = s.accumulate ? static_cast<const float *>(s.add) : nullptr;
   p.ld_add = s.ld_add;
+  p.factor = s.factor;
   p.bf16 = s.bf16 ? 1 : 0;
   const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * parts;
   if (items >= 0x80000000ull) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: too many tiles");
@@ -583,8 +592,8 @@ int bwpp_xent_grad_launch(BwppCudaCtx *ctx, const XentProduct *dx, const XentPro
 }
 
 int bwpp_xent_sum_parts_launch(BwppCudaCtx *ctx, const float *part, uint32_t parts,
-                               size_t part_stride, void *out, uint32_t rows, uint32_t cols,
-                               uint32_t ld, uint32_t ld_out, int bf16) {
+                               size_t part_stride, size_t second, const float *factor, void *out,
+                               uint32_t rows, uint32_t cols, uint32_t ld, uint32_t ld_out, int bf16) {
   const uint32_t spans = (cols + 255) / 256, most = (1u << 28) / spans;
   for (uint32_t r0 = 0; r0 < rows; r0 += most) {
     const uint32_t n = rows - r0 < most ? rows - r0 : most;
@@ -592,7 +601,8 @@ int bwpp_xent_sum_parts_launch(BwppCudaCtx *ctx, const float *part, uint32_t par
     const int rc = bwpp_check_cuda(
         ctx,
         bwpp_launch_dependent(xent_sum_parts_kernel, dim3((n * spans + 7) / 8), dim3(256), 0, ctx->stream,
-                              part + (size_t)r0 * ld, parts, part_stride, to, n, cols, ld, ld_out, bf16),
+                              part + (size_t)r0 * ld, parts, part_stride, second, factor, to, n, cols, ld, ld_out,
+                              bf16),
         "xent sum");
     if (rc) return rc;
   }

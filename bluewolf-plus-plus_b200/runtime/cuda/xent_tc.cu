@@ -12,9 +12,12 @@
 // running maximum and sum of 2^(logit log2 e - maximum) stay in registers over
 // its four 32-column chunks and leave as one (maximum, sum) pair per row and
 // 128 columns, 8 bytes for every 512 of logits.  xent_combine_kernel folds a
-// row's pairs.  The thread that meets the row's target writes its logit.
-// Backward.  The epilogue turns the logits into bf16 scale g (p - hit) and
-// stores the tile by TMA: 2 bytes a logit, read by the two gradient products.
+// row's pairs.  The thread that meets the row's target writes its logit, which
+// stays out of the pair where there are few rows.
+// Backward.  The epilogue turns the logits into bf16 scale g (p - hit) (or p -
+// hit, where all rows have the same g: its mantissa would be rounded the same
+// way in every row) and stores the tile by TMA: 2 bytes a logit, read by the two
+// gradient products.
 //
 // Exponentials are ex2.approx (2 ulp): one per logit, 128 x 256 of them for a
 // tile are 2048 cycles of an SM's MUFU, against 128 cycles of MMA for every 16
@@ -52,11 +55,15 @@ struct XentTile {
   uint32_t v0;          // vocabulary index of column 0
   float c;              // scale * log2(e)
   const int32_t *target;
+  uint32_t chunk;       // EXACT: K blocks of a sum
   // FWD
   float2 *part;         // [ceil(V / 128)][T]
-  float *hit;           // [T] logit of the target
+  float *hit;           // [T] logit of the target, in powers of two like the pairs
+  bool apart;           // EXACT: the pairs leave the target out
   // backward
   const float *lse, *dloss;
+  const float *common;  // [2]: not 0 where all rows have one dloss, which then is
+                        // a factor of the results; NULL: rows have their own
   float scale;
   uint32_t vocab;       // targets below it are live
   // items [0, whole) are tiles, from there on each remaining tile is cut into
@@ -115,6 +122,27 @@ __device__ __forceinline__ void mask_logits(uint64_t (&t)[P], uint32_t col, uint
   }
 }
 
+// Column `at` of these; drop: it becomes -inf.
+template <int P>
+__device__ __forceinline__ float pick_logit(uint64_t (&t)[P], uint32_t at, bool drop) {
+  float h = 0.0f;
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    float x, y;
+    f2unpack(t[j], x, y);
+    if (at == 2u * j) {
+      h = x;
+      if (drop) x = -INFINITY;
+    }
+    if (at == 2u * j + 1) {
+      h = y;
+      if (drop) y = -INFINITY;
+    }
+    t[j] = f2pack(x, y);
+  }
+  return h;
+}
+
 // Tiles go down the row blocks of a group, then to the next 256 columns.
 __device__ __forceinline__ void tile_at(uint32_t i, uint32_t group, uint32_t tiles_m,
                                         uint32_t tiles_n, uint32_t &mb, uint32_t &nb) {
@@ -136,14 +164,18 @@ __device__ __forceinline__ void item_at(const XentTile &a, uint32_t i, uint32_t 
   col = nb * BN + (half ? (j & 1) * (BN / 2) : 0);
 }
 
-// The forward's sums over D are cut into chunks of this many K blocks, each
-// summed in TMEM from zero and added to the others in registers: the tensor
-// core truncates its running sum at each addition, and over D = 4096 the
-// errors, all towards zero, reached 2e-6 of lse (6e-7 at D = 1024).
-constexpr uint32_t CHUNK = 16;
-
-// CHUNKED (FWD, D > 1024): see CHUNK.
-template <bool B_MN, bool PAIR, bool FWD, bool CHUNKED>
+// EXACT: the sums over D are cut into chunks of `chunk` K blocks, each summed in
+// TMEM from zero and added to the others in registers.  The tensor core
+// truncates its running sum at each addition, and the errors, all towards zero,
+// grow with the length of a sum: lse at D = 4096 was off by 2e-6 of its value in
+// one sum, by 7e-7 in chunks of 16 blocks.  A few rows, which wait for W anyway,
+// take chunks of two: the loss of one token has no others to average with, and
+// at 512 to 2048 of D it went from 7e-6 to at most 2e-6 of its value.
+// EXACT, backward: dlogit leaves as two bf16, its rounded value and what the
+// rounding left, XENT_EXACT_ROWS below.  A gradient of few rows is mostly its targets'
+// entries times rows of W or x, so their rounding, up to 2^-8 of them, would be
+// its error; and 1 - p of a sure target is a difference, hence the chunks.
+template <bool B_MN, bool PAIR, bool FWD, bool EXACT>
 __global__ void __launch_bounds__(THREADS, 1)
     xent_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ CUtensorMap tmOut, const XentTile a, int *status) {
@@ -258,8 +290,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         item_at(a, i, tiles_m, tiles_n, mb, col, width);
         const uint32_t idesc = width == BN ? IDESC : IDESC_HALF;
         bool ok = true;
+        uint32_t first_kb = 0;  // of the running sum
         for (uint32_t kb = 0; kb < num_kb; ++kb) {
-          if (CHUNKED && kb && kb % CHUNK == 0) {  // the next accumulator takes over
+          if (EXACT && kb - first_kb == a.chunk) {  // the next accumulator takes over
+            first_kb = kb;
             commit(&tfull[acc]);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
@@ -285,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int ks = 0; ks < BK / 16; ++ks) {
             const uint64_t as = desc_add(ad, ks * 32), bs = desc_add(bd, ks * (B_MN ? 2048 : 32));
-            const uint32_t accum = ((CHUNKED ? kb % CHUNK : kb) | (uint32_t)ks) != 0 ? 1u : 0u;
+            const uint32_t accum = kb != first_kb || ks != 0 ? 1u : 0u;
             if constexpr (PAIR) tc_mma_f16_ss_pair(tmem_base + acc * BN, as, bs, idesc, accum);
             else tc_mma_f16_ss(tmem_base + acc * BN, as, bs, idesc, accum);
           }
@@ -317,6 +351,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t first = col + sub * 128;  // this warp's first column
       const uint32_t end = min(a.V, col + width);
       const bool live_row = row < a.T;
+      // nothing of the tile is this warp's (EXACT dlogit has zeros behind its rows)
+      const bool none = first >= end || row0 >= (!FWD && EXACT ? XENT_EXACT_ROWS : a.T);
       const int32_t target = live_row && a.target ? __ldcg(a.target + row) : -1;
       // the target's column within this warp's 128, or beyond them
       const uint32_t hit_col =
@@ -324,7 +360,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       float g = 0.0f, lse2 = 0.0f;
       if constexpr (!FWD) {
         if (live_row && (uint32_t)target < a.vocab) {
-          g = a.scale * (a.dloss ? __ldcg(a.dloss + row) : 1.0f);
+          const bool shared = a.common ? __ldcg(a.common + 1) != 0.0f : false;
+          g = shared ? 1.0f : a.scale * (a.dloss ? __ldcg(a.dloss + row) : 1.0f);
           lse2 = __ldcg(a.lse + row) * 1.44269504f;
         }
       }
@@ -339,13 +376,58 @@ __global__ void __launch_bounds__(THREADS, 1)
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       };
-      if constexpr (CHUNKED) {
+      // 32 logits in powers of two less lse2 to dlogit in bf16, and, EXACT, to
+      // what the rounding left
+      auto to_dlogit = [&](const uint64_t (&t)[16], uint32_t at, uint32_t *out, uint32_t *rest) {
+        float d[32];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          f2unpack(t[j], d[2 * j], d[2 * j + 1]);
+          d[2 * j] = ex2(d[2 * j]);
+          d[2 * j + 1] = ex2(d[2 * j + 1]);
+        }
+        if (at < 32u) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (at == (uint32_t)j) d[j] -= 1.0f;
+        }
+        const uint64_t g2 = f2pack(g, g);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float x, y;
+          f2unpack(f2mul(f2pack(d[2 * j], d[2 * j + 1]), g2), x, y);
+          const uint32_t both = pack2_16<false>(x, y);
+          out[j] = live ? both : 0u;
+          if constexpr (EXACT)
+            rest[j] = live ? pack2_16<false>(x - __uint_as_float(both << 16),
+                                             y - __uint_as_float(both & 0xFFFF0000u))
+                           : 0u;
+        }
+      };
+      // 32 rows x 64 columns of dlogit (128 bytes a row) from column c0
+      auto put = [&](const uint32_t (&w)[32], uint32_t c0, uint32_t to_row) {
+        uint8_t *stage_c = smem + C::OFF_C + ew * EPI_BUF;
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4 *>(stage_c + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+              make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmOut, stage_c, (int32_t)c0, (int32_t)to_row);
+          tma_store_commit();
+        }
+      };
+      const uint64_t c2 = f2pack(a.c, a.c), l2 = f2pack(-lse2, -lse2);
+      if constexpr (EXACT) {
         uint64_t v[64];  // pairs of columns
 #pragma unroll
         for (int j = 0; j < 64; ++j) v[j] = 0ull;
         bool ok = true;
 #pragma unroll 1
-        for (uint32_t kb = 0; kb < num_kb; kb += CHUNK) {
+        for (uint32_t kb = 0; kb < num_kb; kb += a.chunk) {
           if (!mbar_wait(&tfull[acc], acc_phase, status)) {
             *abort_flag = 1;
             ok = false;
@@ -355,6 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           // 16 columns at a time: 32 more registers would not fit
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
+            if (none) break;
             uint32_t r[16];
             tmem_ld_32x32b_x16(tmem_base + tq + acc * BN + sub * 128 + k * 16, r);
             tc_wait_ld16(r);
@@ -366,26 +449,30 @@ __global__ void __launch_bounds__(THREADS, 1)
           release();
         }
         if (!ok) break;
-        if (first < end) {
-          if (hit_col < 128u) {
-            float h = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              float x, y;
-              f2unpack(v[j], x, y);
-              if (hit_col == 2u * j) h = x;
-              if (hit_col == 2u * j + 1) h = y;
-            }
-            a.hit[row] = h * a.scale;
-          }
-          const uint64_t c2 = f2pack(a.c, a.c);
+        if (none) continue;
+        if constexpr (FWD) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = f2mul(v[j], c2);
+          if (hit_col < 128u) a.hit[row] = pick_logit(v, hit_col, a.apart);
           mask_logits(v, first, end);
           float m = -INFINITY, s = 0.0f;
           fold_logits(v, m, s);
-          if (live_row)
-            a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);
+          if (live_row) a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (first + k * 64 >= end) break;
+            uint32_t out[32], rest[32];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint64_t t[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) t[j] = f2fma(v[k * 32 + h * 16 + j], c2, l2);
+              to_dlogit(t, hit_col - (k * 64 + h * 32), out + h * 16, rest + h * 16);
+            }
+            put(out, first + k * 64, row0);
+            put(rest, first + k * 64, row0 + XENT_EXACT_ROWS);
+          }
         }
         continue;
       }
@@ -396,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
       const uint32_t taddr = tmem_base + tq + acc * BN + sub * 128;
       if constexpr (FWD) {
-        if (first < end) {
+        if (!none) {
           float m = -INFINITY, s = 0.0f;
 #pragma unroll 1
           for (int k = 0; k < 4; ++k) {
@@ -405,70 +492,34 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t r[32];
             tmem_ld_32x32b_x32(taddr + k * 32, r);
             tc_wait_ld(r);
-            if (hit_col - k * 32 < 32u) {
-              float h = 0.0f;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (hit_col - k * 32 == (uint32_t)j) h = __uint_as_float(r[j]);
-              a.hit[row] = h * a.scale;
-            }
-            const uint64_t c2 = f2pack(a.c, a.c);
             uint64_t v[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
               v[j] = f2mul(f2pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2);
+            if (hit_col - k * 32 < 32u) a.hit[row] = pick_logit(v, hit_col - k * 32, false);
             mask_logits(v, cs, end);
             fold_logits(v, m, s);
           }
           if (live_row) a.part[(size_t)(first / 128) * a.T + row] = make_float2(m, s);
         }
       } else {
-        uint8_t *stage_c = smem + C::OFF_C + ew * EPI_BUF;
 #pragma unroll 1
-        for (int k = 0; k < 2; ++k) {  // 64 columns: 128 bytes of bf16
+        for (int k = 0; k < 2; ++k) {
           const uint32_t cs = first + k * 64;
-          if (cs >= end) break;
+          if (none || cs >= end) break;
           uint32_t out[32];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t r[32];
             tmem_ld_32x32b_x32(taddr + k * 64 + h * 32, r);
             tc_wait_ld(r);
-            float d[32];
-            const uint64_t c2 = f2pack(a.c, a.c), l2 = f2pack(-lse2, -lse2);
+            uint64_t t[16];
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              f2unpack(f2fma(f2pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), c2, l2), d[j],
-                       d[j + 1]);
-              d[j] = ex2(d[j]);
-              d[j + 1] = ex2(d[j + 1]);
-            }
-            const uint32_t at = hit_col - (k * 64 + h * 32);
-            if (at < 32u) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (at == (uint32_t)j) d[j] -= 1.0f;
-            }
-            const uint64_t g2 = f2pack(g, g);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float x, y;
-              f2unpack(f2mul(f2pack(d[2 * j], d[2 * j + 1]), g2), x, y);
-              out[h * 16 + j] = live ? pack2_16<false>(x, y) : 0u;
-            }
+            for (int j = 0; j < 16; ++j)
+              t[j] = f2fma(f2pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2, l2);
+            to_dlogit(t, hit_col - (k * 64 + h * 32), out + h * 16, nullptr);
           }
-          if (lane == 0) tma_store_wait_read<0>();
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4 *>(stage_c + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0 && row0 < a.T) {
-            tma_store_2d(&tmOut, stage_c, (int32_t)cs, (int32_t)row0);
-            tma_store_commit();
-          }
+          put(out, cs, row0);
         }
       }
       release();
@@ -492,25 +543,37 @@ __device__ __forceinline__ void fold_pair(float2 &x, float2 y) {
   x.x = top;
 }
 
-// lse and loss of row t from its folded pair.
+// lse and loss of row t from its folded pair.  APART: the pair leaves a live
+// target out.  With h its logit and d = log2 of the others' sum less h, the loss is
+// log(1 + 2^d): it keeps its digits where the target takes nearly all of the
+// probability, and lse - h would lose them.
+template <bool APART>
 __device__ __forceinline__ void finish_row(uint32_t t, float2 x, const float *hit,
                                            const int32_t *target, float *loss, float *lse, uint32_t V,
                                            int *status) {
-  const float l = (x.x + log2f(x.y)) * 0.693147181f;
-  if (lse) lse[t] = l;
-  if (loss) {
-    const int32_t y = target[t];
-    float v = 0.0f;
-    if (y >= 0) {
-      if ((uint32_t)y < V) {
-        v = l - hit[t];
+  const float ln2 = 0.693147181f, nan = __int_as_float(0x7fc00000), more = log2f(x.y);
+  const int32_t y = loss ? target[t] : -1;
+  float l = (x.x + more) * ln2, v = 0.0f;
+  if (y >= 0) {
+    if ((uint32_t)y < V) {
+      // the maximum less the target's logit first: one near the other cancels
+      const float h = hit[t], d = (x.x - h) + more;
+      if (APART) {
+        // equal ones may be infinite: then d is NaN, and so is the loss, but not lse
+        const float others = x.x + more, both = h == others ? ln2 : log1pf(exp2f(-fabsf(d)));
+        l = fmaxf(h, others) * ln2 + both;
+        // an infinite logit of the target: inf - inf
+        v = d > 0.0f ? d * ln2 + both : d == d && h < INFINITY ? both : nan;
       } else {
-        v = __int_as_float(0x7fc00000);
-        bwpp_report(status, BWPP_CUDA_ERR_ARG);
+        v = d * ln2;
       }
+    } else {
+      v = nan;
+      bwpp_report(status, BWPP_CUDA_ERR_ARG);
     }
-    loss[t] = v;
   }
+  if (lse) lse[t] = l;
+  if (loss) loss[t] = v;
 }
 
 // Many rows, 32 a block: lane = row, warp w folds the row's pairs w, w + warps,
@@ -530,7 +593,7 @@ __global__ void __launch_bounds__(32 * COMBINE_WARPS)
   __syncthreads();
   if (warp || t >= T) return;
   for (int w = 1; w < COMBINE_WARPS; ++w) fold_pair(x, got[w][lane]);
-  finish_row(t, x, hit, target, loss, lse, V, status);
+  finish_row<false>(t, x, hit, target, loss, lse, V, status);
 }
 
 // Few rows: a block a row, its threads share the pairs.
@@ -551,18 +614,18 @@ __global__ void __launch_bounds__(FEW_THREADS)
   __syncthreads();
   if (threadIdx.x) return;
   for (int w = 1; w < FEW_THREADS / 32; ++w) fold_pair(x, got[w]);
-  finish_row(t, x, hit, target, loss, lse, V, status);
+  finish_row<true>(t, x, hit, target, loss, lse, V, status);
 }
 
 bool g_smem_set[16][64] = {};
 int g_pairs[16][64] = {};  // resident CTA pairs per device (0: not asked yet)
 
-template <bool B_MN, bool PAIR, bool FWD, bool CHUNKED>
+template <bool B_MN, bool PAIR, bool FWD, bool EXACT>
 int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
            const XentTile &a) {
   using C = Cfg<PAIR>;
-  auto kern = xent_tc_kernel<B_MN, PAIR, FWD, CHUNKED>;
-  const int v = (B_MN ? 1 : 0) + (PAIR ? 2 : 0) + (FWD ? 4 : 0) + (CHUNKED ? 8 : 0), dev = ctx->device;
+  auto kern = xent_tc_kernel<B_MN, PAIR, FWD, EXACT>;
+  const int v = (B_MN ? 1 : 0) + (PAIR ? 2 : 0) + (FWD ? 4 : 0) + (EXACT ? 8 : 0), dev = ctx->device;
   if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: device index >= 64");
   if (!g_smem_set[v][dev]) {
     const int rc = bwpp_check_cuda(
@@ -620,17 +683,28 @@ int launch(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const
                          FWD ? "xent logits" : "xent dlogit");
 }
 
-template <bool FWD, bool CHUNKED>
+template <bool PAIR, bool FWD, bool EXACT>
+int launch_layout(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
+                  const XentTile &a, bool vocab_major) {
+  return vocab_major ? launch<false, PAIR, FWD, EXACT>(ctx, tx, tw, to, a)
+                     : launch<true, PAIR, FWD, EXACT>(ctx, tx, tw, to, a);
+}
+
+// CTA pairs for more than 128 rows: a pair's second CTA would otherwise have
+// rows past T only.
+template <bool FWD, bool EXACT>
 int launch_any(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
                const XentTile &a, bool vocab_major) {
-  if (a.T > (uint32_t)BM) {  // a pair's second CTA would otherwise have rows past T only
-    const int rc = vocab_major ? launch<false, true, FWD, CHUNKED>(ctx, tx, tw, to, a)
-                               : launch<true, true, FWD, CHUNKED>(ctx, tx, tw, to, a);
+  if (a.T > (uint32_t)BM) {
+    const int rc = launch_layout<true, FWD, EXACT>(ctx, tx, tw, to, a, vocab_major);
     if (rc != BWPP_CUDA_ERR_UNSUPPORTED) return rc;
   }
-  return vocab_major ? launch<false, false, FWD, CHUNKED>(ctx, tx, tw, to, a)
-                     : launch<true, false, FWD, CHUNKED>(ctx, tx, tw, to, a);
+  return launch_layout<false, FWD, EXACT>(ctx, tx, tw, to, a, vocab_major);
 }
+
+// K blocks of a sum (see EXACT).  At one token, V = 16384, D = 2048, chunks of two
+// and of four take the same 15.5 us, of one 15.7.
+uint32_t chunk_of(uint32_t T) { return T > XENT_EXACT_ROWS ? 16 : 2; }
 
 // Rows of x in a load.  Few rows are loaded in a box of their own size (whole
 // eights, a swizzle atom): the tile's other rows keep what shared memory holds,
@@ -666,14 +740,18 @@ int bwpp_xent_stats_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_
   a.target = target;
   a.part = part;
   a.hit = hit;
+  const bool few = o.T <= XENT_EXACT_ROWS;
+  a.apart = few;
   a.vocab = o.vocab;
-  return o.D > CHUNK * BK ? launch_any<true, true>(ctx, tx, tw, tx, a, o.vocab_major)
-                          : launch_any<true, false>(ctx, tx, tw, tx, a, o.vocab_major);
+  a.chunk = chunk_of(o.T);
+  return few || o.D > a.chunk * BK
+             ? launch_any<true, true>(ctx, tx, tw, tx, a, o.vocab_major)
+             : launch_any<true, false>(ctx, tx, tw, tx, a, o.vocab_major);
 }
 
 int bwpp_xent_combine_launch(BwppCudaCtx *ctx, const float2 *part, uint32_t nparts, const float *hit,
                              const int32_t *target, float *loss, float *lse, uint32_t T, uint32_t V) {
-  const bool few = T <= 32;
+  const bool few = T <= XENT_EXACT_ROWS;
   return bwpp_check_cuda(
       ctx,
       bwpp_launch_dependent(few ? xent_combine_few_kernel : xent_combine_kernel,
@@ -683,12 +761,15 @@ int bwpp_xent_combine_launch(BwppCudaCtx *ctx, const float2 *part, uint32_t npar
 }
 
 int bwpp_xent_dlogit_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32_t *target,
-                            const float *lse, const float *dloss, uint16_t *dlogit, uint32_t ld) {
+                            const float *lse, const float *dloss, const float *common,
+                            uint16_t *dlogit, uint32_t ld) {
+  const bool exact = o.T <= XENT_EXACT_ROWS;
   CUtensorMap tx, tw, to;
   int rc = operand_maps(ctx, o, &tx, &tw);
   if (!rc)
-    rc = bwpp_make_tmap_2d(ctx, &to, dlogit, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, o.V, o.T,
-                           (uint64_t)ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = bwpp_make_tmap_2d(ctx, &to, dlogit, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, o.V,
+                           exact ? 2 * XENT_EXACT_ROWS : o.T, (uint64_t)ld * 2, 64, 32,
+                           CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
   XentTile a{};
   a.T = o.T;
@@ -701,6 +782,9 @@ int bwpp_xent_dlogit_launch(BwppCudaCtx *ctx, const XentOperands &o, const int32
   a.target = target;
   a.lse = lse;
   a.dloss = dloss;
+  a.common = common;
+  a.chunk = chunk_of(o.T);
   a.vocab = o.vocab;
-  return launch_any<false, false>(ctx, tx, tw, to, a, o.vocab_major);
+  return exact ? launch_layout<false, false, true>(ctx, tx, tw, to, a, o.vocab_major)
+               : launch_any<false, false>(ctx, tx, tw, to, a, o.vocab_major);
 }

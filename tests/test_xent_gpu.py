@@ -47,12 +47,18 @@ def formula(x, w, target, scale):
 
 
 def within(got, want, tol):
-    err = (got.double() - want).abs()
+    most = torch.finfo(got.dtype).max  # a sum beyond it is an infinity
+    beyond = want.abs() > most
+    assert torch.equal(got[beyond].double(), want[beyond] * float("inf"))
+    err = torch.where(beyond, 0.0, (got.double() - want).abs())
     assert bool((err <= tol).all()), (float((err - tol).max()), float(err.max()))
 
 
-def check(ctx, T, V, D, vocab_major, scale=1.0, bf16=1, pad=0, seed=0, ones=False, sharp=2.0, ignored=0.2):
+def check(ctx, T, V, D, vocab_major, scale=1.0, bf16=1, pad=0, seed=0, ones=False, sharp=2.0, ignored=0.2,
+          step=HALF, each_dloss=None):
     x, w, target, dloss, xs, ws = make(T, V, D, vocab_major, seed + T + V, ignored, sharp, pad)
+    if each_dloss is not None:
+        dloss = torch.where(target >= 0, torch.full_like(dloss, each_dloss), dloss)
     ldw = ws.shape[1]
     scale = float(torch.tensor(scale))
     loss, lse = (torch.full((T,), float("nan"), device="cuda") for _ in range(2))
@@ -75,7 +81,7 @@ def check(ctx, T, V, D, vocab_major, scale=1.0, bf16=1, pad=0, seed=0, ones=Fals
     d = p.clone()
     d[torch.arange(T, device="cuda"), target.long().clamp(min=0)] -= 1.0
     d, off = d * g[:, None] * scale, p * (g * abs(scale) * (4 * dl + 2.0**-20 * (wlse.abs() + 2)))[:, None]
-    each = off + HALF * d.abs()
+    each = off + step * d.abs()
     xd, wd = x.double(), w.double()
     out = HALF if bf16 else 2.0**-24
     pieces = 66  # 2^-22 of a sum of magnitudes for each piece, at most 64 here
@@ -200,6 +206,64 @@ def test_one_output_at_a_time(ctx):
     ctx.xent_bwd(xs, ws, target, lse, dloss, None, d2, *a, grads_bf16=1)
     ctx.sync()
     assert torch.equal(loss, l1) and torch.equal(lse, l2) and torch.equal(dx, d1) and torch.equal(dw, d2)
+
+
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("T,V,D", [(1, 1000, 64), (3, 1237, 100), (1, 5000, 300), (64, 900, 64), (50, 3000, 136)])
+def test_few_rows_keep_more_than_one_rounding(ctx, T, V, D, vocab_major):
+    """Up to 64 rows, dlogit is two bf16: half a step of half a step is left."""
+    check(ctx, T, V, D, vocab_major, bf16=0, step=HALF * HALF, ignored=0.0 if T == 1 else 0.2)
+
+
+@pytest.mark.parametrize("each_dloss", [1.0 / 300.0, 1e-30, 3e38, 0.0, -0.7])
+def test_rows_that_share_their_dloss(ctx, each_dloss):
+    """A mean loss: one dloss for all live rows, any others in ignored ones."""
+    check(ctx, 300, 700, 72, 1, each_dloss=each_dloss, bf16=0, scale=0.25)
+    check(ctx, 300, 700, 72, 0, each_dloss=each_dloss, scale=0.25)
+
+
+def test_a_dloss_that_is_not_a_number_stays_in_its_row(ctx):
+    T, V, D = 200, 300, 64
+    x, w, target, dloss, xs, ws = make(T, V, D, 1, 13, ignored=0.0)
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, D, w_vocab_major=1)
+    dx = torch.empty(T, D, device="cuda")
+    for bad in (float("nan"), float("inf")):
+        for rest in (0.5, None):  # one value in the other rows, or their own
+            g = dloss.clone() if rest is None else torch.full_like(dloss, rest)
+            g[77] = bad
+            ctx.xent_bwd(xs, ws, target, lse, g, dx, None, T, V, D, D, D, D, D, w_vocab_major=1)
+            ctx.sync()
+            off = ~torch.isfinite(dx).all(1)
+            assert bool(off[77]) and int(off.sum()) == 1
+
+
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("T,V,D", [(1, 1000, 64), (3, 700, 100), (2, 1300, 1000), (60, 1000, 2500), (64, 999, 64)])
+def test_loss_of_sure_targets(ctx, T, V, D, vocab_major):
+    """Few rows whose target has nearly all of the probability: losses down to
+    1e-7 keep their digits."""
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    w = (torch.randn(V, D, device="cuda", generator=g) / D**0.5).bfloat16()
+    target = torch.randint(0, V, (T,), device="cuda", generator=g)
+    a = 15 + 8 * torch.rand(T, 1, device="cuda", generator=g)
+    x = (a * w[target].float() / w[target].float().square().sum(1, keepdim=True)).bfloat16()
+    ws = w if vocab_major else w.t().contiguous()
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    ctx.xent_fwd(x, ws, target.int(), loss, lse, T, V, D, D, ws.shape[1], w_vocab_major=vocab_major)
+    ctx.sync()
+    logits = x.double() @ w.double().t()
+    hit = logits.gather(1, target[:, None])[:, 0]
+    logits.scatter_(1, target[:, None], float("-inf"))
+    others = torch.logsumexp(logits, 1)
+    want = torch.log1p((others - hit).exp())
+    assert float(want.min()) < 1e-3
+    # d loss = p' d(others - hit): the logits' errors (a truncation of 2^-22 per 16
+    # of up to 256 and per sum of 128, of the terms' magnitudes), roundings of numbers in
+    # powers of two up to 1.45 hit, and a few of the loss itself
+    dl = (min(D, 256) // 16 + D // 128 + 2) * 2.0**-22 * (x.double().abs() @ w.double().abs().t()).amax(1)
+    tol = want * (2 * dl + 2.0**-21 * (hit.abs() + others.abs() + 4))
+    within(loss, want, tol)
 
 
 def test_gradient_by_differences(ctx):
