@@ -2,8 +2,8 @@
 // the epilogue: they never reach memory.
 //
 // logit[t, v] = scale sum_d x[t, d] W[v, d], in tiles of 256 rows x 256
-// vocabulary columns (a CTA pair, cta_group::2) or 128 x 256 (one CTA, at most
-// 128 rows).  Persistent, warp-specialised like the GEMM (gemm.cu): warp 0
+// vocabulary columns (a CTA pair, cta_group::2) or 128 x 256 (one CTA, where a
+// pair would have too few rows).  Persistent, warp-specialised like the GEMM (gemm.cu): warp 0
 // feeds a ring of operand stages by TMA, one thread of warp 1 issues
 // tcgen05.mma, warps 2..9 drain the accumulator; two TMEM accumulators, so the
 // epilogue of a tile runs beside the next tile's main loop.
@@ -690,12 +690,16 @@ int launch_layout(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw
                      : launch<true, PAIR, FWD, EXACT>(ctx, tx, tw, to, a);
 }
 
-// CTA pairs for more than 128 rows: a pair's second CTA would otherwise have
-// rows past T only.
+// CTA pairs, which load each column of W once for 256 rows (T 8192, V 32000, D 1024:
+// 360 us, 425 with one CTA a tile; T 512: 31.9, 34.2), but for an odd number of
+// blocks of 128 rows that is so small that the half of a pair without rows costs
+// more: T 300, V 32000, D 4096: 110 us in pairs, 97 without; T 896, D 4096: 197 and
+// 180 forward, 174 and 179 dlogit.
 template <bool FWD, bool EXACT>
 int launch_any(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, const CUtensorMap &to,
                const XentTile &a, bool vocab_major) {
-  if (a.T > (uint32_t)BM) {
+  const uint32_t blocks = (a.T + BM - 1) / BM;
+  if (blocks % 2 == 0 || blocks > (FWD ? 7u : 5u)) {
     const int rc = launch_layout<true, FWD, EXACT>(ctx, tx, tw, to, a, vocab_major);
     if (rc != BWPP_CUDA_ERR_UNSUPPORTED) return rc;
   }
