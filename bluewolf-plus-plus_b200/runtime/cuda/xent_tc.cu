@@ -36,6 +36,7 @@ constexpr int EPI_WARPS = 8;
 constexpr int EPI_BUF = 32 * 128;   // 32 rows x 64 bf16
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t TMEM_COLS = 2 * BN;
+constexpr uint32_t MANY_CHUNK = 16;  // K blocks of a sum, many rows (see EXACT)
 
 template <bool PAIR>
 struct Cfg {
@@ -200,6 +201,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t workers = PAIR ? cluster_count_x() : gridDim.x;
   const uint32_t tiles_m = (a.T + C::TILE_M - 1) / C::TILE_M, tiles_n = (a.V + BN - 1) / BN;
   const uint32_t num_kb = (a.D + BK - 1) / BK;
+  const uint32_t chunk = PAIR ? MANY_CHUNK : a.chunk;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         bool ok = true;
         uint32_t first_kb = 0;  // of the running sum
         for (uint32_t kb = 0; kb < num_kb; ++kb) {
-          if (EXACT && kb - first_kb == a.chunk) {  // the next accumulator takes over
+          if (EXACT && kb - first_kb == chunk) {  // the next accumulator takes over
             first_kb = kb;
             commit(&tfull[acc]);
             acc ^= 1;
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < 64; ++j) v[j] = 0ull;
         bool ok = true;
 #pragma unroll 1
-        for (uint32_t kb = 0; kb < num_kb; kb += a.chunk) {
+        for (uint32_t kb = 0; kb < num_kb; kb += chunk) {
           if (!mbar_wait(&tfull[acc], acc_phase, status)) {
             *abort_flag = 1;
             ok = false;
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if constexpr (FWD) {
 #pragma unroll
           for (int j = 0; j < 64; ++j) v[j] = f2mul(v[j], c2);
-          if (hit_col < 128u) a.hit[row] = pick_logit(v, hit_col, a.apart);
+          if (hit_col < 128u) a.hit[row] = pick_logit(v, hit_col, !PAIR && a.apart);
           mask_logits(v, first, end);
           float m = -INFINITY, s = 0.0f;
           fold_logits(v, m, s);
@@ -708,7 +710,7 @@ int launch_any(BwppCudaCtx *ctx, const CUtensorMap &tx, const CUtensorMap &tw, c
 
 // K blocks of a sum (see EXACT).  At one token, V = 16384, D = 2048, chunks of two
 // and of four take the same 15.5 us, of one 15.7.
-uint32_t chunk_of(uint32_t T) { return T > XENT_EXACT_ROWS ? 16 : 2; }
+uint32_t chunk_of(uint32_t T) { return T > XENT_EXACT_ROWS ? MANY_CHUNK : 2; }
 
 // Rows of x in a load.  Few rows are loaded in a box of their own size (whole
 // eights, a swizzle atom): the tile's other rows keep what shared memory holds,
