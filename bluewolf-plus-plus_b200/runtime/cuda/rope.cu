@@ -45,12 +45,24 @@ constexpr int batch_of(bool one_vector) { return one_vector ? 8 : 4; }
 // A thread owns one slot (VEC pairs, or VEC columns behind R) of one token in
 // heads lane, lane + lanes, ... of q and then of k: its sines and cosines are
 // computed once for all of them, behind the first loads.
-template <int DT, int VEC, bool IL>
+//
+// SINGLE: at most one head of each, loaded together: q's and k's transfers are all
+// that a thread has in flight, so its registers are few and the threads many.  The
+// turns come from shared memory: a warp's slots are different addresses of the
+// constant bank, read one after another for each head.  (89658 tokens, one head of
+// 196 each, bf16: 105 us as one batch of q and one of k, 78 together, 46 with shared
+// turns; with many heads a thread, shared turns were 1-8% slower.)
+template <int DT, int VEC, bool IL, bool SINGLE>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
   using T = typename Elem<DT>::type;
   constexpr bool ONE = IL && VEC > 1;  // a vector holds both sides of its pairs
   constexpr int PAIRS = ONE ? VEC / 2 : VEC;
   constexpr int kBatch = batch_of(ONE);
+  __shared__ uint64_t shared_turns[SINGLE ? BWPP_CUDA_ROPE_MAX_PAIRS : 1];
+  if constexpr (SINGLE) {
+    for (uint32_t i = threadIdx.x; i < a.table.pairs; i += kThreads) shared_turns[i] = a.table.turns[i];
+    __syncthreads();
+  }
   dependent_wait();
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   if (id >= a.units) return;
@@ -79,13 +91,60 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     const float up = a.table.amplitude, side = a.p.inverse ? -up : up;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
-      const uint64_t turn = (uint64_t)pos * a.table.turns[slot * PAIRS + i];
+      const uint64_t turn = (uint64_t)pos * (SINGLE ? shared_turns[slot * PAIRS + i] : a.table.turns[slot * PAIRS + i]);
       sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &sn[i], &cs[i]);
       cs[i] *= up;
       sn[i] *= side;
     }
     ready = true;
   };
+  if constexpr (SINGLE) {
+    const uint32_t side = c1 - c0;
+    auto at = [&](int head_major, uint32_t heads, size_t ld) {  // of this thread's head
+      return c0 + (head_major ? ((size_t)b * heads + lane) * a.seq * ld + s * ld
+                              : t * ld + (size_t)lane * a.p.head_dim);
+    };
+    const T *from[2] = {static_cast<const T *>(a.q) + at(a.p.head_major_in, a.p.heads_q, a.p.ldq),
+                        static_cast<const T *>(a.k) + at(a.p.head_major_in, a.p.heads_k, a.p.ldk)};
+    T *into[2] = {static_cast<T *>(a.qo) + at(a.p.head_major_out, a.p.heads_q, a.p.ldq_out),
+                  static_cast<T *>(a.ko) + at(a.p.head_major_out, a.p.heads_k, a.p.ldk_out)};
+    const bool in[2] = {lane < a.p.heads_q, lane < a.p.heads_k};
+    Raw<DT, VEC> x[2], y[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (in[u]) x[u].load(from[u]);
+      if (in[u] && two) y[u].load(from[u] + side);
+    }
+    if (turns) angles();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!in[u]) continue;
+      if (turns) {
+        float v[VEC];
+        if constexpr (ONE) {
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) {
+            const float x0 = x[u].get(2 * i), x1 = x[u].get(2 * i + 1);
+            v[2 * i] = x0 * cs[i] - x1 * sn[i];
+            v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+          }
+        } else {
+          float w[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float x0 = x[u].get(i), x1 = y[u].get(i);
+            v[i] = x0 * cs[i] - x1 * sn[i];
+            w[i] = x1 * cs[i] + x0 * sn[i];
+          }
+          y[u].set(w);
+          y[u].store(into[u] + side);
+        }
+        x[u].set(v);
+      }
+      x[u].store(into[u]);
+    }
+    return;
+  }
   auto pass = [&](const void *from, void *into, uint32_t heads, size_t ldi, size_t ldo) {
     const size_t di = a.p.head_major_in ? (size_t)a.seq * ldi : a.p.head_dim;
     const size_t dn = a.p.head_major_out ? (size_t)a.seq * ldo : a.p.head_dim;
@@ -150,11 +209,14 @@ int rope_launch(BwppCudaCtx *ctx, RopeArgs &a) {
   a.slots = a.turn_slots + (in_place ? 0 : (p.head_dim - R) / VEC);
   // A thread per head and slot for few tokens, where latency counts; a thread
   // takes a batch of heads of q and of k where that still leaves 1024 threads
-  // per SM (4084 tokens x 32 heads x 128 fp32: 33.7 us without, 23.2 with).
+  // per SM (4084 tokens x 32 heads x 128 fp32: 33.7 us without, 23.2 with).  One or
+  // two heads are no batch (65536 tokens x 2 + 2 heads of 128, interleaved bf16: 38.5
+  // us as one, 29 as SINGLE; 4 + 1 heads: 39.8 and 52.9).
   const uint32_t kBatch = batch_of(pairs_in_one);
   a.lanes = p.heads_q > p.heads_k ? p.heads_q : p.heads_k;
-  if ((uint64_t)p.tokens * a.slots * a.lanes > (uint64_t)ctx->num_sms * 1024 * kBatch)
+  if (a.lanes > 2 && (uint64_t)p.tokens * a.slots * a.lanes > (uint64_t)ctx->num_sms * 1024 * kBatch)
     a.lanes = (a.lanes + kBatch - 1) / kBatch;
+  const bool single = a.lanes >= p.heads_q && a.lanes >= p.heads_k;
   const uint64_t per = (uint64_t)a.slots * a.lanes;
   const uint64_t most = (1u << 30) / per;  // tokens of a launch: unit ids stay in 31 bits
   if (most == 0)
@@ -164,11 +226,10 @@ int rope_launch(BwppCudaCtx *ctx, RopeArgs &a) {
     a.token0 = (uint32_t)t0;
     a.units = (uint32_t)(n * per);
     const uint32_t grid = (a.units + kThreads - 1) / kThreads;
+    auto kernel = single ? (p.interleaved ? rope_kernel<DT, VEC, true, true> : rope_kernel<DT, VEC, false, true>)
+                         : (p.interleaved ? rope_kernel<DT, VEC, true, false> : rope_kernel<DT, VEC, false, false>);
     const int rc = bwpp_check_cuda(
-        ctx,
-        bwpp_launch_dependent(p.interleaved ? rope_kernel<DT, VEC, true> : rope_kernel<DT, VEC, false>,
-                              dim3(grid), dim3(kThreads), 0, ctx->stream, a),
-        "rope");
+        ctx, bwpp_launch_dependent(kernel, dim3(grid), dim3(kThreads), 0, ctx->stream, a), "rope");
     if (rc) return rc;
   }
   return BWPP_CUDA_OK;

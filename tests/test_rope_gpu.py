@@ -73,6 +73,28 @@ def test_rope(ctx, dtype, interleaved, tokens, hq, hk, hd, R):
                 assert bool(torch.isnan(o).all())
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("tokens,hq,hk,hd,R", [(40000, 5, 3, 64, 32), (30000, 3, 11, 10, 10), (20000, 24, 24, 96, 64),
+                                               (90000, 1, 1, 20, 12), (70000, 2, 1, 34, 34), (30000, 0, 2, 128, 128)])
+def test_many_tokens(ctx, dtype, interleaved, tokens, hq, hk, hd, R):
+    """Batches of heads, and one or two heads a token; per sequence of 10000 and
+    from token-major to head-major."""
+    t, seq = TYPES[dtype], 10000
+    g = torch.Generator(device="cuda").manual_seed(tokens + hd)
+    q = torch.randn(tokens, max(hq, 1), hd, device="cuda", generator=g).to(t)
+    k = torch.randn(tokens, max(hk, 1), hd, device="cuda", generator=g).to(t)
+    qo, ko = torch.full_like(q, float("nan")), torch.full_like(k, float("nan"))
+    call(ctx, dtype)(q, k, qo, ko, bwpp.rope_table(R), tokens, hq, hk, hd, max(hq, 1) * hd, max(hk, 1) * hd, hd, hd,
+                     seq=seq, pos0=3, interleaved=interleaved, head_major_out=1)
+    ctx.sync()
+    pos = 3 + torch.arange(tokens, device="cuda") % seq
+    for o, x, h in ((qo, q, hq), (ko, k, hk)):
+        if h:
+            o = o.view(tokens // seq, h, seq, hd).transpose(1, 2).reshape(tokens, h, hd)
+            check(o, x, pos, frequencies(R), interleaved)
+
+
 @pytest.mark.parametrize("scaling,factor,amp", [("linear", 4.0, 1.0), ("base", 8.0, 1.0), ("parts", 16.0, 1.277)])
 def test_scaled_for_long_contexts(ctx, scaling, factor, amp):
     g = torch.Generator(device="cuda").manual_seed(2)
