@@ -17,8 +17,8 @@
 // 0 * NaN would reach all of dW).  A target >= V reports BWPP_CUDA_ERR_ARG at
 // the next bwpp_cuda_sync, its loss is NaN and its row is ignored.
 //
-// TMA wants row pitches of 16 bytes: x or W with others go through packed copies
-// in scratch (a piece of W at a time), gradients are written with plain stores.
+// TMA wants row pitches of 16 bytes: x, W or gradients with others go through
+// packed copies in scratch (a piece of W at a time).
 #include <math.h>
 
 #include "bwpp_cuda_internal.cuh"
@@ -31,8 +31,8 @@ using bwpp_elem::aligned_to;
 
 constexpr int kThreads = 256;
 
-// Copies from rows of any pitch into rows of 16 bytes in scratch, for the
-// operands that TMA does not take as they are.  A warp takes
+// Copies between rows of any pitch and rows of 16 bytes in scratch, for the
+// operands and results that TMA does not take as they are.  A warp takes
 // kSpan consecutive elements of a row.  (A thread with eight elements of its
 // own, as 2-byte accesses 16 bytes apart, took 60 us for 1001 x 10007 bf16.)
 constexpr uint32_t kSpan = 256;
@@ -134,6 +134,29 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// Results from rows of 16 bytes in scratch into rows of any pitch.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    unpack_rows_kernel(const T *src, T *dst, uint32_t rows, uint32_t cols,
+                       size_t ld_src, size_t ld_dst) {
+  dependent_wait();
+  const uint32_t spans = (cols + kSpan - 1) / kSpan;
+  const uint32_t i = (blockIdx.x * kThreads + threadIdx.x) / 32, lane = threadIdx.x & 31;
+  if (i >= rows * spans) return;
+  const uint32_t r = i / spans, c0 = (i - r * spans) * kSpan;
+  T v[kSpan / 32];
+#pragma unroll
+  for (uint32_t k = 0; k < kSpan / 32; ++k) {
+    const uint32_t c = c0 + k * 32 + lane;
+    if (c < cols) v[k] = src[r * ld_src + c];
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kSpan / 32; ++k) {
+    const uint32_t c = c0 + k * 32 + lane;
+    if (c < cols) dst[r * ld_dst + c] = v[k];
+  }
+}
+
 int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t rows, uint32_t cols,
               uint32_t ld_src, uint32_t ld_dst, const int32_t *target, uint32_t V,
               uint32_t live_rows = 0xffffffffu, uint32_t again = 0, Common common = Common{}) {
@@ -153,6 +176,25 @@ int pack_rows(BwppCudaCtx *ctx, const uint16_t *src, uint16_t *dst, uint32_t row
         "xent pack");
     if (rc) return rc;
     common.out = nullptr;  // the first launch found it, from all rows
+  }
+  return BWPP_CUDA_OK;
+}
+
+template <typename T>
+int unpack_rows(BwppCudaCtx *ctx, const void *src, void *dst, uint32_t rows, uint32_t cols,
+                uint32_t ld_src, uint32_t ld_dst) {
+  const uint32_t spans = (cols + kSpan - 1) / kSpan;
+  const uint32_t most = (1u << 25) / spans;
+  for (uint32_t r0 = 0; r0 < rows; r0 += most) {
+    const uint32_t n = rows - r0 < most ? rows - r0 : most;
+    const int rc = bwpp_check_cuda(
+        ctx,
+        bwpp_launch_dependent(unpack_rows_kernel<T>,
+                              dim3((n * spans + kThreads / 32 - 1) / (kThreads / 32)), dim3(kThreads), 0,
+                              ctx->stream, static_cast<const T *>(src) + (size_t)r0 * ld_src,
+                              static_cast<T *>(dst) + (size_t)r0 * ld_dst, n, cols, ld_src, ld_dst),
+        "xent unpack");
+    if (rc) return rc;
   }
   return BWPP_CUDA_OK;
 }
@@ -188,8 +230,8 @@ uint32_t parts_that_fit(uint64_t rows, uint64_t ld) {
 // where dx is read and written back once; 2659 with all of them kept).
 // Forward: the whole vocabulary, or about 2^25 weights at a time where they
 // are packed.
-Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool backward,
-                 bool stage_dx) {
+Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool backward, bool stage_dx,
+                 bool stage_dw) {
   Layout l{};
   l.dp = up8(p.D);
   l.piece = backward ? piece_of((1ull << 27) / p.T, p.V)
@@ -205,6 +247,7 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
     at += up256(bytes);
     return here;
   };
+  const size_t es = p.grads_bf16 ? 2 : 4;
   if (pack_x || backward) l.x = take((size_t)(backward ? l.k_rows : p.T) * l.dp * 2);
   if (pack_w) l.w = take((size_t)l.piece * l.dp * 2);
   if (!backward) {
@@ -214,8 +257,9 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
     l.common = take(2 * sizeof(float));
     l.dlogit = take((size_t)l.k_rows * l.piece * 2);
     if (stage_dx) l.dx = take((size_t)l.dx_parts * l.dx_rows * l.dp * 4);
-    if (l.dw_parts > 1)
-      l.dw = take((size_t)l.dw_parts * l.dw_rows * (p.w_vocab_major ? l.dp : l.piece) * 4);
+    if (stage_dw || l.dw_parts > 1)
+      l.dw = take((size_t)l.dw_parts * l.dw_rows * (p.w_vocab_major ? l.dp : l.piece) *
+                  (l.dw_parts > 1 ? 4 : es));
   }
   l.total = at;
   return l;
@@ -256,7 +300,7 @@ extern "C" {
 
 size_t bwpp_cuda_xent_workspace_size(const BwppCudaXentParams *p, int backward) {
   if (!p || p->T == 0 || p->V == 0 || p->D == 0) return 0;
-  return layout_of(*p, true, p->ldw % 8 != 0, backward != 0, true).total + BWPP_OP_SCRATCH_PAD;
+  return layout_of(*p, true, p->ldw % 8 != 0, backward != 0, true, true).total + BWPP_OP_SCRATCH_PAD;
 }
 
 int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,
@@ -270,7 +314,7 @@ int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   if (!x || !w || (loss && !target) || (!loss && !lse))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent fwd: NULL buffer");
   const bool pack_x = needs_pack(x, p.ldx), pack_w = needs_pack(w, p.ldw);
-  const Layout l = layout_of(p, pack_x, pack_w, false, false);
+  const Layout l = layout_of(p, pack_x, pack_w, false, false, false);
   uint8_t *scratch;
   rc = bwpp_op_scratch(ctx, l.total, "xent fwd", &scratch);
   if (rc) return rc;
@@ -320,7 +364,8 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent bwd: NULL buffer");
   const bool pack_w = needs_pack(w, p.ldw);
   auto tma_out = [&](const void *q, uint32_t ld) { return (size_t)ld * es % 16 == 0 && aligned_to(q, 16); };
-  const Layout probe = layout_of(p, true, pack_w, true, true);
+  const bool dx_out = dx && tma_out(dx, p.lddx), stage_dw = dw && !tma_out(dw, p.lddw);
+  const Layout probe = layout_of(p, true, pack_w, true, true, true);
   const uint32_t piece = probe.piece, pieces = (p.V - 1) / piece + 1;
   const bool vm = p.w_vocab_major != 0;
   const uint32_t ld_w = pack_w ? (vm ? probe.dp : piece) : p.ldw;
@@ -355,9 +400,9 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
   const bool exact = p.T <= XENT_EXACT_ROWS;
   // dx is summed in scratch, unless the caller's rows take it: all of it in one
   // piece, or fp32 sums
-  const bool one_sum = dx && dx_parts == 1 && !exact;
-  const bool direct = one_sum && (pieces == 1 || (!p.grads_bf16 && tma_out(dx, p.lddx)));
-  const Layout l = layout_of(p, true, pack_w, true, dx && !direct);
+  const bool one_sum = dx_out && dx_parts == 1 && !exact;
+  const bool direct = one_sum && (pieces == 1 || !p.grads_bf16);
+  const Layout l = layout_of(p, true, pack_w, true, dx && !direct, stage_dw);
   uint8_t *scratch;
   rc = bwpp_op_scratch(ctx, l.total, "xent bwd", &scratch);
   if (rc) return rc;
@@ -389,22 +434,23 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     px.ldc = to_user ? p.lddx : l.dp;
     px.bf16 = to_user && last && p.grads_bf16;
     px.factor = to_user && last ? common : nullptr;
-    px.plain = to_user && !tma_out(dx, p.lddx);
     uint8_t *user_w =
         dw ? static_cast<uint8_t *>(dw) + (vm ? (size_t)v0 * p.lddw : (size_t)v0) * es : nullptr;
-    const bool own_w = dw_parts > 1;  // dW's part goes through scratch
+    const bool own_w = stage_dw || dw_parts > 1;  // dW's part goes through scratch
     pw.a = vm ? dlogit : xp;
     pw.b = vm ? xp : dlogit;
     pw.c = own_w ? static_cast<void *>(scratch + l.dw) : static_cast<void *>(user_w);
     pw.ldc = own_w ? (vm ? l.dp : piece) : p.lddw;
     pw.bf16 = p.grads_bf16 && dw_parts == 1;
     pw.factor = dw_parts == 1 ? common : nullptr;
-    pw.plain = !own_w && !tma_out(dw, p.lddw);
     rc = bwpp_xent_grad_launch(ctx, dx ? &px : nullptr, dw ? &pw : nullptr, dx_parts, dw_parts);
     if (!rc && dw && dw_parts > 1)
       rc = bwpp_xent_sum_parts_launch(ctx, static_cast<const float *>(pw.c), dw_parts,
                                       (size_t)l.dw_rows * pw.ldc, 0, common, user_w, pw.M, pw.N, pw.ldc,
                                       p.lddw, p.grads_bf16);
+    else if (!rc && stage_dw)
+      rc = p.grads_bf16 ? unpack_rows<uint16_t>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw)
+                        : unpack_rows<float>(ctx, pw.c, user_w, pw.M, pw.N, pw.ldc, p.lddw);
     if (rc) return rc;
   }
   if (dx && !one_sum) {

@@ -45,7 +45,6 @@ struct XentProduct {
   uint32_t M, N, K, lda, ldb, ldc;
   bool a_mn, b_mn;
   bool bf16;          // C bf16, else fp32
-  bool plain;         // C's rows are of any pitch and address (one part)
   const float *factor; // device scalar that multiplies C, or NULL
   bool accumulate;    // add fp32 rows `add` (pitch ld_add; may be C)
   const void *add;

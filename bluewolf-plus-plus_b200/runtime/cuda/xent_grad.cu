@@ -57,8 +57,6 @@ struct Product {
   uint32_t ld_add;
   const float *factor;      // multiplies C, or NULL
   uint32_t bf16;            // C is bf16, else fp32
-  void *plain;              // C (pitch ldc) where TMA does not take its rows, else NULL
-  uint32_t ldc;
 };
 
 struct Maps {
@@ -161,7 +159,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!work.product[i].items) continue;
       prefetch_tmap(&work.maps[i].a);
       prefetch_tmap(&work.maps[i].b);
-      if (!work.product[i].plain) prefetch_tmap(&work.maps[i].c);
+      prefetch_tmap(&work.maps[i].c);
     }
   }
   if (warp == 1) {
@@ -361,28 +359,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < 8; ++j)
           *reinterpret_cast<uint4 *>(stage_c + lane * 128 + ((j ^ (lane & 7)) << 4)) =
               make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
-        if (p.plain) {
-          // A row at a time, neighbouring lanes on neighbouring columns.  (1001 x
-          // 10007 bf16: 7 us more than by TMA, with 4-byte stores as well; by TMA
-          // into scratch and a copy, 9 us more)
-          __syncwarp();
-          const uint32_t rows = row0 < M ? min(32u, M - row0) : 0;
-#pragma unroll 8
-          for (uint32_t j = 0; j < rows; ++j) {
-            const size_t at = (size_t)(row0 + j) * p.ldc + c0 + lane;
-            const uint8_t *from = stage_c + j * 128;
-            auto word = [&](uint32_t byte) { return from + (((byte >> 4) ^ (j & 7)) << 4) + (byte & 15); };
-            if (!out16) {
-              if (c0 + lane < N)
-                static_cast<float *>(p.plain)[at] = *reinterpret_cast<const float *>(word(4 * lane));
-              continue;
-            }
-            uint16_t *to = static_cast<uint16_t *>(p.plain) + at;
-            if (c0 + lane < N) to[0] = *reinterpret_cast<const uint16_t *>(word(2 * lane));
-            if (c0 + 32 + lane < N) to[32] = *reinterpret_cast<const uint16_t *>(word(64 + 2 * lane));
-          }
-          continue;
-        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0 && row0 < M) {
@@ -545,19 +521,18 @@ int make_product(BwppCudaCtx *ctx, const XentProduct &s, uint32_t tile_m, uint32
   p.ld_add = s.ld_add;
   p.factor = s.factor;
   p.bf16 = s.bf16 ? 1 : 0;
-  p.plain = s.plain ? s.c : nullptr;
-  p.ldc = s.ldc;
   const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * parts;
   if (items >= 0x80000000ull) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: too many tiles");
   p.items = (uint32_t)items;
   int rc = operand_map(ctx, &m.a, s.a, s.a_mn, s.M, s.K, s.lda, BM);
   if (!rc) rc = operand_map(ctx, &m.b, s.b, s.b_mn, s.N, s.K, s.ldb, 64);
-  if (rc || s.plain) return rc;
   const uint64_t rows = parts > 1 ? (uint64_t)parts * s.part_rows : s.M;
-  return s.bf16 ? bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s.N, rows,
+  if (!rc)
+    rc = s.bf16 ? bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s.N, rows,
                                     (uint64_t)s.ldc * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B)
                 : bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, s.N, rows,
                                     (uint64_t)s.ldc * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+  return rc;
 }
 
 // Row blocks that go through the columns together: the workers cover about two
