@@ -372,7 +372,8 @@ int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
 /* dx = scale * dlogit W, dw = scale * dlogit^T x, overwritten, with dlogit[t, v]
  * = dloss[t] (exp(logit - lse[t]) - [v == target[t]]); lse as the forward wrote
  * it; dloss [T] or NULL (ones); dx or dw may be NULL.  dlogit is rounded to
- * bf16 for the tensor cores, so fp32 gradients carry that rounding too. */
+ * bf16 for the tensor cores (twice, value and rest, for up to 64 rows), so fp32
+ * gradients carry that rounding too. */
 int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,
                             const int32_t *target, const float *lse, const float *dloss, void *dx,
                             void *dw, const BwppCudaXentParams *params);
