@@ -312,7 +312,8 @@ extern "C" {
 
 size_t bwpp_cuda_xent_workspace_size(const BwppCudaXentParams *p, int backward) {
   if (!p || p->T == 0 || p->V == 0 || p->D == 0) return 0;
-  return layout_of(*p, true, p->ldw % 8 != 0, backward != 0, true, true).total + BWPP_OP_SCRATCH_PAD;
+  // every copy that a call may need: which it makes depends on addresses as well
+  return layout_of(*p, true, true, backward != 0, true, true).total + BWPP_OP_SCRATCH_PAD;
 }
 
 int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,

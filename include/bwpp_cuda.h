@@ -363,7 +363,9 @@ typedef struct {
   float scale;
 } BwppCudaXentParams;
 
-/* Scratch bytes of a call whose buffers are 16-byte aligned. */
+/* Scratch bytes of a call, wherever its buffers lie: packed copies of x and of a
+ * piece of W are counted, although a call makes them only where addresses or
+ * pitches are no multiples of 16 bytes. */
 size_t bwpp_cuda_xent_workspace_size(const BwppCudaXentParams *params, int backward);
 /* loss (with target) or lse may be NULL. */
 int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,

@@ -95,6 +95,20 @@ def test_xent_workspace_size():
     assert bwpp.xent_workspace_size(T, V, D, D, V) < T * V * 4
 
 
+@pytest.mark.parametrize("backward", [0, 1])
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("T,V,D", [(1, 1000, 64), (150, 1112, 136), (777, 4096, 1024)])
+def test_xent_workspace_size_covers_odd_addresses(T, V, D, vocab_major, backward):
+    """W at an address that is not 16-byte aligned is packed, whatever its pitch:
+    one piece of it (all of these) is part of the size."""
+    ldw = D if vocab_major else V
+    size = bwpp.xent_workspace_size(T, V, D, D, ldw, vocab_major, backward, 1)
+    assert size == bwpp.xent_workspace_size(T, V, D, D, ldw + 1, vocab_major, backward, 1)
+    # what is kept besides: x, and the pairs and hits or dlogit
+    rest = T * D * 2 + (T * V * 2 if backward else (V + 127) // 128 * T * 8 + T * 4)
+    assert size >= rest + V * D * 2
+
+
 def test_struct_layouts():
     assert C.sizeof(bwpp.XentParams) == 40
     assert C.sizeof(bwpp.RopeTable) == 8 + 8 * bwpp.ROPE_MAX_PAIRS

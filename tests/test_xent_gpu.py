@@ -387,3 +387,60 @@ def test_captured_and_replayed(ctx, T):
     del graph
     c.close()
     k.close()
+
+
+@pytest.mark.parametrize("captured", [0, 1])
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("T,V,D", [(3, 1000, 64), (150, 1112, 136), (300, 2104, 256)])
+def test_odd_addresses(T, V, D, vocab_major, bf16, captured):
+    """x, w, dx and dw one element off their 16 bytes, alone and together, with
+    pitches that TMA takes, in a workspace of the queried size: the results of
+    aligned buffers bit for bit, nothing written around them."""
+    stream = torch.cuda.Stream()
+    c = bwpp.Ctx(0, stream.cuda_stream)
+    x, w, target, dloss, xs, ws = make(T, V, D, vocab_major, 17)
+    ldw = ws.shape[1]
+    need = max(bwpp.xent_workspace_size(T, V, D, D, ldw, vocab_major, b, bf16) for b in (0, 1))
+    room = torch.empty(need, dtype=torch.uint8, device="cuda")
+    c.set_workspace(room, need)
+    t = torch.bfloat16 if bf16 else torch.float32
+
+    def at(like, off, dtype):
+        buf = torch.full((like.numel() + 16,), 7.0, device="cuda", dtype=dtype)
+        return buf, buf[off:off + like.numel()].view(like.shape)
+
+    def run(odd):
+        x1, w1 = at(xs, odd[0], xs.dtype)[1], at(ws, odd[1], ws.dtype)[1]
+        x1.copy_(xs)
+        w1.copy_(ws)
+        bufs = [at(xs, odd[2], t), at(ws, odd[3], t)]
+        (bx, dx), (bw, dw) = bufs
+        loss, lse = torch.full((T,), 7.0, device="cuda"), torch.full((T,), 7.0, device="cuda")
+
+        def calls():
+            c.xent_fwd(x1, w1, target, loss, lse, T, V, D, D, ldw, w_vocab_major=vocab_major)
+            c.xent_bwd(x1, w1, target, lse, dloss, dx, dw, T, V, D, D, ldw, D, ldw, w_vocab_major=vocab_major,
+                       grads_bf16=bf16)
+
+        torch.cuda.synchronize()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                calls()
+            graph.replay()
+            graph.replay()
+            torch.cuda.synchronize()
+            del graph
+        else:
+            calls()
+        c.sync()
+        for (buf, _), off, n in ((bufs[0], odd[2], dx.numel()), (bufs[1], odd[3], dw.numel())):
+            assert bool((buf[:off] == 7.0).all()) and bool((buf[off + n:] == 7.0).all())
+        return loss, lse, dx, dw
+
+    want = run((0, 0, 0, 0))
+    assert bool(torch.isfinite(want[2].float()).all()) and bool(torch.isfinite(want[3].float()).all())
+    for odd in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 3, 5, 7)):
+        assert all(torch.equal(a, b) for a, b in zip(run(odd), want)), odd
+    c.close()
