@@ -277,11 +277,18 @@ Layout layout_of(const BwppCudaXentParams &p, bool pack_x, bool pack_w, bool bac
   return l;
 }
 
+// Sizes that the calls take: rounded up to tiles they stay below 2^31, as the
+// 32-bit indices and TMA's coordinates need.
+bool sizes_fit(const BwppCudaXentParams &p) {
+  constexpr uint32_t most = 0x7ffffe00u;
+  return p.V > 0 && p.D > 0 && p.V <= most && p.D <= most && p.T <= most;
+}
+
 int check(BwppCudaCtx *ctx, const BwppCudaXentParams *p) {
   if (!p) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: NULL params");
-  if (p->V == 0 || p->D == 0 || p->V > 0x7ffffe00u || p->T > 0x7ffffe00u)
+  if (!sizes_fit(*p))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG,
-                          "xent: V and D must be positive, V and T at most 2^31 - 512");
+                          "xent: V and D must be positive, T, V and D at most 2^31 - 512");
   if (p->ldx < p->D || p->ldw < (p->w_vocab_major ? p->D : p->V))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: leading dim smaller than row");
   if (!isfinite(p->scale)) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "xent: scale is not finite");
@@ -311,7 +318,7 @@ bool needs_pack(const void *base, uint32_t ld) { return ld % 8 != 0 || !aligned_
 extern "C" {
 
 size_t bwpp_cuda_xent_workspace_size(const BwppCudaXentParams *p, int backward) {
-  if (!p || p->T == 0 || p->V == 0 || p->D == 0) return 0;
+  if (!p || p->T == 0 || !sizes_fit(*p)) return 0;
   // every copy that a call may need: which it makes depends on addresses as well
   return layout_of(*p, true, true, backward != 0, true, true).total + BWPP_OP_SCRATCH_PAD;
 }

@@ -349,7 +349,7 @@ int bwpp_cuda_cast_f32_bf16(BwppCudaCtx *ctx, const float *src, uint16_t *dst,
  *   loss[t] = lse[t] - logit[t, target[t]]
  * W[v, d] = w_vocab_major ? w[v*ldw + d] : w[d*ldw + v].  x and w are bf16
  * bits, products accumulate in fp32 on the tensor cores; loss and lse are
- * fp32.  Any sizes and pitches; row pitches that are no multiple of 8, or
+ * fp32.  Any sizes up to 2^31 - 512 and pitches; row pitches that are no multiple of 8, or
  * addresses that are not 16-byte aligned, cost packed copies in scratch.
  * A negative target ignores its row (loss 0, zero gradient, whatever its x
  * holds).  A target >= V is an error that the next bwpp_cuda_sync reports
@@ -365,7 +365,7 @@ typedef struct {
 
 /* Scratch bytes of a call, wherever its buffers lie: packed copies of x and of a
  * piece of W are counted, although a call makes them only where addresses or
- * pitches are no multiples of 16 bytes. */
+ * pitches are no multiples of 16 bytes.  0 for no rows and for sizes that are refused. */
 size_t bwpp_cuda_xent_workspace_size(const BwppCudaXentParams *params, int backward);
 /* loss (with target) or lse may be NULL. */
 int bwpp_cuda_xent_fwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t *w,

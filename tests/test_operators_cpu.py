@@ -3,6 +3,8 @@ against 64-bit arithmetic, configurations that are refused, scratch sizes, and
 calls without a context."""
 import ctypes as C
 import math
+import subprocess
+import sys
 from fractions import Fraction
 
 import pytest
@@ -107,6 +109,19 @@ def test_xent_workspace_size_covers_odd_addresses(T, V, D, vocab_major, backward
     # what is kept besides: x, and the pairs and hits or dlogit
     rest = T * D * 2 + (T * V * 2 if backward else (V + 127) // 128 * T * 8 + T * 4)
     assert size >= rest + V * D * 2
+
+
+@pytest.mark.parametrize("T,V,D", [(4, 4, 2**32 - 1), (4, 4, 2**31 - 511), (2**32 - 1, 4, 4), (2**32 - 1, 4, 2**32 - 1),
+                                   (4, 2**32 - 1, 4), (4, 0, 4), (4, 4, 0)])
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("backward", [0, 1])
+def test_xent_workspace_size_of_sizes_that_are_refused(T, V, D, vocab_major, backward):
+    """No scratch, and no arithmetic that wraps: a process of its own, as a
+    division by a size that wrapped to zero ends it."""
+    code = (f"import sys; sys.path[:0] = {sys.path!r}; import bwpp; "
+            f"print(bwpp.xent_workspace_size({T}, {V}, {D}, {D}, {D if vocab_major else V}, {vocab_major}, {backward}))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert (r.returncode, r.stdout.strip()) == (0, "0"), r
 
 
 def test_struct_layouts():

@@ -444,3 +444,18 @@ def test_odd_addresses(T, V, D, vocab_major, bf16, captured):
     for odd in ((1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 3, 5, 7)):
         assert all(torch.equal(a, b) for a, b in zip(run(odd), want)), odd
     c.close()
+
+
+@pytest.mark.parametrize("T,V,D", [(4, 4, 2**32 - 1), (4, 4, 2**31 - 511), (2**32 - 1, 4, 4), (4, 2**32 - 1, 4)])
+@pytest.mark.parametrize("vocab_major", [0, 1])
+def test_sizes_past_31_bits_are_refused(ctx, T, V, D, vocab_major):
+    z = torch.zeros(16, device="cuda").bfloat16()
+    f = torch.zeros(16, device="cuda")
+    ldw = D if vocab_major else V
+    for call in (lambda: ctx.xent_fwd(z, z, f.int(), f, f, T, V, D, D, ldw, w_vocab_major=vocab_major),
+                 lambda: ctx.xent_bwd(z, z, f.int(), f, None, z, z, T, V, D, D, ldw, D, ldw, w_vocab_major=vocab_major,
+                                      grads_bf16=1)):
+        with pytest.raises(bwpp.BwppError) as e:
+            call()
+        assert e.value.status == bwpp.ERR_ARG
+    ctx.sync()
