@@ -780,14 +780,17 @@ bool make_chunks(BwppCudaCtx *ctx, uint32_t rows, uint32_t gate_rows, uint32_t p
   return n < (1u << 31) - 2;
 }
 
+constexpr uint32_t kMostSize = 0x7fffffffu;
+
 int check_args(BwppCudaCtx *ctx, const BwppCudaJunctionParams *p, bool has_b, bool has_gate,
                bool has_y) {
   if (!p) return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: NULL params");
   if (p->ldh < p->cols || (has_b && p->ldb < p->cols) || (has_gate && p->ldgate < p->cols) ||
       (has_y && p->ldy < p->cols))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: leading dim smaller than row");
-  if (p->rows > 0x7fffffffu)
-    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: more than 2^31 - 1 rows");
+  // a column index steps past the row's end by up to a block's threads, in 32 bits
+  if (p->rows > kMostSize || p->cols > kMostSize)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "junction: more than 2^31 - 1 rows or columns");
   return BWPP_CUDA_OK;
 }
 
@@ -1067,7 +1070,7 @@ extern "C" {
 
 size_t bwpp_cuda_junction_bwd_workspace_size(BwppCudaCtx *ctx, uint32_t rows, uint32_t cols,
                                              uint32_t gate_rows) {
-  if (!ctx || rows == 0 || cols == 0) return 0;
+  if (!ctx || rows == 0 || cols == 0 || rows > kMostSize || cols > kMostSize) return 0;
   Chunks k;
   if (!make_chunks(ctx, rows, gate_rows ? gate_rows : rows, kMaxPerSm, k)) return 0;
   return 2 * (size_t)k.chunks * cols * sizeof(float) + BWPP_OP_SCRATCH_PAD;

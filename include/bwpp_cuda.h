@@ -451,7 +451,8 @@ int bwpp_cuda_rope_f32(BwppCudaCtx *ctx, const float *q, const float *k, float *
  * The stream h, the gains [cols] and the gate are fp32; b and y have the
  * call's type.  Gains and gate may be NULL (1), y NULL (not computed).  Row r
  * takes gate row r / gate_rows: 1 a gate per token, the sequence length one
- * per sequence, rows (or 0) one for all.  h_out may be h. */
+ * per sequence, rows (or 0) one for all.  h_out may be h.  At most 2^31 - 1 rows
+ * and columns. */
 typedef struct {
   uint32_t rows, cols;
   uint32_t ldh, ldb, ldy, ldgate;  /* pitches of h/h_out/dh_out/dh, b/db, y/dy, gate/dgate */
@@ -471,7 +472,7 @@ int bwpp_cuda_junction_fwd_f16(BwppCudaCtx *ctx, const float *h, const uint16_t 
                                const float *gain_post, const float *gate, const float *gain_pre,
                                float *h_out, uint16_t *y, const BwppCudaJunctionParams *params);
 
-/* Scratch bytes of the backward. */
+/* Scratch bytes of the backward; 0 for no rows and for sizes that are refused. */
 size_t bwpp_cuda_junction_bwd_workspace_size(BwppCudaCtx *ctx, uint32_t rows, uint32_t cols,
                                              uint32_t gate_rows);
 /* From the forward's h_out and b, the gradient dh_out of h_out (NULL: zero) and

@@ -333,3 +333,15 @@ def test_captured_replayed_and_the_workspace(ctx):
     assert e.value.status == bwpp.ERR_NOMEM
     del graph
     c.close()
+
+
+@pytest.mark.parametrize("cols", [2**31, 2**32 - 1])
+def test_rows_of_2_31_columns_are_refused(ctx, cols):
+    z = torch.zeros(16, device="cuda")
+    for call in (lambda: ctx.junction_fwd_f32(z, z, None, None, None, z, z, 1, cols),
+                 lambda: ctx.junction_bwd_f32(z, z, None, None, None, z, z, z, z.clone(), None, None, None, 1, cols)):
+        with pytest.raises(bwpp.BwppError) as e:
+            call()
+        assert e.value.status == bwpp.ERR_ARG
+    assert bwpp.load().bwpp_cuda_junction_bwd_workspace_size(ctx.handle, 4, cols, 0) == 0
+    ctx.sync()
