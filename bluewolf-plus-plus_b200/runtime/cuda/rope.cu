@@ -246,6 +246,9 @@ int rope(BwppCudaCtx *ctx, const void *q, const void *k, void *qo, void *ko,
   if (table->pairs == 0 || table->pairs > BWPP_CUDA_ROPE_MAX_PAIRS || R > p.head_dim)
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: table of %u pairs for head_dim %u",
                           table->pairs, p.head_dim);
+  // a thread's head index steps past the last head, in 32 bits
+  if (p.heads_q > 0x7fffffffu || p.heads_k > 0x7fffffffu)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: more than 2^31 - 1 heads");
   if (p.tokens == 0 || (p.heads_q == 0 && p.heads_k == 0)) return BWPP_CUDA_OK;
   if ((p.heads_q && (!q || !qo)) || (p.heads_k && (!k || !ko)))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_ARG, "rope: NULL buffer");

@@ -241,3 +241,14 @@ def test_refusals(ctx):
         assert e.value.status == bwpp.ERR_ARG, b
     ctx.rope_f32(**{**ok, "tokens": 0})
     ctx.sync()
+
+
+@pytest.mark.parametrize("heads", [2**31, 2**32 - 1])
+def test_2_31_heads_are_refused(ctx, heads):
+    """Head major, where no pitch grows with the heads."""
+    x = torch.zeros(16, device="cuda")
+    for hq, hk in ((heads, 0), (0, heads), (1, heads)):
+        with pytest.raises(bwpp.BwppError) as e:
+            ctx.rope_f32(x, x, x, x, bwpp.rope_table(2), 1, hq, hk, 2, 2, 2, 2, 2, head_major_in=1, head_major_out=1)
+        assert e.value.status == bwpp.ERR_ARG
+    ctx.sync()
