@@ -996,6 +996,8 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
       rc = bwpp_check_cuda(ctx, cudaMemsetAsync(dgain_post, 0, sizeof(float) * p->cols, s), "memset");
     if (!rc && dgain_pre)
       rc = bwpp_check_cuda(ctx, cudaMemsetAsync(dgain_pre, 0, sizeof(float) * p->cols, s), "memset");
+    if (!rc && dgate && p->gate_rows == 0)  // one gate for all rows: there without rows too
+      rc = bwpp_check_cuda(ctx, cudaMemsetAsync(dgate, 0, sizeof(float) * p->cols, s), "memset");
     return rc;
   }
   // b is read where the norm's, the gate's or the gain's gradient needs it

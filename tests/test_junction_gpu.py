@@ -345,3 +345,17 @@ def test_rows_of_2_31_columns_are_refused(ctx, cols):
         assert e.value.status == bwpp.ERR_ARG
     assert bwpp.load().bwpp_cuda_junction_bwd_workspace_size(ctx.handle, 4, cols, 0) == 0
     ctx.sync()
+
+
+@pytest.mark.parametrize("gate_rows", [0, 3])
+def test_no_rows_leave_no_gradient(ctx, gate_rows):
+    """One gate for all rows has a gradient of zero where there are no rows; a
+    gate for every three rows has none."""
+    z = torch.zeros(1, 16, device="cuda")
+    gate, dgate = torch.ones(1, 24, device="cuda"), torch.full((1, 24), 5.0, device="cuda")
+    gains = torch.full((2, 16), 5.0, device="cuda")
+    ctx.junction_bwd_f32(z, z, None, gate, None, z, z, None, None, gains[0], dgate, gains[1], 0, 16,
+                         gate_rows=gate_rows, ldgate=24)
+    ctx.sync()
+    assert not bool(gains.any())
+    assert bool((dgate[0, 16:] == 5.0).all()) and bool((dgate[0, :16] == (5.0 if gate_rows else 0.0)).all())
