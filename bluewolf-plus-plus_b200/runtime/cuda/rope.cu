@@ -315,6 +315,7 @@ int bwpp_cuda_rope_table(BwppCudaRopeTable *out, const BwppCudaRopeConfig *cfg) 
     case BWPP_CUDA_ROPE_BASE:
       if (R == 2) return BWPP_CUDA_ERR_ARG;  // one pair does not depend on the base
       base *= pow(cfg->factor, (double)R / (R - 2));
+      if (!(base > 0) || !isfinite(base)) return BWPP_CUDA_ERR_ARG;
       break;
     case BWPP_CUDA_ROPE_PARTS:
       if (!(cfg->context > 0) || !isfinite(cfg->context) || !(cfg->high > cfg->low) ||

@@ -64,6 +64,16 @@ def test_rope_table_refusals(kw):
     assert e.value.status == bwpp.ERR_ARG
 
 
+@pytest.mark.parametrize("kw", [dict(rotary_dim=4, base=1e200, factor=1e200), dict(rotary_dim=64, base=1e300, factor=1e10),
+                                dict(rotary_dim=4, base=1e-200, factor=1e-200)])
+def test_rope_table_of_a_base_out_of_range(kw):
+    """base * factor^(R / (R - 2)) overflows or vanishes: without an error all
+    pairs but the first would stand still, or turn by any amount."""
+    with pytest.raises(bwpp.BwppError) as e:
+        bwpp.rope_table(scaling="base", **kw)
+    assert e.value.status == bwpp.ERR_ARG
+
+
 def test_rope_table_null_and_unknown_scaling():
     lib = bwpp.load()
     cfg = bwpp.RopeConfig(8, 4, 10000.0, 1.0, 0.0, 1.0, 32.0, 1.0)
