@@ -261,6 +261,7 @@ def _ptr(t):
 # cost, and a value that does not fit its field is an error.
 _XENT = struct.Struct("@7I2if")       # XentParams
 _ROPE = struct.Struct("@9I5i")        # RopeParams
+_ROPE_CONFIG = struct.Struct("@Ii5df0d")  # RopeConfig
 _JUNCTION = struct.Struct("@7Ii4f")   # JunctionParams
 
 
@@ -469,14 +470,16 @@ class Ctx:
 
 def xent_workspace_size(T, V, D, ldx, ldw, w_vocab_major=0, backward=0, grads_bf16=0) -> int:
     """Scratch bytes of Ctx.xent_fwd (backward=0) or Ctx.xent_bwd (backward=1)."""
-    p = XentParams(T, V, D, ldx, ldw, 0, 0, int(w_vocab_major), int(grads_bf16), 1.0)
+    p = XentParams.from_buffer_copy(_XENT.pack(T, V, D, ldx, ldw, 0, 0, int(w_vocab_major),
+                                                    int(grads_bf16), 1.0))
     return load().bwpp_cuda_xent_workspace_size(C.byref(p), int(backward))
 
 
 def rope_table(rotary_dim, base=10000.0, scaling="none", factor=1.0, context=0.0, low=1.0, high=32.0,
                amplitude=1.0) -> RopeTable:
     """The rotary frequencies of one model configuration, for Ctx.rope_*."""
-    cfg = RopeConfig(rotary_dim, ROPE_SCALING[scaling], base, factor, context, low, high, amplitude)
+    cfg = RopeConfig.from_buffer_copy(_ROPE_CONFIG.pack(rotary_dim, ROPE_SCALING[scaling], base, factor, context,
+                                                        low, high, amplitude))
     table = RopeTable()
     rc = load().bwpp_cuda_rope_table(C.byref(table), C.byref(cfg))
     if rc != OK:

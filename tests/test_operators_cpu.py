@@ -156,3 +156,23 @@ def test_sizes_that_do_not_fit_their_field_are_errors():
         bwpp._JUNCTION.pack(1 << 32, *range(7), 1.0, 1.0, 0.0, 0.0)
     with pytest.raises(Exception):
         bwpp._ROPE.pack(*range(9), 1 << 31, 0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("at", range(5))
+@pytest.mark.parametrize("value", [1 << 32, (1 << 32) + 8, -1])
+def test_workspace_sizes_that_do_not_fit_their_field_are_errors(at, value):
+    sizes = [8] * 5
+    sizes[at] = value
+    with pytest.raises(Exception):
+        bwpp.xent_workspace_size(*sizes)
+
+
+@pytest.mark.parametrize("rotary_dim", [(1 << 32) + 8, -1])
+def test_rotary_dims_that_do_not_fit_their_field_are_errors(rotary_dim):
+    with pytest.raises(Exception):
+        bwpp.rope_table(rotary_dim)
+
+
+def test_packed_rope_config_is_the_struct():
+    cfg = bwpp.RopeConfig.from_buffer_copy(bwpp._ROPE_CONFIG.pack(1, 2, 3.0, 4.0, 5.0, 6.0, 7.0, 8.5))
+    assert [getattr(cfg, n) for n, _ in cfg._fields_] == [1, 2, 3.0, 4.0, 5.0, 6.0, 7.0, 8.5]
