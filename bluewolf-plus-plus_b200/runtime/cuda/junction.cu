@@ -854,75 +854,108 @@ int launch_fwd(BwppCudaCtx *ctx, const JunctionArgs &a) {
   return bwpp_check_cuda(ctx, rc, "junction fwd");
 }
 
-// How the backward takes a row width: CTAs per SM (as many as are resident:
-// 4055 x 1003 fp32 took 23.0 us with the 3 that fit, 26.8 with 4), and for rows
-// staged in shared memory the stages (else 0).
+// How the backward takes a row width: CTAs per SM, and for rows staged in shared
+// memory the stages (else 0) and the shared memory that a CTA asks for.
 struct Plan {
   uint32_t stages, per_sm, bytes;
 };
-template <int DT>
-Plan plan_bwd(const JunctionArgs &a) {
-  const uint32_t cols = a.p.cols;
-  const bool vec = vectors<DT>(a);
-  // threads of a block: 128 (VEC 8, or up to 128 columns), then a fourth of the
-  // columns up to 512; about 80 registers a thread, 128 in the widest
-  const uint32_t per = vec && cols <= 256 ? 4 : cols <= 128 ? 6 : cols <= 256 ? 12 : cols <= 512 ? 6
-                       : cols <= 1024 ? 3 : cols <= 4096 ? 1 : 2;
-  const Plan held{0, per, 0};
-  if (!vec || cols <= 256 || cols > 8192) return held;
-  Plan g{0, 0, 0};
-  const bool token = a.p.gate_rows == 1 && a.gate;
-  const uint32_t row = cols * (8 + (token ? 4 : 0) + 2 * (uint32_t)sizeof(typename Elem<DT>::type));
-  constexpr uint32_t sm = 220 * 1024;  // of an SM's 228 KB; 1 KB and the static part go with each CTA
-  // 16 warps per SM hide a row's two reductions (32768 x 2048 bf16: 323 us with
-  // one CTA of 8 warps, 205 with two, 218 with three, 227 with four; 8192 x 2560
-  // bf16: 115 us with one CTA of 16 warps, 77 with two of 8); two or more stages
-  // make no difference then.  Rows of two warps have less to do between their
-  // reductions: 32768 x 512 bf16 86 us with 8 CTAs, 76 with 10, 71 with the 12 whose
-  // registers fit.
-  const uint32_t want = cols <= 512 ? 12 : cols <= 1024 ? 4 : cols <= 4096 ? 2 : 1;
-  for (uint32_t per = want; per >= 1 && g.stages < 2; --per) {
-    g.per_sm = per;
-    g.stages = sm / per / row;
-  }
-  if (g.stages > (uint32_t)kMaxStages) g.stages = kMaxStages;
-  if (g.stages < 2) return held;
-  // A CTA asks for its whole share of shared memory: one more on an SM would
-  // leave another SM with one less, which happens when the kernel in front still
-  // holds SMs as these are placed (32768 x 2048 bf16: 263 us instead of 211).
-  g.bytes = sm / g.per_sm;
-  return g;
+
+// An instantiation of the staged kernel on a device.
+struct StagedFit {
+  bool known;
+  uint32_t by_regs;  // CTAs that an SM's registers and warps hold
+  uint32_t fixed;    // shared memory of a CTA besides what it asks for
+};
+StagedFit g_staged_fit[64][32] = {};
+constexpr uint32_t kSharedOfSm = 228 * 1024, kSharedOfCta = 227 * 1024;  // sm_100: 1 KB of a CTA is the system's
+constexpr uint32_t kSharedUnit = 128;                                   // in which it is given out
+
+// The instantiation for rows of `cols` columns: f(kernel, threads, its number).
+template <int DT, bool TOKEN, typename F>
+int with_staged(uint32_t cols, F f) {
+  constexpr int n = DT * 2 + (TOKEN ? 1 : 0);
+  if (cols <= 512) return f(junction_bwd_staged_kernel<DT, 2, 64, TOKEN>, 64, n);
+  if (cols <= 1024) return f(junction_bwd_staged_kernel<DT, 2, 128, TOKEN>, 128, n + 6);
+  if (cols <= 2048) return f(junction_bwd_staged_kernel<DT, 2, 256, TOKEN>, 256, n + 12);
+  if (cols <= 4096) return f(junction_bwd_staged_kernel<DT, 4, 256, TOKEN>, 256, n + 18);
+  return f(junction_bwd_staged_kernel<DT, 4, 512, TOKEN>, 512, n + 24);
 }
 
-bool g_staged_set[64][32] = {};
+// The plan of a staged row; stages 0 where two of them do not fit.
+template <int DT, bool TOKEN>
+int plan_staged(BwppCudaCtx *ctx, uint32_t cols, Plan &g) {
+  g = Plan{0, 0, 0};
+  if (ctx->device >= 64)
+    return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction: device index >= 64");
+  return with_staged<DT, TOKEN>(cols, [&](auto kern, int threads, int id) {
+    StagedFit &fit = g_staged_fit[ctx->device][id];
+    if (!fit.known) {
+      cudaFuncAttributes at;
+      int n = 0;
+      cudaError_t e = cudaFuncGetAttributes(&at, kern);
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0);
+      const uint32_t own = e == cudaSuccess ? ((uint32_t)at.sharedSizeBytes + kSharedUnit - 1) & ~(kSharedUnit - 1) : 0;
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedOfCta - own));
+      const int rc = bwpp_check_cuda(ctx, e, "junction smem attribute");
+      if (rc) return rc;
+      fit.by_regs = (uint32_t)n;
+      fit.fixed = kSharedOfSm - kSharedOfCta + own;
+      fit.known = true;
+    }
+    const uint32_t row = cols * (8 + (TOKEN ? 4 : 0) + 2 * (uint32_t)sizeof(typename Elem<DT>::type));
+    // 16 warps per SM hide a row's two reductions (32768 x 2048 bf16: 323 us with
+    // one CTA of 8 warps, 205 with two, 218 with three, 227 with four; 8192 x 2560
+    // bf16: 115 us with one CTA of 16 warps, 77 with two of 8); two or more stages
+    // make no difference then.  Rows of two warps have less to do between their
+    // reductions and take all the CTAs that are resident, 12 at most (32768 x 512
+    // bf16: 62.8 us with 12, 65.4 with 11, 60.1 with 10; x 384: 53.3, 57.2, 54.3).
+    // Chunks for more than are resident leave a second round that is nearly empty:
+    // planned as 12 where 11 fit, 32768 x 512 took 72.5 us, fp32 with a gate per token,
+    // where 10 fit, 8000 x 512 33.8 instead of 29.0.
+    const uint32_t want = cols <= 512 ? kMaxPerSm : cols <= 1024 ? 4 : cols <= 4096 ? 2 : 1;
+    for (uint32_t per = want < fit.by_regs ? want : fit.by_regs; per >= 1; --per) {
+      // A CTA asks for its whole share of shared memory: one more on an SM would
+      // leave another SM with one less, which happens when the kernel in front still
+      // holds SMs as these are placed (32768 x 2048 bf16: 263 us instead of 211).
+      const uint32_t bytes = (kSharedOfSm / per & ~(kSharedUnit - 1)) - fit.fixed;
+      if (bytes / row < 2) continue;
+      g.per_sm = per;
+      g.bytes = bytes;
+      g.stages = bytes / row < (uint32_t)kMaxStages ? bytes / row : (uint32_t)kMaxStages;
+      break;
+    }
+    return (int)BWPP_CUDA_OK;
+  });
+}
 
-template <int DT, int NV, int TPR, bool TOKEN>
-int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Plan &g, int id) {
-  auto kern = junction_bwd_staged_kernel<DT, NV, TPR, TOKEN>;
-  const int dev = ctx->device;
-  if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction: device index >= 64");
-  bool &set = g_staged_set[dev][id * 6 + DT * 2 + (TOKEN ? 1 : 0)];
-  if (!set) {
-    const int rc = bwpp_check_cuda(
-        ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024),
-        "junction smem attribute");
-    if (rc) return rc;
-    set = true;
+template <int DT>
+int plan_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, Plan &g) {
+  const uint32_t cols = a.p.cols;
+  const bool vec = vectors<DT>(a);
+  if (vec && cols > 256 && cols <= 8192) {
+    const int rc = a.p.gate_rows == 1 && a.gate ? plan_staged<DT, true>(ctx, cols, g)
+                                                : plan_staged<DT, false>(ctx, cols, g);
+    if (rc || g.stages) return rc;
   }
-  return bwpp_check_cuda(ctx,
-                         bwpp_launch_dependent(kern, dim3(chunks), dim3(TPR), g.bytes, ctx->stream, a,
-                                               g.stages, ctx->status_word),
-                         "junction bwd");
+  // threads of a block: 128 (VEC 8, or up to 128 columns), then a fourth of the
+  // columns up to 512; 72 to 80 registers a thread, 128 in the widest and with VEC 8.
+  // No more than are resident (4055 x 1003 fp32 took 23.0 us with the 3 that fit,
+  // 26.8 with 4)
+  const uint32_t per = vec && cols <= 256 ? 4 : cols <= 128 ? 6 : cols <= 256 ? 12 : cols <= 512 ? 6
+                       : cols <= 1024 ? 3 : cols <= 4096 ? 1 : 2;
+  g = Plan{0, per, 0};
+  return BWPP_CUDA_OK;
 }
 
 template <int DT, bool TOKEN>
-int launch_staged_any(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Plan &g) {
-  const uint32_t cols = a.p.cols;
-  if (cols <= 512) return launch_staged<DT, 2, 64, TOKEN>(ctx, a, chunks, g, 0);
-  if (cols <= 1024) return launch_staged<DT, 2, 128, TOKEN>(ctx, a, chunks, g, 1);
-  if (cols <= 2048) return launch_staged<DT, 2, 256, TOKEN>(ctx, a, chunks, g, 2);
-  if (cols <= 4096) return launch_staged<DT, 4, 256, TOKEN>(ctx, a, chunks, g, 3);
-  return launch_staged<DT, 4, 512, TOKEN>(ctx, a, chunks, g, 4);
+int launch_staged(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const Plan &g) {
+  return with_staged<DT, TOKEN>(a.p.cols, [&](auto kern, int threads, int) {
+    return bwpp_check_cuda(ctx,
+                           bwpp_launch_dependent(kern, dim3(chunks), dim3(threads), g.bytes, ctx->stream, a,
+                                                 g.stages, ctx->status_word),
+                           "junction bwd");
+  });
 }
 
 template <int DT>
@@ -930,8 +963,8 @@ int launch_bwd(BwppCudaCtx *ctx, const JunctionArgs &a, uint32_t chunks, const P
   const uint32_t cols = a.p.cols;
   cudaStream_t s = ctx->stream;
   if (g.stages)
-    return a.p.gate_rows == 1 && a.gate ? launch_staged_any<DT, true>(ctx, a, chunks, g)
-                                        : launch_staged_any<DT, false>(ctx, a, chunks, g);
+    return a.p.gate_rows == 1 && a.gate ? launch_staged<DT, true>(ctx, a, chunks, g)
+                                        : launch_staged<DT, false>(ctx, a, chunks, g);
   cudaError_t rc;
 #define BWPP_BWD(VEC, NV, TPR)                                                              \
   rc = bwpp_launch_dependent(junction_bwd_kernel<DT, VEC, NV, TPR>, dim3(chunks),           \
@@ -1022,7 +1055,9 @@ int junction_bwd(BwppCudaCtx *ctx, const float *h_out, const void *b, const floa
   a.db = db;
   const bool per_row = a.p.gate_rows == 1;
   a.dgate = per_row ? dgate : nullptr;
-  const Plan g = plan_bwd<DT>(a);
+  Plan g;
+  rc = plan_bwd<DT>(ctx, a, g);
+  if (rc) return rc;
   Chunks k;
   if (!make_chunks(ctx, a.p.rows, a.p.gate_rows, g.per_sm, k))
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction bwd: too many gate rows");

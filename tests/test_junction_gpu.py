@@ -359,3 +359,13 @@ def test_no_rows_leave_no_gradient(ctx, gate_rows):
     ctx.sync()
     assert not bool(gains.any())
     assert bool((dgate[0, 16:] == 5.0).all()) and bool((dgate[0, :16] == (5.0 if gate_rows else 0.0)).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("gate_rows", [0, 1])
+@pytest.mark.parametrize("rows,cols", [(2000, 264), (1800, 512), (700, 520), (350, 2560), (301, 5632), (301, 5800),
+                                       (301, 5808), (151, 7168), (151, 7248), (151, 7256), (150, 8192)])
+def test_backward_of_staged_rows(ctx, dtype, gate_rows, rows, cols):
+    """Widths on both sides of what two stages of a row leave room for, with more
+    chunks of rows than an SM holds at a time, and with one."""
+    check_backward(ctx, dtype, rows, cols, gate_rows, 1, 0.7, 1.3)
