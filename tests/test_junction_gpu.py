@@ -369,3 +369,36 @@ def test_backward_of_staged_rows(ctx, dtype, gate_rows, rows, cols):
     """Widths on both sides of what two stages of a row leave room for, with more
     chunks of rows than an SM holds at a time, and with one."""
     check_backward(ctx, dtype, rows, cols, gate_rows, 1, 0.7, 1.3)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols", [40, 264, 1003])
+def test_many_gate_groups(ctx, dtype, cols):
+    """A gate for every two rows of twenty thousand.  Column sums over all rows add
+    a group's two rows, then ceil(groups / 32) partial rows and 32 warps' sums; a
+    gate's gradient its two rows and what one partial row passes."""
+    rows, gate_rows = 20001, 2
+    x = make(dtype, rows, cols, gate_rows, 1, cols)
+    groups = x["gate"].shape[0]
+    assert groups == 10001
+    dh, db = torch.empty_like(x["h"]), torch.empty_like(x["b"])
+    dgp, dgate, dgq = torch.full((cols,), 7.0, device="cuda"), torch.full_like(x["gate"], 7.0), torch.full((cols,), 7.0, device="cuda")
+    bwd(ctx, dtype)(x["h"], x["b"], x["gain_post"], x["gate"], x["gain_pre"], x["dh_out"], x["dy"], dh, db, dgp, dgate,
+                    dgq, rows, cols, gate_rows=gate_rows)
+    ctx.sync()
+    h, b, gp, gate, gq = (wide(x[k]).requires_grad_() for k in ("h", "b", "gain_post", "gate", "gain_pre"))
+    (rms(h, 1e-5) * gq).backward(wide(x["dy"]))
+    dH = wide(x["dh_out"]) + h.grad
+    after(b, gp, gate, rows, gate_rows, 1, 1e-5).backward(dH)
+    at = torch.arange(rows, device="cuda") // gate_rows
+    r = (h.detach().square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+    g = (gq.detach() * wide(x["dy"])).abs()
+    hat = (h.detach() * r).abs()
+    parts = wide(x["dh_out"]).abs() + r * (g + hat * (g * hat).mean(-1, keepdim=True))  # of dH
+    bh = (b.detach() * (b.detach().square().mean(-1, keepdim=True) + 1e-5).rsqrt()).abs()
+    close(dh, dH, parts, ROW)
+    depth = gate_rows + -(-groups // 32) + 32 + 80
+    close(dgp, gp.grad, (gate.detach()[at].abs() * parts * bh).sum(0), depth * STEP)
+    close(dgq, gq.grad, (wide(x["dy"]).abs() * hat).sum(0), depth * STEP)
+    size = torch.zeros_like(gate.detach()).index_add_(0, at, parts * bh * gp.detach().abs())
+    close(dgate, gate.grad, size, (gate_rows + 32 + 80) * STEP)

@@ -459,3 +459,46 @@ def test_sizes_past_31_bits_are_refused(ctx, T, V, D, vocab_major):
             call()
         assert e.value.status == bwpp.ERR_ARG
     ctx.sync()
+
+
+@pytest.mark.parametrize("T,V,D,vocab_major", [(24, 400, 64, 1), (64, 1000, 136, 0), (65, 700, 96, 0), (300, 900, 264, 1)])
+def test_gradient_along_itself_by_differences(ctx, T, V, D, vocab_major):
+    """d sum(dloss loss) along the gradient's own direction, by central differences
+    of the 64-bit formula, is the gradient's norm: a wrong scale, sign or missing
+    term would be off by a large part of it.
+
+    With d = grad / |grad| the sum of terms is |grad|, and an element's error e, at
+    most `step` of the sum of its products' magnitudes, enters as d . e.  Each term
+    of the sum is rounded on its own: by at most `step` of itself, so d . e is at
+    most step * sum over rows and columns of |dlogit| (|d W|) = step * A, A taken
+    in 64 bits.  `step` is half a step of bf16, or of what it leaves up to 64 rows,
+    and twice that bounds the logits' and sums' errors of fp32 size as well (2^-16).
+    The differences are off by the third derivative, 1e-7 of |grad| here."""
+    x, w, target, dloss, xs, ws = make(T, V, D, vocab_major, 23)
+    ldw = ws.shape[1]
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    dx, dw = torch.empty(T, D, device="cuda"), torch.empty(tuple(ws.shape), device="cuda")
+    ctx.xent_fwd(xs, ws, target, loss, lse, T, V, D, D, ldw, w_vocab_major=vocab_major, scale=0.5)
+    ctx.xent_bwd(xs, ws, target, lse, dloss, dx, dw, T, V, D, D, ldw, D, ldw, w_vocab_major=vocab_major, scale=0.5)
+    ctx.sync()
+    dw = dw if vocab_major else dw.t().contiguous()
+    x, w = x.double(), w.double()
+    step = HALF * HALF if T <= 64 else HALF
+
+    def f(x, w):
+        return float((formula(x, w, target, 0.5)[2] * dloss.double()).sum())
+
+    logits, wlse = formula(x, w, target, 0.5)[:2]
+    p = (logits - wlse[:, None]).exp()
+    p[torch.arange(T, device="cuda"), target.long().clamp(min=0)] -= 1.0
+    dlogit = torch.where(target >= 0, dloss.double(), 0.0)[:, None] * p
+    for grad, is_x in ((dx, True), (dw, False)):
+        norm = float(grad.double().norm())
+        d = grad.double() / norm
+        h = 1e-3
+        at = [(x + s * h * d, w) if is_x else (x, w + s * h * d) for s in (1, -1)]
+        num = (f(*at[0]) - f(*at[1])) / (2 * h)
+        each = 0.5 * (d @ w.t() if is_x else x @ d.t())  # the derivative of each logit along d
+        tol = 2 * (step + 2.0**-16) * float((dlogit * each).abs().sum()) + 1e-6 * norm
+        assert abs(num - norm) <= tol, (is_x, num, norm, tol)
+        assert tol <= 0.05 * norm  # the bound says something
