@@ -22,6 +22,8 @@
 // columns in registers, then writes one partial row per chunk.  A second
 // kernel adds the partial rows in a fixed order: dgain_post weights each
 // with its chunk's gate row, dgate adds those of its group.
+#include <atomic>
+
 #include "bwpp_cuda_internal.cuh"
 #include "elem.cuh"
 #include "rowwise.cuh"
@@ -860,13 +862,10 @@ struct Plan {
   uint32_t stages, per_sm, bytes;
 };
 
-// An instantiation of the staged kernel on a device.
-struct StagedFit {
-  bool known;
-  uint32_t by_regs;  // CTAs that an SM's registers and warps hold
-  uint32_t fixed;    // shared memory of a CTA besides what it asks for
-};
-StagedFit g_staged_fit[64][32] = {};
+// An instantiation of the staged kernel on a device: the CTAs that an SM's registers
+// and warps hold, and above 16 bits a CTA's shared memory besides what it asks for.  0: not
+// asked yet.  One word, as contexts on several threads may ask at once.
+std::atomic<uint32_t> g_staged_fit[64][32] = {};
 constexpr uint32_t kSharedOfSm = 228 * 1024, kSharedOfCta = 227 * 1024;  // sm_100: 1 KB of a CTA is the system's
 constexpr uint32_t kSharedUnit = 128;                                   // in which it is given out
 
@@ -888,8 +887,8 @@ int plan_staged(BwppCudaCtx *ctx, uint32_t cols, Plan &g) {
   if (ctx->device >= 64)
     return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "junction: device index >= 64");
   return with_staged<DT, TOKEN>(cols, [&](auto kern, int threads, int id) {
-    StagedFit &fit = g_staged_fit[ctx->device][id];
-    if (!fit.known) {
+    uint32_t fit = g_staged_fit[ctx->device][id].load();
+    if (!fit) {
       cudaFuncAttributes at;
       int n = 0;
       cudaError_t e = cudaFuncGetAttributes(&at, kern);
@@ -899,10 +898,10 @@ int plan_staged(BwppCudaCtx *ctx, uint32_t cols, Plan &g) {
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSharedOfCta - own));
       const int rc = bwpp_check_cuda(ctx, e, "junction smem attribute");
       if (rc) return rc;
-      fit.by_regs = (uint32_t)n;
-      fit.fixed = kSharedOfSm - kSharedOfCta + own;
-      fit.known = true;
+      fit = (uint32_t)n | (kSharedOfSm - kSharedOfCta + own) << 16;
+      g_staged_fit[ctx->device][id].store(fit);
     }
+    const uint32_t by_regs = fit & 0xffffu, fixed = fit >> 16;
     const uint32_t row = cols * (8 + (TOKEN ? 4 : 0) + 2 * (uint32_t)sizeof(typename Elem<DT>::type));
     // 16 warps per SM hide a row's two reductions (32768 x 2048 bf16: 323 us with
     // one CTA of 8 warps, 205 with two, 218 with three, 227 with four; 8192 x 2560
@@ -914,11 +913,11 @@ int plan_staged(BwppCudaCtx *ctx, uint32_t cols, Plan &g) {
     // planned as 12 where 11 fit, 32768 x 512 took 72.5 us, fp32 with a gate per token,
     // where 10 fit, 8000 x 512 33.8 instead of 29.0.
     const uint32_t want = cols <= 512 ? kMaxPerSm : cols <= 1024 ? 4 : cols <= 4096 ? 2 : 1;
-    for (uint32_t per = want < fit.by_regs ? want : fit.by_regs; per >= 1; --per) {
+    for (uint32_t per = want < by_regs ? want : by_regs; per >= 1; --per) {
       // A CTA asks for its whole share of shared memory: one more on an SM would
       // leave another SM with one less, which happens when the kernel in front still
       // holds SMs as these are placed (32768 x 2048 bf16: 263 us instead of 211).
-      const uint32_t bytes = (kSharedOfSm / per & ~(kSharedUnit - 1)) - fit.fixed;
+      const uint32_t bytes = (kSharedOfSm / per & ~(kSharedUnit - 1)) - fixed;
       if (bytes / row < 2) continue;
       g.per_sm = per;
       g.bytes = bytes;
