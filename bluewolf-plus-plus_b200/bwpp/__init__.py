@@ -471,7 +471,7 @@ class Ctx:
 def xent_workspace_size(T, V, D, ldx, ldw, w_vocab_major=0, backward=0, grads_bf16=0) -> int:
     """Scratch bytes of Ctx.xent_fwd (backward=0) or Ctx.xent_bwd (backward=1)."""
     p = XentParams.from_buffer_copy(_XENT.pack(T, V, D, ldx, ldw, 0, 0, int(w_vocab_major),
-                                                    int(grads_bf16), 1.0))
+                                               int(grads_bf16), 1.0))
     return load().bwpp_cuda_xent_workspace_size(C.byref(p), int(backward))
 
 

@@ -402,3 +402,41 @@ def test_many_gate_groups(ctx, dtype, cols):
     close(dgq, gq.grad, (wide(x["dy"]).abs() * hat).sum(0), depth * STEP)
     size = torch.zeros_like(gate.detach()).index_add_(0, at, parts * bh * gp.detach().abs())
     close(dgate, gate.grad, size, (gate_rows + 32 + 80) * STEP)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("gate_rows", [0, 1])
+@pytest.mark.parametrize("cols", [64, 520, 2048, 4104])
+def test_odd_addresses(ctx, dtype, gate_rows, cols):
+    """Each tensor one element off its 16 bytes, in turn, with pitches in eights:
+    what aligned tensors give, up to both sides' errors (2 * ROW and half a step of
+    the type each, of parts that are at most three times the result here), and
+    nothing written around the outputs."""
+    rows = 9
+    x = make(dtype, rows, cols, gate_rows, 1, cols)
+    names = ["h", "b", "gain_post", "gate", "gain_pre", "dh_out", "dy"]
+    outs = {"ho": x["h"], "y": x["b"], "dh": x["h"], "db": x["b"], "dgain_post": x["gain_post"], "dgate": x["gate"],
+            "dgain_pre": x["gain_pre"]}
+
+    def at(like, off):
+        buf = torch.full((like.numel() + 16,), 7.0, device="cuda", dtype=like.dtype)
+        return buf, buf[off:off + like.numel()].view(like.shape)
+
+    def run(odd):
+        t = {k: at(x[k], odd == k)[1].copy_(x[k]) for k in names}
+        o = {k: at(v, odd == k) for k, v in outs.items()}
+        g = {k: v[1] for k, v in o.items()}
+        fwd(ctx, dtype)(t["h"], t["b"], t["gain_post"], t["gate"], t["gain_pre"], g["ho"], g["y"], rows, cols,
+                        gate_rows=gate_rows)
+        bwd(ctx, dtype)(t["h"], t["b"], t["gain_post"], t["gate"], t["gain_pre"], t["dh_out"], t["dy"], g["dh"], g["db"],
+                        g["dgain_post"], g["dgate"], g["dgain_pre"], rows, cols, gate_rows=gate_rows)
+        ctx.sync()
+        for k, (buf, v) in o.items():
+            off = int(odd == k)
+            assert bool((buf[:off] == 7.0).all()) and bool((buf[off + v.numel():] == 7.0).all()), (odd, k)
+        return g
+
+    want = run(None)
+    for odd in names + list(outs):
+        for k, v in run(odd).items():
+            close(v, want[k].double(), want[k].double(), 3 * 2 * (2 * ROW + torch.finfo(v.dtype).eps / 2))
