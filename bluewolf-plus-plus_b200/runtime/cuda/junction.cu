@@ -691,7 +691,9 @@ __global__ void __launch_bounds__(kLoopThreads)
 // Sums of the chunks' partial rows.  blockIdx.x: 0 dgain_post, 1 dgain_pre,
 // 2 + g dgate of group g; blockIdx.y: 32 columns, one per lane.  Warp w adds
 // rows w, w + 32, ... in order, then a thread per column adds the 32 warps'
-// sums in warp order.
+// sums in warp order.  A block per group and 32 columns, however few partial rows the
+// group has: 32768 x 2048 bf16 take 4.7 ms with a gate for every two rows, 1.3 for eight,
+// 0.37 for 64, 0.28 for 2048.
 struct JunctionSums {
   const float *part_post, *part_pre;
   const float *gain_post, *gate;

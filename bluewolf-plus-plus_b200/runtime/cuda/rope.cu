@@ -11,7 +11,8 @@
 // position * fraction mod 2^64 is the angle's fraction of a turn: the whole
 // turns, which carry no information, drop out exactly for any 32-bit position
 // (an fp32 product is 0.03 rad off at position 10^6).  The top 32 bits go to
-// sincospif, whose argument is then within [-1, 1).
+// sincospif, whose argument is then within [-1, 1), rounded to fp32: results are off by
+// 5.5e-8 of their norm, 4.2e-8 with 64-bit angles.
 #include <math.h>
 
 #include "bwpp_cuda_internal.cuh"
