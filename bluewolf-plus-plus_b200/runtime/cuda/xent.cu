@@ -453,6 +453,7 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     px.c = to_user ? dx : static_cast<void *>(scratch + l.dx);
     px.ldc = to_user ? p.lddx : l.dp;
     px.bf16 = to_user && last && p.grads_bf16;
+    px.guarded = to_user;
     px.factor = to_user && last ? common : nullptr;
     uint8_t *user_w =
         dw ? static_cast<uint8_t *>(dw) + (vm ? (size_t)v0 * p.lddw : (size_t)v0) * es : nullptr;
@@ -462,6 +463,7 @@ int bwpp_cuda_xent_bwd_bf16(BwppCudaCtx *ctx, const uint16_t *x, const uint16_t 
     pw.c = own_w ? static_cast<void *>(scratch + l.dw) : static_cast<void *>(user_w);
     pw.ldc = own_w ? (vm ? l.dp : piece) : p.lddw;
     pw.bf16 = p.grads_bf16 && dw_parts == 1;
+    pw.guarded = !own_w;
     pw.factor = dw_parts == 1 ? common : nullptr;
     rc = bwpp_xent_grad_launch(ctx, dx ? &px : nullptr, dw ? &pw : nullptr, dx_parts, dw_parts);
     if (!rc && dw && dw_parts > 1)

@@ -45,6 +45,7 @@ struct XentProduct {
   uint32_t M, N, K, lda, ldb, ldc;
   bool a_mn, b_mn;
   bool bf16;          // C bf16, else fp32
+  bool guarded;       // what lies behind C's N columns is not to be written
   const float *factor; // device scalar that multiplies C, or NULL
   bool accumulate;    // add fp32 rows `add` (pitch ld_add; may be C)
   const void *add;

@@ -57,6 +57,10 @@ struct Product {
   uint32_t ld_add;
   const float *factor;      // multiplies C, or NULL
   uint32_t bf16;            // C is bf16, else fp32
+  // TMA stores a row up to a multiple of 16 bytes, behind its last column as well:
+  // it takes the columns below `whole`, and the few from there on are stored as they are
+  uint32_t whole, ldc;
+  void *c;
 };
 
 struct Maps {
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       uint32_t mb, nb, part, kb0, kb1;
       item_at(p, i, mb, nb, part, kb0, kb1);
       const bool out16 = p.bf16 != 0;
-      const uint32_t M = p.M, N = p.N;
+      const uint32_t M = p.M, N = p.N, whole = p.whole;
       const CUtensorMap *mc = &work.maps[which].c;
       const uint32_t cw = out16 ? 64 : 32;  // columns of 128 bytes
       const uint32_t row0 = mb * C::TILE_M + rank * BM + q * 32, row = row0 + lane;
@@ -361,9 +365,26 @@ __global__ void __launch_bounds__(THREADS, 1)
               make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0 && row0 < M) {
+        if (lane == 0 && row0 < M && c0 < whole) {
           tma_store_2d(mc, stage_c, (int32_t)c0, (int32_t)out_row);
           tma_store_commit();
+        }
+      }
+      // the columns from `whole` on: in one 16-byte piece of each row, and in this warp's
+      // last chunk if in one of its chunks, so they are still staged
+      const uint32_t at = whole - nb * BN;
+      if (whole < N && at < BN && (at / cw & 1) == (uint32_t)sub && row < M) {
+        const uint32_t j = at % cw / (out16 ? 8 : 4);
+        const uint4 t = *reinterpret_cast<const uint4 *>(stage_c + lane * 128 + ((j ^ (lane & 7)) << 4));
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+        const size_t to = (size_t)(out_row + lane) * p.ldc + whole;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+          if (whole + e >= N) break;
+          if (out16)
+            static_cast<uint16_t *>(p.c)[to + e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+          else if (e < 4)
+            static_cast<float *>(p.c)[to + e] = __uint_as_float(w[e]);
         }
       }
       tc_fence_before();
@@ -521,16 +542,21 @@ int make_product(BwppCudaCtx *ctx, const XentProduct &s, uint32_t tile_m, uint32
   p.ld_add = s.ld_add;
   p.factor = s.factor;
   p.bf16 = s.bf16 ? 1 : 0;
+  const uint32_t unit = s.bf16 ? 8 : 4;  // columns of 16 bytes
+  p.whole = s.guarded ? s.N / unit * unit : s.N;
+  p.ldc = s.ldc;
+  p.c = s.c;
   const uint64_t items = (uint64_t)p.tiles_m * p.tiles_n * parts;
   if (items >= 0x80000000ull) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "xent: too many tiles");
   p.items = (uint32_t)items;
   int rc = operand_map(ctx, &m.a, s.a, s.a_mn, s.M, s.K, s.lda, BM);
   if (!rc) rc = operand_map(ctx, &m.b, s.b, s.b_mn, s.N, s.K, s.ldb, 64);
   const uint64_t rows = parts > 1 ? (uint64_t)parts * s.part_rows : s.M;
+  const uint32_t cols = p.whole ? p.whole : unit;  // without whole pieces the map is not used
   if (!rc)
-    rc = s.bf16 ? bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s.N, rows,
+    rc = s.bf16 ? bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cols, rows,
                                     (uint64_t)s.ldc * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B)
-                : bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, s.N, rows,
+                : bwpp_make_tmap_2d(ctx, &m.c, s.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, cols, rows,
                                     (uint64_t)s.ldc * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
   return rc;
 }

@@ -502,3 +502,13 @@ def test_gradient_along_itself_by_differences(ctx, T, V, D, vocab_major):
         tol = 2 * (step + 2.0**-16) * float((dlogit * each).abs().sum()) + 1e-6 * norm
         assert abs(num - norm) <= tol, (is_x, num, norm, tol)
         assert tol <= 0.05 * norm  # the bound says something
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("vocab_major", [0, 1])
+@pytest.mark.parametrize("T,V,D,pad", [(194, 37, 77, 3), (743, 1, 1, 7), (3, 999, 127, 1), (300, 2099, 83, 5), (500, 258, 66, 6),
+                                       (1500, 1284, 516, 4), (130, 1, 1001, 7), (9000, 9003, 67, 5)])
+def test_padding_of_rows_that_end_inside_16_bytes(ctx, T, V, D, pad, vocab_major, bf16):
+    """Pitches that TMA takes, rows that are no multiple of 16 bytes: what lies
+    behind a row is not the gradient's."""
+    check(ctx, T, V, D, vocab_major, bf16=bf16, pad=pad)
