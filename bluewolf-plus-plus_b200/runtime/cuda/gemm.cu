@@ -98,6 +98,11 @@ struct GemmEpi {
   // 1: the residual operand multiplies instead of adding (the gate of a
   // SwiGLU: silu(A B + bias) * R)
   int res_mul;
+  // C, for what its tensor map does not take.  TMA stores a row up to a multiple of
+  // 16 bytes, behind its last column as well: it takes the columns below `whole`,
+  // the few from there on are stored as they are.
+  void *c;
+  uint32_t ldc, whole;
   };
 
 // Work of a launch, handed out round-robin to `workers` workers (CTA pairs,
@@ -199,7 +204,9 @@ __device__ __forceinline__ bool get_item(const GemmWork &w, uint32_t tiles_m, ui
   return true;
 }
 
-template <bool A_MN, bool B_MN, bool PAIR>
+// RAGGED: C's rows end inside 16 bytes (see GemmEpi::whole).  A kernel of its own:
+// with the case in all of them, 300 x 32000 x 1024 took 45.0 us instead of 43.9.
+template <bool A_MN, bool B_MN, bool PAIR, bool RAGGED>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA,
                    const __grid_constant__ CUtensorMap tmB,
@@ -757,9 +764,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                 make_uint4(outw[4 * j], outw[4 * j + 1], outw[4 * j + 2], outw[4 * j + 3]);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && row0 < M) {
+          if (lane == 0 && row0 < M && (!RAGGED || col0 < epi.whole)) {
             tma_store_2d(&tmC, sc, (int32_t)col0, (int32_t)row0);
             tma_store_commit();
+          }
+        }
+        if constexpr (RAGGED) {
+          // the columns from `whole` on: in one 16-byte piece of each row, and if they
+          // are in one of these chunks, in the last one, which is still staged
+          const uint32_t at =
+              epi.whole - (first_col + (uint32_t)(sub + 2 * (cls + (own_chunks - 1) * parts)) * cw);
+          if (own_chunks > 0 && at < (uint32_t)cw && my_row < M) {
+            const uint32_t es = out16 ? 2 : 4;
+            const uint8_t *from = stage_c + lane * 128 + (((at * es / 16) ^ (lane & 7)) << 4);
+#pragma unroll 1
+            for (uint32_t col = epi.whole; col < N; ++col, from += es) {
+              const size_t to = (size_t)my_row * epi.ldc + col;
+              if (out16) static_cast<uint16_t *>(epi.c)[to] = *reinterpret_cast<const uint16_t *>(from);
+              else static_cast<float *>(epi.c)[to] = *reinterpret_cast<const float *>(from);
+            }
           }
         }
         if (depth) cp_async_wait_pending(0);  // the ring is reused by the next class
@@ -855,8 +878,8 @@ __global__ void cast_f32_bf16_kernel(const float *__restrict__ src,
   }
 }
 
-bool g_attr_set[8][64] = {};
-int g_pair_clusters[4][64] = {};  // resident CTA pairs per device (0: not queried)
+bool g_attr_set[16][64] = {};
+int g_pair_clusters[8][64] = {};  // resident CTA pairs per device (0: not queried)
 
 inline bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -924,22 +947,22 @@ bool split_first_enabled() {
 // waves; the 24-tile tail runs as 3 x 24 third-tiles in one round.)  When
 // no split applies (a tail of more than half a round, under 8 K blocks, or
 // no scratch), a tail that fits twice into one round runs as N halves.
-template <bool A_MN, bool B_MN, bool PAIR>
+template <bool A_MN, bool B_MN, bool PAIR, bool RAGGED>
 int launch_tc(BwppCudaCtx *ctx, const CUtensorMap &ta, const CUtensorMap &tb,
               const CUtensorMap &tcm, const GemmEpi &epi, uint32_t M, uint32_t N,
               uint32_t K, uint32_t ab_f16) {
   using Cfg = GemmCfg<PAIR>;
-  auto kern = gemm_tc_kernel<A_MN, B_MN, PAIR>;
-  const int v = (A_MN ? 2 : 0) + (B_MN ? 1 : 0);
+  auto kern = gemm_tc_kernel<A_MN, B_MN, PAIR, RAGGED>;
+  const int v = (A_MN ? 2 : 0) + (B_MN ? 1 : 0) + (RAGGED ? 4 : 0);
   const int dev = ctx->device;
   if (dev >= 64) return bwpp_set_error(ctx, BWPP_CUDA_ERR_UNSUPPORTED, "gemm: device index >= 64");
-  if (!g_attr_set[v + (PAIR ? 4 : 0)][dev]) {
+  if (!g_attr_set[v + (PAIR ? 8 : 0)][dev]) {
     int rc = bwpp_check_cuda(ctx,
                              cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                   Cfg::SMEM_ALLOC),
                              "gemm smem attribute");
     if (rc) return rc;
-    g_attr_set[v + (PAIR ? 4 : 0)][dev] = true;
+    g_attr_set[v + (PAIR ? 8 : 0)][dev] = true;
   }
   const uint32_t tiles = ((M + Cfg::TILE_M - 1) / Cfg::TILE_M) * ((N + BN - 1) / BN);
   cudaLaunchAttribute attr[1];
@@ -1009,15 +1032,27 @@ int launch_tc(BwppCudaCtx *ctx, const CUtensorMap &ta, const CUtensorMap &tb,
       PAIR ? "gemm tcgen05 pair" : "gemm tcgen05");
 }
 
-template <bool A_MN, bool B_MN>
+template <bool A_MN, bool B_MN, bool RAGGED>
 int launch_tc_any(BwppCudaCtx *ctx, const CUtensorMap &ta, const CUtensorMap &tb,
                   const CUtensorMap &tcm, const GemmEpi &epi,
                   uint32_t M, uint32_t N, uint32_t K, bool pair, uint32_t ab_f16) {
   if (pair) {
-    const int rc = launch_tc<A_MN, B_MN, true>(ctx, ta, tb, tcm, epi, M, N, K, ab_f16);
+    const int rc = launch_tc<A_MN, B_MN, true, RAGGED>(ctx, ta, tb, tcm, epi, M, N, K, ab_f16);
     if (rc != BWPP_CUDA_ERR_UNSUPPORTED) return rc;
   }
-  return launch_tc<A_MN, B_MN, false>(ctx, ta, tb, tcm, epi, M, N, K, ab_f16);
+  return launch_tc<A_MN, B_MN, false, RAGGED>(ctx, ta, tb, tcm, epi, M, N, K, ab_f16);
+}
+
+template <bool RAGGED>
+int launch_tc_layout(BwppCudaCtx *ctx, const CUtensorMap &ta, const CUtensorMap &tb,
+                     const CUtensorMap &tcm, const GemmEpi &epi, uint32_t M, uint32_t N, uint32_t K,
+                     bool pair, uint32_t ab_f16, bool a_mn, bool b_mn) {
+  if (a_mn) {
+    return b_mn ? launch_tc_any<true, true, RAGGED>(ctx, ta, tb, tcm, epi, M, N, K, pair, ab_f16)
+                : launch_tc_any<true, false, RAGGED>(ctx, ta, tb, tcm, epi, M, N, K, pair, ab_f16);
+  }
+  return b_mn ? launch_tc_any<false, true, RAGGED>(ctx, ta, tb, tcm, epi, M, N, K, pair, ab_f16)
+              : launch_tc_any<false, false, RAGGED>(ctx, ta, tb, tcm, epi, M, N, K, pair, ab_f16);
 }
 
 }  // namespace
@@ -1039,7 +1074,11 @@ int bwpp_gemm_launch_dt(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint32_t 
   // makes the residual a multiplier
   GemmEpi epi{bias, residual, ldr, silu ? 1 : 0, out_bf16 ? 1 : 0, out_f16 ? 1 : 0, res16 & 3};
   epi.res_mul = (res16 >> 2) & 1;
-  const uint32_t out_es = out_bf16 ? 2 : 4;
+  const uint32_t out_es = out_bf16 ? 2 : 4, unit = 16 / out_es;  // unit: columns of 16 bytes
+  epi.c = c;
+  epi.ldc = ldc;
+  epi.whole = N / unit * unit;
+  const uint32_t map_cols = epi.whole ? epi.whole : unit;  // without whole pieces the map is not used
   const bool tc_ok = !force_simt && K > 0 && al16(a) && al16(b) && al16(c) &&
                      (lda % 8) == 0 && (ldb % 8) == 0 && ((ldc * out_es) % 16) == 0 &&
                      (!bias || al16(bias));
@@ -1065,17 +1104,13 @@ int bwpp_gemm_launch_dt(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint32_t 
     rc = b_mn ? bwpp_make_tmap_2d(ctx, &tb, b, BF, N, K, (uint64_t)ldb * 2, 64, BK, SW)
               : bwpp_make_tmap_2d(ctx, &tb, b, BF, K, N, (uint64_t)ldb * 2, BK, 64, SW);
   if (!rc)
-    rc = out_bf16 ? bwpp_make_tmap_2d(ctx, &tcm, c, OUT16, N, M, (uint64_t)ldc * 2, 64, 32, SW)
-                  : bwpp_make_tmap_2d(ctx, &tcm, c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, N, M,
+    rc = out_bf16 ? bwpp_make_tmap_2d(ctx, &tcm, c, OUT16, map_cols, M, (uint64_t)ldc * 2, 64, 32, SW)
+                  : bwpp_make_tmap_2d(ctx, &tcm, c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, map_cols, M,
                                       (uint64_t)ldc * 4, EPI_COLS, 32, SW);
   if (rc) return rc;
   const uint32_t f = ab_f16 ? 1u : 0u;
-  if (a_mn) {
-    return b_mn ? launch_tc_any<true, true>(ctx, ta, tb, tcm, epi, M, N, K, pair, f)
-                : launch_tc_any<true, false>(ctx, ta, tb, tcm, epi, M, N, K, pair, f);
-  }
-  return b_mn ? launch_tc_any<false, true>(ctx, ta, tb, tcm, epi, M, N, K, pair, f)
-              : launch_tc_any<false, false>(ctx, ta, tb, tcm, epi, M, N, K, pair, f);
+  return epi.whole < N ? launch_tc_layout<true>(ctx, ta, tb, tcm, epi, M, N, K, pair, f, a_mn, b_mn)
+                       : launch_tc_layout<false>(ctx, ta, tb, tcm, epi, M, N, K, pair, f, a_mn, b_mn);
 }
 
 // d(gate | up) of a SwiGLU from the product d(a) = A B (M x F), fused into the
@@ -1096,6 +1131,9 @@ int bwpp_gemm_launch_glu_bwd(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint
   epi.glu_up_out = dgu + F;
   epi.ldglu = ldgu;
   epi.glu_F = F;
+  epi.c = dgu;
+  epi.ldc = ldgu;
+  epi.whole = F;
   const bool pair = pairs_enabled() && M > (uint32_t)BM;
   CUtensorMap ta, tb, tcm;
   const auto BF = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -1107,12 +1145,7 @@ int bwpp_gemm_launch_glu_bwd(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint
               : bwpp_make_tmap_2d(ctx, &tb, b, BF, K, F, (uint64_t)ldb * 2, BK, 64, SW);
   if (!rc) rc = bwpp_make_tmap_2d(ctx, &tcm, dgu, BF, F, M, (uint64_t)ldgu * 2, 64, 32, SW);
   if (rc) return rc;
-  if (a_mn) {
-    return b_mn ? launch_tc_any<true, true>(ctx, ta, tb, tcm, epi, M, F, K, pair, 0)
-                : launch_tc_any<true, false>(ctx, ta, tb, tcm, epi, M, F, K, pair, 0);
-  }
-  return b_mn ? launch_tc_any<false, true>(ctx, ta, tb, tcm, epi, M, F, K, pair, 0)
-              : launch_tc_any<false, false>(ctx, ta, tb, tcm, epi, M, F, K, pair, 0);
+  return launch_tc_layout<false>(ctx, ta, tb, tcm, epi, M, F, K, pair, 0, a_mn, b_mn);
 }
 
 int bwpp_gemm_launch_ex(BwppCudaCtx *ctx, const uint16_t *a, int a_mn, uint32_t lda,

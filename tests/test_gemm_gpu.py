@@ -390,3 +390,37 @@ def test_split_tiles_with_residual_and_16bit_out(ctx, out_bf16):
                     ldr=N)
         ctx.sync()
         assert rel_fro(host(cd), ref) <= TIGHT
+
+
+@pytest.mark.parametrize("out_bf16", [0, 1])
+@pytest.mark.parametrize("a_mn,b_mn", [(0, 1), (0, 0), (1, 1)])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 64), (130, 7, 72), (300, 261, 1000), (256, 1037, 4096), (700, 515, 2048),
+                                   (1000, 5002, 520), (129, 2059, 64)])
+def test_rows_that_end_inside_16_bytes(ctx, M, N, K, a_mn, b_mn, out_bf16):
+    """A pitch that TMA takes and a width that is no multiple of 16 bytes: the
+    padding of C stays untouched, and C ends with its last row's last column."""
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    up8 = lambda n: -(-n // 8) * 8  # noqa: E731
+    lda, ldb, ldc = up8(M if a_mn else K), up8(N if b_mn else K), up8(N) + 8
+    a = torch.randn(K if a_mn else M, lda, device="cuda", generator=g).bfloat16()
+    b = torch.randn(K if b_mn else N, ldb, device="cuda", generator=g).bfloat16()
+    bias = torch.randn(up8(N), device="cuda", generator=g)
+    residual = torch.randn(M, N + 3, device="cuda", generator=g)
+    t = torch.bfloat16 if out_bf16 else torch.float32
+    whole = torch.full(((M - 1) * ldc + N + 64,), 7.0, device="cuda", dtype=t)
+    ctx.gemm_ex(a, b, whole, M, N, K, lda, ldb, ldc, a_mn=a_mn, b_mn=b_mn, out_bf16=out_bf16, bias=bias,
+                residual=residual, ldr=N + 3)
+    ctx.sync()
+    af = (a[:, :M].t() if a_mn else a[:, :K]).double()
+    bf = (b[:, :N] if b_mn else b[:, :K].t()).double()
+    want = af @ bf + bias[:N].double() + residual[:, :N].double()
+    assert bool((whole[(M - 1) * ldc + N:] == 7.0).all())
+    c = torch.as_strided(whole, (M, N), (ldc, 1))
+    gap = torch.as_strided(whole, (M - 1, ldc - N), (ldc, 1), N)
+    assert bool((gap == 7.0).all())
+    # TIGHT for the sums, and half a step of bf16 where C is rounded to it
+    assert float((c.double() - want).norm() / want.norm()) <= TIGHT + (2.0**-8 if out_bf16 else 0.0)
+    # no single column is wrong: the last ones are stored apart.  K / 16 additions, each
+    # off by at most 2^-22 of the sum of magnitudes, and a few for bias and residual
+    size = af.abs() @ bf.abs() + bias[:N].double().abs() + residual[:, :N].double().abs()
+    assert bool(((c.double() - want).abs() <= 2.0**-18 * size * (1 + K / 256) + (2.0**-8 * want.abs() if out_bf16 else 0.0)).all())
